@@ -55,6 +55,12 @@ enum {
     IQK_BF16 = 2
 };
 
+/* How the router scores logits. */
+enum {
+    IQK_SOFTMAX = 0,
+    IQK_SIGMOID = 1
+};
+
 /* Status codes. The Python layer maps them onto the reference's exception
  * classes: IqkFormatError (MEMBER), IqkKernelError (WIDTH, GEOMETRY) and
  * IqkRuntimeError (the rest) -- src/mlx_iqk/format.py:265,
@@ -419,6 +425,115 @@ int iqk_dense_dequant(int member, const void *const *streams, int64_t out_featur
 int iqk_dense_gemv(int member, const void *x, int64_t tokens, const void *const *streams,
                    int64_t out_features, int64_t in_features, void *y, int y_dtype,
                    iqk_stream_t stream);
+
+/*
+ * Expert router (no reference counterpart: the reference is handed indices
+ * and scores, src/mlx_iqk/nn.py:1-22).
+ *
+ * logits [tokens, num_experts] in f32, f16 or bf16, row_stride elements from
+ * row to row; num_experts at most 1024, top_k at most 32 and num_experts.
+ * mask (or NULL) holds one byte per token, 0 for a row to leave out.
+ *
+ * iqk_route: indices [tokens, top_k] int32, the largest logits in falling
+ * order (ties: the lowest index; NaN counts as largest), and weights
+ * [tokens, top_k] f32, scale times the scores (softmax over the experts, or
+ * sigmoid) of the chosen, divided by their sum when renormalize is not 0. A
+ * logit of -inf is no expert: a row that has fewer than top_k others, or
+ * that the mask leaves out, gets index -1 with weight 0 in the places left.
+ *
+ * iqk_route_balanced: the same choice, and per segment g the rows that chose
+ * each expert, counts [segments, num_experts], and the balance loss
+ *   loss = mean over segments with rows of sum_e f_ge P_ge,
+ *   f_ge = num_experts count_ge / (top_k N_g),  P_ge = mean over rows of s_te,
+ * s_te the score normalised over the experts and N_g the segment's rows that
+ * the mask keeps. offsets [segments + 1] int32 on the device (not falling,
+ * from 0 to tokens) cuts the rows into segments; NULL is one segment. With
+ * weights NULL the choice is the caller's: indices is read, entries outside
+ * [0, num_experts) count for no expert. slope [segments, num_experts] is kept
+ * for the backward call. workspace: iqk_balance_workspace_bytes. Sums are
+ * joined in a fixed order: results repeat bit for bit.
+ *
+ * iqk_route_backward: grad_logits [tokens, num_experts] (the logits' type,
+ * contiguous) from the gradient of the weights (grad_weights [tokens, top_k],
+ * with the call's indices) and of the loss (the forward's slope, and one f32
+ * at grad_loss); either may be NULL.
+ */
+int iqk_route(const void *logits, int dtype, int64_t tokens, int64_t num_experts,
+              int64_t row_stride, const uint8_t *mask, int top_k, int scoring, int renormalize,
+              float scale, int32_t *indices, float *weights, iqk_stream_t stream);
+
+size_t iqk_balance_workspace_bytes(int64_t tokens, int64_t num_experts, int64_t segments);
+
+int iqk_route_balanced(const void *logits, int dtype, int64_t tokens, int64_t num_experts,
+                       int64_t row_stride, const uint8_t *mask, const int32_t *offsets,
+                       int64_t segments, int top_k, int scoring, int renormalize, float scale,
+                       int32_t *indices, float *weights, float *loss, int32_t *counts,
+                       float *slope, void *workspace, size_t workspace_bytes,
+                       iqk_stream_t stream);
+
+int iqk_route_backward(const void *logits, int dtype, int64_t tokens, int64_t num_experts,
+                       int64_t row_stride, const uint8_t *mask, const int32_t *offsets,
+                       int64_t segments, int top_k, int scoring, int renormalize, float scale,
+                       const int32_t *indices, const float *grad_weights, const float *slope,
+                       const float *grad_loss, void *grad_logits, iqk_stream_t stream);
+
+/*
+ * MXFP4 (OCP Microscaling Formats 1.0): 32 consecutive values of a row share
+ * one E8M0 scale 2^(byte - 127); each value is an E2M1 code (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 and their negatives). No reference counterpart: its formats are
+ * integer codes with float scales.
+ *
+ *   codes  [rows, width / 2]  two codes a byte, the even column in the low
+ *                             nibble; rows packed, 16-byte aligned
+ *   scales [rows, width / 32] scale_stride bytes from row to row, a multiple
+ *                             of 16; 16-byte aligned
+ *
+ * width is a multiple of 32.
+ *
+ * iqk_mx_quantize: x [rows, width] (f32, f16 or bf16, row_stride elements
+ * from row to row) to codes and scales. The scale is 2^(floor(log2 m) - 2), m
+ * the block's largest magnitude (2^-127 at least); values round to the nearest
+ * code, ties to the even one, beyond 6 to 6. A block that holds a NaN or an
+ * infinity gets scale byte 255, which makes all of it NaN.
+ *
+ * iqk_mx_dequantize: the values, exact in f32, rounded once to f16 or bf16;
+ * out [rows, width] contiguous.
+ *
+ * iqk_mx_linear: y [rows, out_features] = q(x) W^T, q the quantisation above,
+ * products and sums in f32, rounded once to y's type. W is codes and scales
+ * [out_features, width]. workspace: iqk_mx_workspace_bytes(rows, 1, width,
+ * out_features).
+ *
+ * iqk_mx_routed: y [pairs, out_features], y[p] = q(x[r(p)]) W[sel[p]]^T over
+ * stacked matrices (codes and scales [num_experts, out_features, width],
+ * packed over the experts), r(p) = p / (pairs / x_rows) (one row for the
+ * top_k pairs of a token, or one row per pair). sel -1 is no expert: its row
+ * of y is zeros. Another index outside [0, num_experts) also gives zeros, and
+ * sets IQK_DEVERR_EXPERT in the workspace (iqk_mx_read_error, which
+ * synchronises the stream). At most 4096 experts and 2^24 pairs.
+ */
+int iqk_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width, int64_t row_stride,
+                    uint8_t *codes, uint8_t *scales, int64_t scale_stride, iqk_stream_t stream);
+
+int iqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+                      int64_t rows, int64_t width, void *out, int out_dtype,
+                      iqk_stream_t stream);
+
+size_t iqk_mx_workspace_bytes(int64_t pairs, int64_t num_experts, int64_t width,
+                              int64_t out_features);
+
+int iqk_mx_linear(const void *x, int x_dtype, int64_t rows, int64_t row_stride,
+                  const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+                  int64_t out_features, int64_t width, void *y, int y_dtype, void *workspace,
+                  size_t workspace_bytes, iqk_stream_t stream);
+
+int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride,
+                  const int32_t *sel, int64_t pairs, const uint8_t *codes,
+                  const uint8_t *scales, int64_t scale_stride, int64_t num_experts,
+                  int64_t out_features, int64_t width, void *y, int y_dtype, void *workspace,
+                  size_t workspace_bytes, iqk_stream_t stream);
+
+int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream);
 
 #ifdef __cplusplus
 }

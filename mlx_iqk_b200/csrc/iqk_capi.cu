@@ -4,35 +4,20 @@
 // any launch (the reference fails closed the same way before compiling:
 // src/mlx_iqk/kernels.py:100-128, src/mlx_iqk/nn.py:110-126) and returns a
 // status instead of raising.
-#include <atomic>
 #include <cstdio>
 
 #include "iqk_common.cuh"
 #include "iqk_gemv.cuh"
 #include "iqk_dense.cuh"
 #include "iqk_grouped.cuh"
+#include "iqk_host.cuh"
 
 namespace {
 
 using namespace iqk;
 
 bool member_ok(int m) { return m == IQK_IQ2_KS || m == IQK_IQ2_K || m == IQK_IQ1_S_R4; }
-bool dtype_ok(int d) { return d == IQK_F32 || d == IQK_F16 || d == IQK_BF16; }
 bool width_ok(int64_t n) { return n == 2048 || n == 4096; }
-bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
-// SM count of the current device, queried once per device.
-int num_sms_current() {
-    static std::atomic<int> cached[64];
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-    if (dev >= 0 && dev < 64 && (sms = cached[dev].load()) > 0) return sms;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-        sms = 148;
-    if (dev >= 0 && dev < 64) cached[dev].store(sms);
-    return sms;
-}
-
 // Stream pointers: present, and 16-byte aligned (the kernels move them with
 // 16-byte copies; the caller's allocator gives 256).
 int check_streams(int member, const void *const *streams) {
@@ -61,12 +46,6 @@ int check_dense_streams(int member, const void *const *streams) {
         if (!aligned(streams[i], 16)) return IQK_ERR_ALIGNMENT;
     }
     return IQK_OK;
-}
-
-int cuda_status(cudaError_t err) {
-    if (err == cudaSuccess) return IQK_OK;
-    cudaGetLastError();  // clear a sticky launch error for the caller
-    return IQK_ERR_CUDA;
 }
 
 }  // namespace

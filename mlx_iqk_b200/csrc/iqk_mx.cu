@@ -1,0 +1,366 @@
+// MXFP4 quantisation and its inverse, and the entry points of the MXFP4
+// products (sm_100a).
+//
+// A block is 32 consecutive values of a row. With m its largest magnitude,
+//
+//   scale = 2^max(floor(log2 m) - 2, -127),  code = round(v / scale) to E2M1
+//
+// so the largest value lands in [4, 8). Both steps are exact up to the one
+// rounding: floor(log2 m) is m's exponent field, dividing by a power of two
+// changes no digit, and cvt.rn.satfinite.e2m1x2 rounds to nearest even and
+// holds what lies beyond 6 at 6. A NaN or an infinity has the largest exponent
+// field, so the maximum of the magnitudes' bit patterns finds it, and the
+// block's scale byte is 255 (NaN).
+//
+// Both kernels are bound by HBM: four threads a block, eight values each, in
+// 16-byte accesses.
+#include "iqk_host.cuh"
+#include "iqk_mx.cuh"
+
+namespace iqk {
+namespace {
+
+// Eight consecutive values as f32.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    if constexpr (!WIDE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j]);
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0];
+        const float4 b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(e[j]);
+    }
+}
+
+// Two values to two codes, `lo` in the low nibble.
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8], float inv) {
+    uint32_t r;
+    asm("{\n .reg .b8 a, b, c, d;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        " mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(r)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv),
+          "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+    return r;
+}
+
+// The scale byte of a block whose magnitudes' largest bit pattern is `amax`,
+// and the factor that its values are multiplied with.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax, float &inv) {
+    const uint32_t field = amax >> 23;  // floor(log2) + 127; 255: NaN or infinity
+    const uint32_t byte = field <= 2u ? 0u : field - 2u;
+    inv = __uint_as_float((254u - byte) << 23);
+    return field == 255u ? 255u : byte;
+}
+
+// Row r of the output is row r of x, or with `order` row order[r] / per_row
+// (a pair's activation row) for the first *count of them.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256)
+mx_quantize_kernel(const T *__restrict__ x, int64_t rows, int64_t width, int64_t row_stride,
+                   uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
+                   int64_t scale_stride, const int32_t *__restrict__ order,
+                   const int32_t *__restrict__ count, int64_t per_row) {
+    const int64_t per = width / 8;  // threads of a row
+    const int64_t all = (order ? (int64_t)*count : rows) * per;
+    // whole groups of four lanes run or stop together: `per` is a multiple of 4
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / per, c = i % per;
+        const int64_t src = order ? order[r] / per_row : r;
+        float v[8];
+        load8<T, WIDE>(x + src * row_stride + c * 8, v);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+        const unsigned group = 0xfu << (threadIdx.x & 28u);
+        amax = max(amax, __shfl_xor_sync(group, amax, 1));
+        amax = max(amax, __shfl_xor_sync(group, amax, 2));
+        float inv;
+        const uint32_t byte = scale_byte(amax, inv);
+        *reinterpret_cast<uint32_t *>(codes + r * (width / 2) + c * 4) = codes8(v, inv);
+        if ((c & 3) == 0) scales[r * scale_stride + c / 4] = (uint8_t)byte;
+    }
+}
+
+// 2^(byte - 127); 255 is NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    if (byte == 255u) return __uint_as_float(0x7fffffffu);
+    return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+
+__device__ __forceinline__ float code_value(uint32_t code) {
+    // {0, 1, 2, 3, 4, 6, 8, 12} halves: 4-bit entries of one word
+    const float size = 0.5f * (float)((0xC8643210u >> (4 * (code & 7u))) & 15u);
+    return (code & 8u) ? -size : size;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                     int64_t scale_stride, int64_t rows, int64_t width, T *__restrict__ out) {
+    const int64_t per = width / 8, all = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / per, c = i % per;
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + r * (width / 2) + c * 4);
+        const float s = scale_value(scales[r * scale_stride + c / 4]);
+        T v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = from_float<T>(code_value((w >> (4 * j)) & 15u) * s);
+        uint4 *dst = reinterpret_cast<uint4 *>(out + r * width + c * 8);
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+            dst[j] = reinterpret_cast<const uint4 *>(v)[j];
+    }
+}
+
+// Pairs by expert: one block counts, cuts each expert's run into tiles of at
+// most L.cap rows and scatters the pairs; those without an expert go to the
+// tail. The order of an expert's pairs changes no result: each is a row of
+// its own.
+__global__ void __launch_bounds__(1024)
+mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLayout L,
+               char *ws) {
+    extern __shared__ int32_t cnt[];
+    __shared__ int32_t warp_rows[32], warp_tiles[32], bad, tail;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, wid = tid >> 5;
+    int32_t *hdr = reinterpret_cast<int32_t *>(ws + L.hdr);
+    int32_t *order = reinterpret_cast<int32_t *>(ws + L.order);
+    int4 *tiles = reinterpret_cast<int4 *>(ws + L.tiles);
+    for (int e = tid; e < num_experts; e += nt) cnt[e] = 0;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    for (int p = tid; p < pairs; p += nt) {
+        const int e = sel[p];
+        if (e >= 0 && e < num_experts) atomicAdd(&cnt[e], 1);
+        else if (e != -1) bad = IQK_DEVERR_EXPERT;
+    }
+    __syncthreads();
+    // exclusive sums of rows and tiles over the experts, `per` a thread
+    const int per = (num_experts + nt - 1) / nt;
+    const int e0 = min(tid * per, num_experts), e1 = min(e0 + per, num_experts);
+    int rows = 0, made = 0;
+    for (int e = e0; e < e1; ++e) {
+        rows += cnt[e];
+        made += (cnt[e] + L.cap - 1) / L.cap;
+    }
+    int at = rows, tile = made;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, at, o), b = __shfl_up_sync(0xffffffffu, tile, o);
+        if (lane >= o) at += a, tile += b;
+    }
+    if (lane == 31) warp_rows[wid] = at, warp_tiles[wid] = tile;
+    __syncthreads();
+    at -= rows, tile -= made;
+    int all_rows = 0, all_tiles = 0;
+    for (int w = 0; w < (nt >> 5); ++w) {
+        if (w == wid) at += all_rows, tile += all_tiles;
+        all_rows += warp_rows[w], all_tiles += warp_tiles[w];
+    }
+    for (int e = e0; e < e1; ++e) {
+        const int c = cnt[e];
+        for (int i = 0; i < c; i += L.cap)
+            tiles[tile++] = make_int4(e, at + i, min(L.cap, c - i), 0);
+        cnt[e] = at;
+        at += c;
+    }
+    if (tid == 0) {
+        hdr[0] = bad;
+        hdr[1] = all_tiles;
+        hdr[2] = all_rows;
+        tail = all_rows;
+    }
+    __syncthreads();
+    for (int p = tid; p < pairs; p += nt) {
+        const int e = sel[p];
+        order[e >= 0 && e < num_experts ? atomicAdd(&cnt[e], 1) : atomicAdd(&tail, 1)] = p;
+    }
+}
+
+size_t element(int dtype) { return dtype == IQK_F32 ? 4 : 2; }
+
+int check_matrix(const uint8_t *codes, const uint8_t *scales, int64_t scale_stride, int64_t rows,
+                 int64_t width) {
+    if (width <= 0 || width % kMxBlock || width > (1 << 20)) return IQK_ERR_GEOMETRY;
+    if (rows < 0 || rows > ((int64_t)1 << 31) - 1) return IQK_ERR_GEOMETRY;
+    if (scale_stride < width / kMxBlock || scale_stride % 16) return IQK_ERR_ALIGNMENT;
+    if (rows == 0) return IQK_OK;
+    if (!codes || !scales) return IQK_ERR_ARGUMENT;
+    if (!aligned(codes, 16) || !aligned(scales, 16)) return IQK_ERR_ALIGNMENT;
+    return IQK_OK;
+}
+
+int check_rows(const void *x, int dtype, int64_t rows, int64_t width, int64_t row_stride) {
+    if (!dtype_ok(dtype)) return IQK_ERR_ARGUMENT;
+    if (rows < 0 || rows > ((int64_t)1 << 31) - 1) return IQK_ERR_GEOMETRY;
+    if (rows > 1 && row_stride < width && row_stride != 0) return IQK_ERR_GEOMETRY;
+    if (rows == 0) return IQK_OK;
+    if (!x) return IQK_ERR_ARGUMENT;
+    if (!aligned(x, element(dtype))) return IQK_ERR_ALIGNMENT;
+    return IQK_OK;
+}
+
+}  // namespace
+
+cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
+                               int64_t row_stride, uint8_t *codes, uint8_t *scales,
+                               int64_t scale_stride, const int32_t *order, const int32_t *count,
+                               int64_t per_row, cudaStream_t stream, int sms) {
+    const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)sms * 16;
+    const unsigned blocks = (unsigned)(want < most ? want : most);
+    const bool wide = aligned(x, 16) && row_stride * (int64_t)element(dtype) % 16 == 0;
+#define IQK_Q(T, W)                                                                           \
+    mx_quantize_kernel<T, W><<<blocks, 256, 0, stream>>>(static_cast<const T *>(x), rows,     \
+                                                         width, row_stride, codes, scales,    \
+                                                         scale_stride, order, count, per_row)
+    if (dtype == IQK_F32) {
+        if (wide) IQK_Q(float, true);
+        else IQK_Q(float, false);
+    } else if (dtype == IQK_F16) {
+        if (wide) IQK_Q(__half, true);
+        else IQK_Q(__half, false);
+    } else {
+        if (wide) IQK_Q(__nv_bfloat16, true);
+        else IQK_Q(__nv_bfloat16, false);
+    }
+#undef IQK_Q
+    return cudaGetLastError();
+}
+
+}  // namespace iqk
+
+using namespace iqk;
+
+extern "C" {
+
+int iqk_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width, int64_t row_stride,
+                    uint8_t *codes, uint8_t *scales, int64_t scale_stride, iqk_stream_t stream) {
+    int st = check_matrix(codes, scales, scale_stride, rows, width);
+    if (st == IQK_OK) st = check_rows(x, dtype, rows, width, row_stride);
+    if (st != IQK_OK || rows == 0) return st;
+    return cuda_status(launch_mx_quantize(x, dtype, rows, width, row_stride, codes, scales,
+                                          scale_stride, nullptr, nullptr, 1,
+                                          reinterpret_cast<cudaStream_t>(stream),
+                                          num_sms_current()));
+}
+
+int iqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+                      int64_t rows, int64_t width, void *out, int out_dtype,
+                      iqk_stream_t stream) {
+    const int st = check_matrix(codes, scales, scale_stride, rows, width);
+    if (st != IQK_OK) return st;
+    if (!dtype_ok(out_dtype)) return IQK_ERR_ARGUMENT;
+    if (rows == 0) return IQK_OK;
+    if (!out) return IQK_ERR_ARGUMENT;
+    if (!aligned(out, 16)) return IQK_ERR_ALIGNMENT;
+    const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)num_sms_current() * 16;
+    const unsigned blocks = (unsigned)(want < most ? want : most);
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+#define IQK_D(T)                                                                        \
+    mx_dequantize_kernel<T><<<blocks, 256, 0, s>>>(codes, scales, scale_stride, rows, width, \
+                                                   static_cast<T *>(out))
+    if (out_dtype == IQK_F32) IQK_D(float);
+    else if (out_dtype == IQK_F16) IQK_D(__half);
+    else IQK_D(__nv_bfloat16);
+#undef IQK_D
+    return cuda_status(cudaGetLastError());
+}
+
+size_t iqk_mx_workspace_bytes(int64_t pairs, int64_t num_experts, int64_t width,
+                              int64_t out_features) {
+    if (pairs < 0 || pairs > (1 << 24) || num_experts <= 0 || num_experts > 4096 || width <= 0 ||
+        width % kMxBlock || width > (1 << 20) || out_features <= 0)
+        return 0;
+    return mx_layout(pairs, num_experts, width, out_features).total;
+}
+
+int iqk_mx_linear(const void *x, int x_dtype, int64_t rows, int64_t row_stride,
+                  const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+                  int64_t out_features, int64_t width, void *y, int y_dtype, void *workspace,
+                  size_t workspace_bytes, iqk_stream_t stream) {
+    if (out_features <= 0) return IQK_ERR_GEOMETRY;
+    int st = check_matrix(codes, scales, scale_stride, out_features, width);
+    if (st == IQK_OK) st = check_rows(x, x_dtype, rows, width, row_stride);
+    if (st != IQK_OK) return st;
+    if (!dtype_ok(y_dtype)) return IQK_ERR_ARGUMENT;
+    if (rows > (1 << 24)) return IQK_ERR_GEOMETRY;
+    if (rows == 0) return IQK_OK;
+    if (!y || !workspace) return IQK_ERR_ARGUMENT;
+    if (!aligned(y, element(y_dtype)) || !aligned(workspace, 256)) return IQK_ERR_ALIGNMENT;
+    MxProduct p{codes, scales, scale_stride, out_features, width, rows, 1,
+                static_cast<char *>(workspace), mx_layout(rows, 1, width, out_features), false,
+                y, y_dtype};
+    if (workspace_bytes < p.L.total) return IQK_ERR_WORKSPACE;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int sms = num_sms_current();
+    cudaError_t err = cudaMemsetAsync(p.ws + p.L.hdr, 0, 64, s);
+    if (err != cudaSuccess) return cuda_status(err);
+    err = launch_mx_quantize(x, x_dtype, rows, width, row_stride,
+                             reinterpret_cast<uint8_t *>(p.ws + p.L.codes),
+                             reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch, nullptr,
+                             nullptr, 1, s, sms);
+    if (err != cudaSuccess) return cuda_status(err);
+    return cuda_status(launch_mx_product(p, s, sms));
+}
+
+int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride,
+                  const int32_t *sel, int64_t pairs, const uint8_t *codes,
+                  const uint8_t *scales, int64_t scale_stride, int64_t num_experts,
+                  int64_t out_features, int64_t width, void *y, int y_dtype, void *workspace,
+                  size_t workspace_bytes, iqk_stream_t stream) {
+    if (out_features <= 0 || num_experts <= 0 || num_experts > 4096) return IQK_ERR_GEOMETRY;
+    if (out_features > ((int64_t)1 << 31) / num_experts) return IQK_ERR_GEOMETRY;
+    int st = check_matrix(codes, scales, scale_stride, num_experts * out_features, width);
+    if (st == IQK_OK) st = check_rows(x, x_dtype, x_rows, width, row_stride);
+    if (st != IQK_OK) return st;
+    if (!dtype_ok(y_dtype)) return IQK_ERR_ARGUMENT;
+    if (pairs < 0 || pairs > (1 << 24)) return IQK_ERR_GEOMETRY;
+    if (pairs == 0) return IQK_OK;
+    if (x_rows <= 0 || pairs % x_rows) return IQK_ERR_GEOMETRY;
+    if (!y || !workspace || !sel) return IQK_ERR_ARGUMENT;
+    if (!aligned(y, element(y_dtype)) || !aligned(workspace, 256) || !aligned(sel, 4))
+        return IQK_ERR_ALIGNMENT;
+    MxProduct p{codes, scales, scale_stride, out_features, width, pairs, num_experts,
+                static_cast<char *>(workspace),
+                mx_layout(pairs, num_experts, width, out_features), true, y, y_dtype};
+    if (workspace_bytes < p.L.total) return IQK_ERR_WORKSPACE;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int sms = num_sms_current();
+    mx_sort_kernel<<<1, 1024, sizeof(int32_t) * (size_t)num_experts, s>>>(
+        sel, (int)pairs, (int)num_experts, p.L, p.ws);
+    cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cuda_status(err);
+    err = launch_mx_quantize(x, x_dtype, pairs, width, row_stride,
+                             reinterpret_cast<uint8_t *>(p.ws + p.L.codes),
+                             reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch,
+                             reinterpret_cast<const int32_t *>(p.ws + p.L.order),
+                             reinterpret_cast<const int32_t *>(p.ws + p.L.hdr) + 2,
+                             pairs / x_rows, s, sms);
+    if (err != cudaSuccess) return cuda_status(err);
+    return cuda_status(launch_mx_product(p, s, sms));
+}
+
+int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream) {
+    if (!workspace || !flags) return IQK_ERR_ARGUMENT;
+    *flags = 0;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    int32_t word = 0;
+    cudaError_t err = cudaMemcpyAsync(&word, workspace, sizeof(word), cudaMemcpyDeviceToHost, s);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(s);
+    if (err == cudaSuccess) *flags = word;
+    return cuda_status(err);
+}
+
+}  // extern "C"

@@ -1,0 +1,42 @@
+// MXFP4 operators: host-side layout and launchers.
+#pragma once
+
+#include "iqk_common.cuh"
+
+namespace iqk {
+
+constexpr int kMxBlock = 32;  // values under one scale
+
+// Workspace of one product, written by its preparation:
+//   hdr    [16] int32: [0] device error bits, [1] work tiles, [2] routable pairs
+//   order  [pairs] int32: sorted position -> pair (the others at the tail)
+//   tiles  [max_tiles] int4: {expert, first position, rows (<= cap), 0}
+//   codes  [pairs, width / 2], scales [pairs, pitch]: the activations in
+//          sorted order
+struct MxLayout {
+    size_t hdr, order, tiles, codes, scales, total;
+    int64_t max_tiles, pitch;
+    int cap;  // rows of a tile
+};
+
+MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t out_features);
+
+// One call of the product: pairs sorted by expert (order and tiles), or, for a
+// single matrix, every row in its own place (order null).
+struct MxProduct {
+    const uint8_t *codes, *scales;  // the matrices, [experts * out_features] rows
+    int64_t scale_stride, out_features, width, pairs, num_experts;
+    char *ws;
+    MxLayout L;
+    bool routed;
+    void *y;
+    int y_dtype;
+};
+
+cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
+                               int64_t row_stride, uint8_t *codes, uint8_t *scales,
+                               int64_t scale_stride, const int32_t *order, const int32_t *count,
+                               int64_t per_row, cudaStream_t stream, int sms);
+cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms);
+
+}  // namespace iqk

@@ -152,6 +152,30 @@ def library() -> ctypes.CDLL:
     lib.iqk_pairs_swiglu.restype = i32
     lib.iqk_pairs_combine.argtypes = [vp, vp, i64, i32, i64, i64, vp, i32, vp]
     lib.iqk_pairs_combine.restype = i32
+    f32 = ctypes.c_float
+    lib.iqk_route.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, i32, f32, vp, vp, vp]
+    lib.iqk_route.restype = i32
+    lib.iqk_balance_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.iqk_balance_workspace_bytes.restype = sz
+    lib.iqk_route_balanced.argtypes = [vp, i32, i64, i64, i64, vp, vp, i64, i32, i32, i32, f32,
+                                       vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.iqk_route_balanced.restype = i32
+    lib.iqk_route_backward.argtypes = [vp, i32, i64, i64, i64, vp, vp, i64, i32, i32, i32, f32,
+                                       vp, vp, vp, vp, vp, vp]
+    lib.iqk_route_backward.restype = i32
+    lib.iqk_mx_quantize.argtypes = [vp, i32, i64, i64, i64, vp, vp, i64, vp]
+    lib.iqk_mx_quantize.restype = i32
+    lib.iqk_mx_dequantize.argtypes = [vp, vp, i64, i64, i64, vp, i32, vp]
+    lib.iqk_mx_dequantize.restype = i32
+    lib.iqk_mx_workspace_bytes.argtypes = [i64, i64, i64, i64]
+    lib.iqk_mx_workspace_bytes.restype = sz
+    lib.iqk_mx_linear.argtypes = [vp, i32, i64, i64, vp, vp, i64, i64, i64, vp, i32, vp, sz, vp]
+    lib.iqk_mx_linear.restype = i32
+    lib.iqk_mx_routed.argtypes = [vp, i32, i64, i64, vp, i64, vp, vp, i64, i64, i64, i64, vp, i32,
+                                  vp, sz, vp]
+    lib.iqk_mx_routed.restype = i32
+    lib.iqk_mx_read_error.argtypes = [vp, ctypes.POINTER(ctypes.c_int32), vp]
+    lib.iqk_mx_read_error.restype = i32
     _LIB = lib
     return lib
 
@@ -168,7 +192,10 @@ def exported_symbols() -> list[str]:
             "iqk_pairs_swiglu", "iqk_pairs_combine", "iqk_gemv_floor_run",
             "iqk_dequant_floor", "iqk_grouped_run_range", "iqk_pack",
             "iqk_gemv_glu_run", "iqk_swiglu_rows", "iqk_check_bounded_wait",
-            "iqk_dense_dequant", "iqk_dense_gemv"]
+            "iqk_dense_dequant", "iqk_dense_gemv",
+            "iqk_route", "iqk_balance_workspace_bytes", "iqk_route_balanced",
+            "iqk_route_backward", "iqk_mx_quantize", "iqk_mx_dequantize",
+            "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error"]
 
 
 def check_bounded_wait(limit_ns: int, device: torch.device) -> int:
@@ -201,6 +228,14 @@ def check_device(device: torch.device) -> None:
         with torch.cuda.device(idx):
             raise_for_status(library().iqk_check_device(), "device check")
         _DEVICE_OK[idx] = True
+
+
+def check_current(device: torch.device) -> None:
+    """The kernels launch on the current device: refuse tensors of another one."""
+    if device.index != torch.cuda.current_device():
+        raise IqkRuntimeError(
+            f"tensors on {device}, but the current device is {torch.cuda.current_device()}")
+    check_device(device)
 
 
 def stream_handle(device: torch.device) -> int:
@@ -502,6 +537,124 @@ def grouped_read_error(workspace: torch.Tensor) -> int:
     raise_for_status(library().iqk_grouped_read_error(workspace.data_ptr(), ctypes.byref(flags),
                                                       stream_handle(workspace.device)),
                      "iqk_grouped_read_error")
+    return int(flags.value)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def route(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int, renormalize: bool,
+          scale: float, indices, balance: bool):
+    """``iqk_route`` / ``iqk_route_balanced`` over logits ``rows [tokens, experts]``:
+    ``(indices, weights, loss, counts, slope)``, the last three None without
+    ``balance``. ``indices`` given (a choice already made): weights are None."""
+    lib, dev = library(), rows.device
+    tokens, experts = rows.shape
+    weights = None
+    if indices is None:
+        indices = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
+        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    stream = stream_handle(dev)
+    if not balance:
+        status = lib.iqk_route(rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts,
+                               rows.stride(0), _ptr(mask), top_k, scoring, renormalize, scale,
+                               indices.data_ptr(), weights.data_ptr(), stream)
+        raise_for_status(status, "iqk_route")
+        return indices, weights, None, None, None
+    segments = 1 if offsets is None else offsets.numel() - 1
+    need = int(lib.iqk_balance_workspace_bytes(tokens, experts, segments))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty((segments, experts), dtype=torch.int32, device=dev)
+    slope = torch.empty((segments, experts), dtype=torch.float32, device=dev)
+    status = lib.iqk_route_balanced(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
+        _ptr(offsets), segments, top_k, scoring, renormalize, scale, indices.data_ptr(),
+        _ptr(weights), loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), ws.data_ptr(), need,
+        stream)
+    raise_for_status(status, "iqk_route_balanced")
+    return indices, weights, loss, counts, slope
+
+
+def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
+                   renormalize: bool, scale: float, indices, grad_weights, slope,
+                   grad_loss) -> torch.Tensor:
+    """``iqk_route_backward``: the logits' gradient ``[tokens, experts]``."""
+    tokens, experts = rows.shape
+    if grad_weights is not None:
+        grad_weights = grad_weights.to(torch.float32).contiguous()
+    if grad_loss is not None:
+        grad_loss = grad_loss.to(torch.float32).contiguous()
+    grad = torch.empty((tokens, experts), dtype=rows.dtype, device=rows.device)
+    status = library().iqk_route_backward(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
+        _ptr(offsets), 1 if offsets is None else offsets.numel() - 1, top_k, scoring, renormalize,
+        scale, indices.data_ptr(), _ptr(grad_weights), _ptr(slope), _ptr(grad_loss),
+        grad.data_ptr(), stream_handle(rows.device))
+    raise_for_status(status, "iqk_route_backward")
+    return grad
+
+
+def mx_quantize(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                scale_stride: int) -> None:
+    """``iqk_mx_quantize``: float rows ``[rows, width]`` into ``codes`` and ``scales``."""
+    status = library().iqk_mx_quantize(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], rows.shape[0], rows.shape[1], rows.stride(0),
+        codes.data_ptr(), scales.data_ptr(), scale_stride, stream_handle(rows.device))
+    raise_for_status(status, "iqk_mx_quantize")
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, scale_stride: int,
+                  out: torch.Tensor) -> None:
+    """``iqk_mx_dequantize`` into ``out [..., width]``."""
+    width = out.shape[-1]
+    status = library().iqk_mx_dequantize(
+        codes.data_ptr(), scales.data_ptr(), scale_stride, out.numel() // width, width,
+        out.data_ptr(), DTYPE_IDS[out.dtype], stream_handle(out.device))
+    raise_for_status(status, "iqk_mx_dequantize")
+
+
+@functools.lru_cache(maxsize=1024)
+def mx_workspace_bytes(pairs: int, num_experts: int, width: int, out_features: int) -> int:
+    return int(library().iqk_mx_workspace_bytes(pairs, num_experts, width, out_features))
+
+
+def mx_linear(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, scale_stride: int,
+              out_features: int, y: torch.Tensor) -> None:
+    """``iqk_mx_linear``: ``y [rows, out] = q(rows) W^T``."""
+    count, width = rows.shape
+    need = mx_workspace_bytes(count, 1, width, out_features)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
+    status = library().iqk_mx_linear(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], count, rows.stride(0), codes.data_ptr(),
+        scales.data_ptr(), scale_stride, out_features, width, y.data_ptr(), DTYPE_IDS[y.dtype],
+        ws.data_ptr(), ws.numel(), stream_handle(y.device))
+    raise_for_status(status, "iqk_mx_linear")
+
+
+def mx_routed(rows: torch.Tensor, sel: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+              scale_stride: int, y: torch.Tensor, workspace: torch.Tensor | None = None) -> None:
+    """``iqk_mx_routed``: ``y [pairs, out]`` through the stacked matrices."""
+    pairs, width = sel.numel(), rows.shape[1]
+    experts, out_features = codes.shape[0], codes.shape[1]
+    if workspace is None:
+        need = mx_workspace_bytes(pairs, experts, width, out_features)
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
+    status = library().iqk_mx_routed(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], rows.shape[0], rows.stride(0), sel.data_ptr(),
+        pairs, codes.data_ptr(), scales.data_ptr(), scale_stride, experts, out_features, width,
+        y.data_ptr(), DTYPE_IDS[y.dtype], workspace.data_ptr(), workspace.numel(),
+        stream_handle(y.device))
+    raise_for_status(status, "iqk_mx_routed")
+
+
+def mx_read_error(workspace: torch.Tensor) -> int:
+    """``iqk_mx_read_error``: the device error bits of a routed product's workspace."""
+    flags = ctypes.c_int32(0)
+    raise_for_status(library().iqk_mx_read_error(workspace.data_ptr(), ctypes.byref(flags),
+                                                 stream_handle(workspace.device)),
+                     "iqk_mx_read_error")
     return int(flags.value)
 
 

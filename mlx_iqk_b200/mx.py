@@ -1,0 +1,264 @@
+"""MXFP4: microscaled 4-bit floating point, quantisation and products.
+
+The OCP Microscaling format beside the IQ_K members: 32 consecutive values of
+a row share one power-of-two scale (E8M0, a byte), each value a 4-bit E2M1
+code. A matrix ``[..., rows, width]`` is two tensors that the caller holds, as
+the dense members' streams are:
+
+- ``codes  uint8 [..., rows, width / 2]``, two codes a byte, the even column in
+  the low nibble, contiguous;
+- ``scales uint8 [..., rows, width / 32]``, each row on a 16-byte boundary
+  (:func:`mx_quantize` returns it as a view of such rows;
+  :func:`mx_aligned_scales` makes one of packed scales, once, at load time).
+
+Functions:
+
+- :func:`mx_quantize`, :func:`mx_dequantize`  to the format and back;
+- :func:`mx_linear`         ``q(x) W^T`` through one matrix;
+- :func:`mx_switch_linear`  the same through the experts that a router picked,
+  on the seam of ``IqkSwitchLinear`` (``src/mlx_iqk/nn.py:105-333``);
+- :class:`MxSwitchGLU`      one SwitchGLU layer of MXFP4 experts.
+
+Activations are quantised inside the product, so that both operands are 4-bit
+on the tensor cores; products and sums are float32, rounded once to
+``out_dtype`` (the activations' type unless given). These are serving
+operators: they carry no gradient and refuse an input that asks for one.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import kernels as K
+from .kernels import IqkKernelError, IqkRuntimeError
+
+MX_BLOCK = 32
+
+
+def _rows(x, what="x"):
+    """``x`` as float rows ``[rows, width]`` whose columns are adjacent."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise IqkRuntimeError(f"{what} must be a tensor on the GPU")
+    if x.dtype not in K.DTYPE_IDS:
+        raise IqkRuntimeError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise IqkRuntimeError(f"the MXFP4 operators carry no gradient: detach {what}")
+    if x.dim() < 1 or x.shape[-1] <= 0 or x.shape[-1] % MX_BLOCK:
+        raise IqkKernelError(
+            f"{what} must have a width that is a positive multiple of {MX_BLOCK}, "
+            f"got shape {tuple(x.shape)}")
+    K.check_current(x.device)
+    rows = x.reshape(-1, x.shape[-1])
+    if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]
+                               and rows.stride(0) != 0):
+        rows = rows.contiguous()
+    return rows
+
+
+def _matrix(codes, scales, dims, device=None):
+    """Checks a matrix's two tensors; returns the byte stride of its scale rows."""
+    for t, name in ((codes, "codes"), (scales, "scales")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise IqkRuntimeError(f"{name} must be a tensor on the GPU")
+        if t.dtype != torch.uint8:
+            raise IqkRuntimeError(f"{name} must be uint8, got {t.dtype}")
+    if codes.device != scales.device or (device is not None and codes.device != device):
+        raise IqkRuntimeError("codes, scales and activations must be on one device")
+    if codes.dim() < 1 or (dims and codes.dim() != dims):
+        raise IqkRuntimeError(f"codes must have {dims or 'at least 1'} axes, got {codes.dim()}")
+    blocks = scales.shape[-1] if scales.dim() else 0
+    if scales.shape[:-1] != codes.shape[:-1] or codes.shape[-1] != blocks * MX_BLOCK // 2 \
+            or blocks == 0:
+        raise IqkRuntimeError(
+            f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not belong "
+            f"together: {MX_BLOCK // 2} code bytes to a scale")
+    if not codes.is_contiguous() or codes.data_ptr() % 16:
+        raise IqkRuntimeError("codes must be contiguous and 16-byte aligned")
+    if scales.numel() == blocks:  # one row: any stride will do
+        stride = (blocks + 15) // 16 * 16
+        packed = True
+    else:
+        stride, packed = None, True
+        step = None
+        for axis in range(scales.dim() - 2, -1, -1):
+            if scales.shape[axis] == 1:
+                continue
+            if step is None:
+                stride = step = scales.stride(axis)
+            packed = packed and scales.stride(axis) == step
+            step = step * scales.shape[axis]
+    if blocks > 1 and scales.stride(-1) != 1 or not packed or stride % 16 \
+            or stride < blocks or scales.data_ptr() % 16:
+        raise IqkRuntimeError(
+            "scale rows must be evenly spaced and start on 16-byte boundaries "
+            "(mx_aligned_scales lays packed scales out so)")
+    return stride
+
+
+def mx_aligned_scales(scales: torch.Tensor) -> torch.Tensor:
+    """A copy of ``scales [..., rows, blocks]`` whose rows start on 16-byte boundaries."""
+    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.uint8 or scales.dim() < 1:
+        raise IqkRuntimeError("scales must be a uint8 tensor")
+    out = _scale_rows(scales.shape[:-1], scales.shape[-1], scales.device)
+    out.copy_(scales)
+    return out
+
+
+def _scale_rows(lead, blocks, device) -> torch.Tensor:
+    pitch = (blocks + 15) // 16 * 16
+    t = torch.empty(tuple(lead) + (pitch,), dtype=torch.uint8, device=device)
+    return t if pitch == blocks else t[..., :blocks]
+
+
+def mx_quantize(x):
+    """``(codes, scales)`` of ``x [..., width]`` (float32, float16 or bfloat16).
+
+    Each block's scale is ``2^(floor(log2 m) - 2)``, ``m`` its largest magnitude
+    (``2^-127`` at least); values round to the nearest code, ties to the even
+    one, and hold at 6 beyond it. A block with a NaN or an infinity gets scale
+    byte 255: all of it reads NaN."""
+    rows = _rows(x)
+    width = x.shape[-1]
+    codes = torch.empty(x.shape[:-1] + (width // 2,), dtype=torch.uint8, device=x.device)
+    scales = _scale_rows(x.shape[:-1], width // MX_BLOCK, x.device)
+    K.mx_quantize(rows, codes, scales, (width // MX_BLOCK + 15) // 16 * 16)
+    return codes, scales
+
+
+def mx_dequantize(codes, scales, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values ``[..., width]`` of an MXFP4 tensor: exact in float32, rounded once
+    to float16 or bfloat16."""
+    stride = _matrix(codes, scales, 0)
+    if dtype not in K.DTYPE_IDS:
+        raise IqkRuntimeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    K.check_current(codes.device)
+    width = codes.shape[-1] * 2
+    out = torch.empty(codes.shape[:-1] + (width,), dtype=dtype, device=codes.device)
+    K.mx_dequantize(codes, scales, stride, out)
+    return out
+
+
+def _out_dtype(x, out_dtype):
+    dtype = x.dtype if out_dtype is None else out_dtype
+    if dtype not in K.DTYPE_IDS:
+        raise IqkRuntimeError(f"out_dtype must be float32, float16 or bfloat16, got {dtype}")
+    return dtype
+
+
+def mx_linear(x, codes, scales, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``q(x) W^T`` ``[..., out]`` for ``x [..., width]`` and ``W`` = ``codes [out,
+    width / 2]``, ``scales [out, width / 32]``; ``q`` is :func:`mx_quantize`."""
+    rows = _rows(x)
+    stride = _matrix(codes, scales, 2, x.device)
+    if codes.shape[-1] * 2 != x.shape[-1]:
+        raise IqkRuntimeError(f"x of width {x.shape[-1]} meets a matrix of {codes.shape[-1] * 2}")
+    out = codes.shape[0]
+    y = torch.empty(x.shape[:-1] + (out,), dtype=_out_dtype(x, out_dtype), device=x.device)
+    if y.numel():
+        K.mx_linear(rows, codes, scales, stride, out, y)
+    return y
+
+
+def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``q(x) W_e^T`` through the experts that ``indices [..., top_k]`` names:
+    ``[..., top_k, 1, out]``.
+
+    ``x`` is ``[..., 1, 1, width]`` (one row per token, shared by its experts) or
+    ``[..., top_k, 1, width]`` (one row per pair); the matrices are ``codes
+    [experts, out, width / 2]`` and ``scales [experts, out, width / 32]``. Each
+    picked expert's matrix is read once for all its pairs. Index -1 (a token
+    that the router left out) gives a zero row. So does an index beyond the
+    experts, which also sets ``DEVERR_EXPERT`` in a caller's ``workspace``
+    (uint8, ``kernels.mx_workspace_bytes``), read by
+    ``kernels.mx_read_error``."""
+    rows = _rows(x)
+    stride = _matrix(codes, scales, 3, x.device)
+    if not isinstance(indices, torch.Tensor) or indices.device != x.device \
+            or indices.dtype not in (torch.int32, torch.int64):
+        raise IqkRuntimeError("indices must be an int32 or int64 tensor beside x")
+    if codes.shape[-1] * 2 != x.shape[-1]:
+        raise IqkRuntimeError(f"x of width {x.shape[-1]} meets matrices of {codes.shape[-1] * 2}")
+    sel = indices.to(torch.int32).contiguous()
+    pairs, out = sel.numel(), codes.shape[1]
+    y = torch.empty(tuple(indices.shape) + (1, out), dtype=_out_dtype(x, out_dtype),
+                    device=x.device)
+    if pairs and (rows.shape[0] == 0 or pairs % rows.shape[0]):
+        raise IqkRuntimeError(
+            f"{pairs} token-expert pairs do not tile {rows.shape[0]} activation "
+            f"row(s); the operand and the routing disagree")
+    if y.numel():
+        if codes.shape[0] == 0:
+            return y.zero_()
+        K.mx_routed(rows, sel, codes, scales, stride, y, workspace)
+    return y
+
+
+class MxSwitchGLU(nn.Module):
+    """One SwitchGLU layer of MXFP4 experts, ``(x, indices, scores)`` as
+    ``IqkSwitchGLU``: gate and up ``[experts, inter, hidden]``, down ``[experts,
+    hidden, inter]``, ``h = silu(gate) * up * score`` in float32, and each
+    token's sum over its experts."""
+
+    def __init__(self, num_experts: int, hidden: int, inter: int, device=None):
+        super().__init__()
+        for what, value in (("hidden", hidden), ("inter", inter)):
+            if value <= 0 or value % MX_BLOCK:
+                raise IqkKernelError(f"{what} {value} is not a positive multiple of {MX_BLOCK}")
+        if not 0 < num_experts <= 4096:
+            raise IqkRuntimeError(f"num_experts {num_experts} is not in 1 to 4096")
+        self.num_experts, self.hidden, self.inter = num_experts, hidden, inter
+        for name, (rows, width) in self._shapes().items():
+            self.register_buffer(f"{name}_codes", torch.zeros(
+                (num_experts, rows, width // 2), dtype=torch.uint8, device=device))
+            self.register_buffer(f"{name}_scales", _scale_rows(
+                (num_experts, rows), width // MX_BLOCK, device).zero_())
+
+    def _shapes(self):
+        return {"gate": (self.inter, self.hidden), "up": (self.inter, self.hidden),
+                "down": (self.hidden, self.inter)}
+
+    def load(self, name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        """Install one projection's matrices (``gate``, ``up`` or ``down``)."""
+        if name not in self._shapes():
+            raise IqkRuntimeError(f"projection must be gate, up or down, got {name!r}")
+        into = getattr(self, f"{name}_codes"), getattr(self, f"{name}_scales")
+        for new, old, what in zip((codes, scales), into, ("codes", "scales")):
+            if tuple(new.shape) != tuple(old.shape) or new.dtype != torch.uint8:
+                raise IqkRuntimeError(f"{name} {what} must be uint8 {tuple(old.shape)}, got "
+                                      f"{new.dtype} {tuple(new.shape)}")
+        into[0].copy_(codes)
+        into[1].copy_(scales)
+
+    def load_weights(self, name: str, weights: torch.Tensor) -> None:
+        """Quantise and install one projection's float matrices ``[experts, rows, width]``."""
+        self.load(name, *mx_quantize(weights))
+
+    def forward(self, x, indices, scores) -> torch.Tensor:
+        """``x [..., hidden]``, ``indices`` and ``scores [..., top_k]`` ->
+        ``[..., hidden]`` float32."""
+        lead, k = tuple(indices.shape[:-1]), indices.shape[-1]
+        if tuple(x.shape) != lead + (self.hidden,) or scores.shape != indices.shape:
+            raise IqkRuntimeError(
+                f"x {tuple(x.shape)}, indices {tuple(indices.shape)} and scores "
+                f"{tuple(scores.shape)} do not belong together")
+        sel = indices.reshape(-1, k).to(torch.int32).contiguous()
+        rows = x.reshape(-1, 1, 1, self.hidden)
+        out = torch.empty((rows.shape[0], self.hidden), dtype=torch.float32, device=x.device)
+        if not sel.numel():
+            return out.zero_().view(lead + (self.hidden,))
+        f32 = torch.float32
+        gate = mx_switch_linear(rows, sel, self.gate_codes, self.gate_scales, f32)
+        up = mx_switch_linear(rows, sel, self.up_codes, self.up_scales, f32)
+        w = scores.reshape(-1).to(f32).contiguous()
+        h = torch.empty((sel.numel(), self.inter), dtype=f32, device=x.device)
+        K.swiglu_rows(gate.view(-1, self.inter), up.view(-1, self.inter), w, h)
+        y = mx_switch_linear(h.view(-1, k, 1, self.inter), sel, self.down_codes,
+                             self.down_scales, f32)
+        K.pairs_combine(y, sel, k, self.num_experts, out)
+        return out.view(lead + (self.hidden,))
+
+
+__all__ = ["MX_BLOCK", "MxSwitchGLU", "mx_aligned_scales", "mx_dequantize", "mx_linear",
+           "mx_quantize", "mx_switch_linear"]

@@ -1,0 +1,157 @@
+"""Expert router: top-k choice, router weights, counts and the balance loss.
+
+The step in front of the routed experts (the reference is handed ``indices``
+and ``scores``, ``src/mlx_iqk/nn.py:1-22``; here they can be made on the device
+that uses them):
+
+- :func:`route`           ``(indices, weights)`` of each token's top-k experts;
+- :func:`balance_loss`    the loss that keeps experts evenly used, and the
+  per-expert counts, of a choice already made;
+- :func:`route_balanced`  both in one pass over the logits, as a training step
+  takes them.
+
+Scores are ``softmax`` over the experts or ``sigmoid`` of each logit. A logit
+of ``-inf`` is no expert, and ``mask`` (bool, one per token) leaves whole rows
+out: the places of a row without an expert hold index ``-1`` and weight 0,
+which the experts' products turn into zero rows. Everything is differentiable
+in ``logits`` (float32, float16 or bfloat16); sums are float32 and joined in a
+fixed order, so results repeat bit for bit.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels as K
+from .kernels import IqkKernelError, IqkRuntimeError
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 32
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def _check(logits, top_k, scoring, mask, offsets=None):
+    """The call's logits as ``[tokens, experts]`` rows, its mask, offsets and scoring id."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise IqkRuntimeError("logits must be a tensor on the GPU")
+    if logits.dtype not in K.DTYPE_IDS:
+        raise IqkRuntimeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    if logits.dim() < 1:
+        raise IqkRuntimeError("logits must have an expert axis")
+    experts = logits.shape[-1]
+    if not 0 < experts <= MAX_EXPERTS:
+        raise IqkKernelError(f"the router covers 1 to {MAX_EXPERTS} experts, got {experts}")
+    if not 0 < top_k <= min(MAX_TOP_K, experts):
+        raise IqkKernelError(f"top_k {top_k} is not in 1 to {min(MAX_TOP_K, experts)}")
+    if scoring not in _SCORING:
+        raise IqkRuntimeError(f"scoring must be one of {sorted(_SCORING)}, got {scoring!r}")
+    dev = logits.device
+    K.check_current(dev)
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, experts)
+    if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < experts):
+        rows = rows.contiguous()
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.device != dev:
+            raise IqkRuntimeError("mask must be a bool tensor beside the logits")
+        if mask.shape != logits.shape[:-1]:
+            raise IqkRuntimeError(
+                f"mask {tuple(mask.shape)} does not match tokens {tuple(logits.shape[:-1])}")
+        mask = mask.contiguous()
+    if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.device != dev or offsets.dim() != 1 \
+                or offsets.numel() < 2:
+            raise IqkRuntimeError("offsets must be int32 [segments + 1] beside the logits")
+        offsets = offsets.contiguous()
+    return rows, mask, offsets, _SCORING[scoring]
+
+
+class _Route(torch.autograd.Function):
+    """Choice and balance loss with one gradient kernel. ``indices`` None: chosen here."""
+
+    @staticmethod
+    def forward(ctx, logits, rows, indices, top_k, scoring, renormalize, scale, mask, offsets,
+                balance):
+        ctx.set_materialize_grads(False)
+        choose = indices is None
+        indices, weights, loss, counts, slope = K.route(
+            rows, mask, offsets, top_k, scoring, renormalize, scale, indices, balance)
+        ctx.call = (top_k, scoring, renormalize, scale, logits.shape)
+        ctx.save_for_backward(rows, mask, offsets, indices, slope)
+        ctx.mark_non_differentiable(*(t for t in (indices if choose else None, counts)
+                                      if t is not None))
+        return (indices if choose else None), weights, loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _indices, grad_weights, grad_loss, _counts):
+        rows, mask, offsets, indices, slope = ctx.saved_tensors
+        top_k, scoring, renormalize, scale, shape = ctx.call
+        if grad_loss is None:
+            slope = None
+        if grad_weights is None and slope is None:
+            return (None,) * 10
+        grad = K.route_backward(rows, mask, offsets, top_k, scoring, renormalize, scale, indices,
+                                grad_weights, slope, grad_loss)
+        return (grad.view(shape),) + (None,) * 9
+
+
+def _run(logits, indices, top_k, scoring, renormalize, scale, mask, offsets, balance):
+    rows, mask, offsets, scoring = _check(logits, top_k, scoring, mask, offsets)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, rows.detach(), indices, top_k, scoring, renormalize, scale,
+                            mask, offsets, balance)
+    return K.route(rows, mask, offsets, top_k, scoring, renormalize, scale, indices, balance)[:4]
+
+
+def route(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = True,
+          scale: float = 1.0, mask=None):
+    """``(indices int32 [..., top_k], weights float32 [..., top_k])`` of ``logits
+    [..., experts]``: the ``top_k`` largest in falling order (equal ones by
+    index), and ``scale`` times their scores, divided by the scores' sum when
+    ``renormalize``. Differentiable in ``logits`` through the weights."""
+    indices, weights, _, _ = _run(logits, None, top_k, scoring, renormalize, scale, mask, None,
+                                  False)
+    if logits.dim() == 2:
+        return indices, weights
+    shape = logits.shape[:-1] + (top_k,)
+    return indices.view(shape), weights.view(shape)
+
+
+def route_balanced(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = True,
+                   scale: float = 1.0, mask=None, offsets=None):
+    """``(indices, weights, loss, counts)``: :func:`route` and :func:`balance_loss`
+    in one pass over the logits, forward and backward."""
+    indices, weights, loss, counts = _run(logits, None, top_k, scoring, renormalize, scale, mask,
+                                          offsets, True)
+    if logits.dim() != 2:
+        shape = logits.shape[:-1] + (top_k,)
+        indices, weights = indices.view(shape), weights.view(shape)
+    return indices, weights, loss, counts
+
+
+def balance_loss(logits, indices, *, scoring: str = "softmax", mask=None, offsets=None):
+    """``(loss, counts)`` of a choice ``indices [..., top_k]``.
+
+    Per segment ``g`` with ``N`` tokens, ``f_e = experts * counts_e / (top_k * N)``
+    and ``P_e`` the mean over its tokens of the score normalised over the
+    experts; the loss is the mean over the segments that hold a token of
+    ``sum_e f_e P_e`` (1 when the experts are used evenly). ``offsets`` (int32
+    ``[segments + 1]`` on the GPU, not falling, from 0 to the token count) cuts
+    the tokens, flattened, into segments, as packed sequences do; None is one
+    segment. ``counts`` is int32 ``[segments, experts]``; entries of
+    ``indices`` outside the experts count for none. Differentiable in
+    ``logits`` through the mean scores (a count has no gradient).
+    """
+    if not isinstance(indices, torch.Tensor) or not isinstance(logits, torch.Tensor) \
+            or indices.dim() != logits.dim() or indices.shape[:-1] != logits.shape[:-1]:
+        raise IqkRuntimeError("indices must be [..., top_k] beside logits [..., experts]")
+    if indices.device != logits.device:
+        raise IqkRuntimeError("indices must be on the logits' device")
+    top_k = indices.shape[-1]
+    sel = indices.to(torch.int32).contiguous()
+    return _run(logits, sel, top_k, scoring, True, 1.0, mask, offsets, True)[2:]
+
+
+__all__ = ["MAX_EXPERTS", "MAX_TOP_K", "balance_loss", "route", "route_balanced"]
