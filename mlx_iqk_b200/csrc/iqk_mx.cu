@@ -64,13 +64,17 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax, float &inv) {
 }
 
 // Row r of the output is row r of x, or with `order` row order[r] / per_row
-// (a pair's activation row) for the first *count of them.
+// (a pair's activation row) for the first *count of them. Block 0 clears the
+// words that the product kernel counts in.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const T *__restrict__ x, int64_t rows, int64_t width, int64_t row_stride,
                    uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                    int64_t scale_stride, const int32_t *__restrict__ order,
-                   const int32_t *__restrict__ count, int64_t per_row) {
+                   const int32_t *__restrict__ count, int64_t per_row,
+                   int32_t *__restrict__ zero, int zero_words) {
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero[i] = 0;
     const int64_t per = width / 8;  // threads of a row
     const int64_t all = (order ? (int64_t)*count : rows) * per;
     // whole groups of four lanes run or stop together: `per` is a multiple of 4
@@ -139,6 +143,7 @@ mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLa
     int32_t *order = reinterpret_cast<int32_t *>(ws + L.order);
     int4 *tiles = reinterpret_cast<int4 *>(ws + L.tiles);
     for (int e = tid; e < num_experts; e += nt) cnt[e] = 0;
+    for (int i = tid; i < L.zeroed(); i += nt) hdr[i] = 0;
     if (tid == 0) bad = 0;
     __syncthreads();
     for (int p = tid; p < pairs; p += nt) {
@@ -217,14 +222,16 @@ int check_rows(const void *x, int dtype, int64_t rows, int64_t width, int64_t ro
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
                                int64_t row_stride, uint8_t *codes, uint8_t *scales,
                                int64_t scale_stride, const int32_t *order, const int32_t *count,
-                               int64_t per_row, cudaStream_t stream, int sms) {
+                               int64_t per_row, int32_t *zero, int zero_words,
+                               cudaStream_t stream, int sms) {
     const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)sms * 16;
     const unsigned blocks = (unsigned)(want < most ? want : most);
     const bool wide = aligned(x, 16) && row_stride * (int64_t)element(dtype) % 16 == 0;
 #define IQK_Q(T, W)                                                                           \
     mx_quantize_kernel<T, W><<<blocks, 256, 0, stream>>>(static_cast<const T *>(x), rows,     \
                                                          width, row_stride, codes, scales,    \
-                                                         scale_stride, order, count, per_row)
+                                                         scale_stride, order, count, per_row,    \
+                                                         zero, zero_words)
     if (dtype == IQK_F32) {
         if (wide) IQK_Q(float, true);
         else IQK_Q(float, false);
@@ -251,7 +258,7 @@ int iqk_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width, int64
     if (st == IQK_OK) st = check_rows(x, dtype, rows, width, row_stride);
     if (st != IQK_OK || rows == 0) return st;
     return cuda_status(launch_mx_quantize(x, dtype, rows, width, row_stride, codes, scales,
-                                          scale_stride, nullptr, nullptr, 1,
+                                          scale_stride, nullptr, nullptr, 1, nullptr, 0,
                                           reinterpret_cast<cudaStream_t>(stream),
                                           num_sms_current()));
 }
@@ -305,12 +312,11 @@ int iqk_mx_linear(const void *x, int x_dtype, int64_t rows, int64_t row_stride,
     if (workspace_bytes < p.L.total) return IQK_ERR_WORKSPACE;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = num_sms_current();
-    cudaError_t err = cudaMemsetAsync(p.ws + p.L.hdr, 0, 64, s);
-    if (err != cudaSuccess) return cuda_status(err);
-    err = launch_mx_quantize(x, x_dtype, rows, width, row_stride,
+    cudaError_t err = launch_mx_quantize(x, x_dtype, rows, width, row_stride,
                              reinterpret_cast<uint8_t *>(p.ws + p.L.codes),
                              reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch, nullptr,
-                             nullptr, 1, s, sms);
+                             nullptr, 1, reinterpret_cast<int32_t *>(p.ws + p.L.hdr),
+                             p.L.zeroed(), s, sms);
     if (err != cudaSuccess) return cuda_status(err);
     return cuda_status(launch_mx_product(p, s, sms));
 }
@@ -347,7 +353,7 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
                              reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch,
                              reinterpret_cast<const int32_t *>(p.ws + p.L.order),
                              reinterpret_cast<const int32_t *>(p.ws + p.L.hdr) + 2,
-                             pairs / x_rows, s, sms);
+                             pairs / x_rows, nullptr, 0, s, sms);
     if (err != cudaSuccess) return cuda_status(err);
     return cuda_status(launch_mx_product(p, s, sms));
 }

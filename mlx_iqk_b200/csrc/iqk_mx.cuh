@@ -9,14 +9,18 @@ constexpr int kMxBlock = 32;  // values under one scale
 
 // Workspace of one product, written by its preparation:
 //   hdr    [16] int32: [0] device error bits, [1] work tiles, [2] routable pairs
+//   tickets  int32: parts that are done of each item that CTAs share,
+//          per 32 outputs
 //   order  [pairs] int32: sorted position -> pair (the others at the tail)
 //   tiles  [max_tiles] int4: {expert, first position, rows (<= cap), 0}
 //   codes  [pairs, width / 2], scales [pairs, pitch]: the activations in
 //          sorted order
+//   slots  f32: shared items' parts
 struct MxLayout {
-    size_t hdr, order, tiles, codes, scales, total;
+    size_t hdr, tickets, order, tiles, codes, scales, slots, total;
     int64_t max_tiles, pitch;
-    int cap;  // rows of a tile
+    int cap;  // rows of a tile, a row box of the product kernel
+    __host__ __device__ int zeroed() const { return (int)((order - hdr) / 4); }  // words that start at 0
 };
 
 MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t out_features);
@@ -36,7 +40,8 @@ struct MxProduct {
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
                                int64_t row_stride, uint8_t *codes, uint8_t *scales,
                                int64_t scale_stride, const int32_t *order, const int32_t *count,
-                               int64_t per_row, cudaStream_t stream, int sms);
+                               int64_t per_row, int32_t *zero, int zero_words,
+                               cudaStream_t stream, int sms);
 cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms);
 
 }  // namespace iqk

@@ -138,6 +138,19 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc
         : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem]^T, kind::mxf4: E2M1 operands, 64 columns of K,
+// a UE8M0 scale per 32 of them from tensor memory, f32 accumulate.
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t scale_a, uint32_t scale_b,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
+        " [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+
 // 32 lanes x 32-bit, 32 consecutive columns per thread (its own lane).
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -150,6 +163,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+// 32 lanes x 32-bit, 4 consecutive columns per thread (its own lane).
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c,
+                                         uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(taddr),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
 }
 // 32 lanes x 32-bit, 8 consecutive columns per thread (its own lane).
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -182,6 +202,14 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
     return (1u << 4) | (0u << 7) | (0u << 10) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
+}
+
+// Instruction descriptor, kind::mxf4: E2M1 A and B (format 1), both K-major,
+// UE8M0 scales (bit 23), shape M x N. The scale words in tensor memory hold
+// four scales; `part` 0 or 2 names the pair that this K = 64 step uses.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int part) {
+    return ((uint32_t)part << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
+           (1u << 23) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)part << 29);
 }
 
 }  // namespace dev
