@@ -217,6 +217,11 @@ int check_rows(const void *x, int dtype, int64_t rows, int64_t width, int64_t ro
     return IQK_OK;
 }
 
+// The product kernel counts its items in 32 bits.
+bool mx_items_ok(const MxProduct &p) {
+    return p.L.max_tiles * ((p.out_features + 127) / 128) < (int64_t)1 << 31;
+}
+
 }  // namespace
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
@@ -310,6 +315,7 @@ int iqk_mx_linear(const void *x, int x_dtype, int64_t rows, int64_t row_stride,
                 static_cast<char *>(workspace), mx_layout(rows, 1, width, out_features), false,
                 y, y_dtype};
     if (workspace_bytes < p.L.total) return IQK_ERR_WORKSPACE;
+    if (!mx_items_ok(p)) return IQK_ERR_GEOMETRY;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = num_sms_current();
     cudaError_t err = launch_mx_quantize(x, x_dtype, rows, width, row_stride,
@@ -342,6 +348,7 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
                 static_cast<char *>(workspace),
                 mx_layout(pairs, num_experts, width, out_features), true, y, y_dtype};
     if (workspace_bytes < p.L.total) return IQK_ERR_WORKSPACE;
+    if (!mx_items_ok(p)) return IQK_ERR_GEOMETRY;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = num_sms_current();
     mx_sort_kernel<<<1, 1024, sizeof(int32_t) * (size_t)num_experts, s>>>(

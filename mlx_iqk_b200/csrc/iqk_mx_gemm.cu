@@ -84,23 +84,24 @@ struct Maps {
 
 // The items of a call and how they are dealt to the CTAs.
 struct Plan {
-    int64_t items, whole;  // whole: items dealt in full waves
-    int64_t tiles, units;  // units of an item
-    int64_t s0, s1;        // this CTA's run of units over the shared items
-    __device__ int64_t start(int64_t cta) const {
-        const int64_t all = (items - whole) * units;
-        return all * cta / gridDim.x;
-    }
+    uint32_t items, whole;   // whole: items dealt in full waves
+    uint32_t tiles, units;   // units of an item
+    uint32_t all, runs;      // units of the shared items, CTAs that take a run of them
+    uint32_t s0, s1;         // this CTA's run
+    __device__ uint32_t start(uint32_t cta) const { return all * min(cta, runs) / runs; }
 };
 
 __device__ __forceinline__ Plan make_plan(const ProductArgs &a) {
     Plan p;
-    const int64_t nblocks = (a.out_features + kOuts - 1) / kOuts;
-    p.tiles = a.tiles ? a.hdr[1] : (a.pairs + a.cap - 1) / a.cap;
-    p.units = (a.width + kUnit - 1) / kUnit;
+    const uint32_t nblocks = (uint32_t)((a.out_features + kOuts - 1) / kOuts), ctas = gridDim.x;
+    p.tiles = a.tiles ? (uint32_t)a.hdr[1] : (uint32_t)((a.pairs + a.cap - 1) / a.cap);
+    p.units = (uint32_t)((a.width + kUnit - 1) / kUnit);
     p.items = p.tiles * nblocks;
-    const int64_t waves = p.items / gridDim.x;
-    p.whole = p.items % gridDim.x == 0 ? p.items : waves > 1 ? (waves - 1) * gridDim.x : 0;
+    const uint32_t waves = p.items / ctas;
+    p.whole = p.items % ctas == 0 ? p.items : waves > 1 ? (waves - 1) * ctas : 0;
+    // under two waves of items, at most 2^11 units each: 32 bits hold all * runs
+    p.all = (p.items - p.whole) * p.units;
+    p.runs = max(1u, min(ctas, p.all));
     p.s0 = p.start(blockIdx.x);
     p.s1 = p.start(blockIdx.x + 1);
     return p;
@@ -108,33 +109,32 @@ __device__ __forceinline__ Plan make_plan(const ProductArgs &a) {
 
 // One CTA's part of an item: units [u0, u1).
 struct Part {
-    int64_t item;
+    uint32_t item;
     int u0, u1;
 };
 
-__device__ __forceinline__ bool part_of(const Plan &p, int i, Part &q) {
-    const int64_t mine = (p.whole + gridDim.x - 1 - blockIdx.x) / gridDim.x;
+__device__ __forceinline__ bool part_of(const Plan &p, uint32_t i, Part &q) {
+    const uint32_t mine = (p.whole + gridDim.x - 1 - blockIdx.x) / gridDim.x;
     if (i < mine) {
-        q.item = blockIdx.x + (int64_t)i * gridDim.x;
+        q.item = blockIdx.x + i * gridDim.x;
         q.u0 = 0;
         q.u1 = (int)p.units;
         return true;
     }
-    const int64_t it = p.s0 / p.units + (i - mine), base = it * p.units;
-    const int64_t u0 = max(p.s0, base) - base, u1 = min(p.s1, base + p.units) - base;
-    if (u0 >= u1 || it >= p.items - p.whole) return false;
+    const uint32_t it = p.s0 / p.units + (i - mine), base = it * p.units;
+    if (base >= p.s1 || p.s0 == p.s1) return false;
     q.item = p.whole + it;
-    q.u0 = (int)u0;
-    q.u1 = (int)u1;
+    q.u0 = (int)(max(p.s0, base) - base);
+    q.u1 = (int)(min(p.s1, base + p.units) - base);
     return true;
 }
 
-__device__ __forceinline__ int4 tile_of(const ProductArgs &a, const Plan &p, int64_t item,
+__device__ __forceinline__ int4 tile_of(const ProductArgs &a, const Plan &p, uint32_t item,
                                         int &out0) {
-    const int64_t t = item % p.tiles;
+    const uint32_t t = item % p.tiles;
     out0 = (int)(item / p.tiles) * kOuts;
     if (a.tiles) return a.tiles[t];
-    return make_int4(0, (int)(t * a.cap), (int)min((int64_t)a.cap, a.pairs - t * a.cap), 0);
+    return make_int4(0, (int)(t * a.cap), (int)min((int64_t)a.cap, a.pairs - (int64_t)t * a.cap), 0);
 }
 
 // The smallest box that holds `rows`.
@@ -153,6 +153,14 @@ __device__ __forceinline__ void store(const ProductArgs &a, int64_t i, float v) 
     if (a.y_dtype == IQK_F32) static_cast<float *>(a.y)[i] = v;
     else if (a.y_dtype == IQK_F16) static_cast<__half *>(a.y)[i] = from_float<__half>(v);
     else static_cast<__nv_bfloat16 *>(a.y)[i] = from_float<__nv_bfloat16>(v);
+}
+
+// Where the output row of the tile's row c + lane begins.
+__device__ __forceinline__ int64_t row_base(const ProductArgs &a, const int4 &tile, int c,
+                                            int lane) {
+    if (c + lane >= tile.z) return 0;
+    const int64_t pos = (int64_t)tile.y + c + lane;
+    return (a.order ? a.order[pos] : pos) * a.out_features;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -220,7 +228,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
             int g = 0;
             bool ok = true;
             Part q;
-            for (int i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
+            for (uint32_t i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
                 int out0;
                 const int4 tl = tile_of(a, plan, q.item, out0);
                 const int box = box_of(tl.z), rows = 16 << box;
@@ -256,7 +264,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
         int g = 0, n = 0;
         bool ok = true;
         Part q;
-        for (int i = 0; ok && part_of(plan, i, q); ++i, ++n) {
+        for (uint32_t i = 0; ok && part_of(plan, i, q); ++i, ++n) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int rows = 16 << box_of(tl.z);
@@ -301,7 +309,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
         int g = 0;
         bool ok = true;
         Part q;
-        for (int i = 0; ok && part_of(plan, i, q); ++i) {
+        for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int rows = 16 << box_of(tl.z);
@@ -341,7 +349,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
         const int r = 32 * quarter + lane;  // this thread's output of the item
         int n = 0;
         Part q;
-        for (int i = 0; part_of(plan, i, q); ++i, ++n) {
+        for (uint32_t i = 0; part_of(plan, i, q); ++i, ++n) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int acc = n & 1;
@@ -351,69 +359,73 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
                 break;
             }
             tc_fence_after();
-            const bool whole = q.u1 - q.u0 == plan.units;
+            const bool whole = (uint32_t)(q.u1 - q.u0) == plan.units;
             const bool there = out0 + r < a.out_features;
-            const int64_t shared_item = q.item - plan.whole;
-            float *slot = nullptr;
-            if (!whole)
-                slot = a.slots + ((int64_t)blockIdx.x * 2 +
-                                  (plan.s0 / plan.units == shared_item ? 0 : 1)) * cap * kOuts;
+            const uint32_t shared_item = q.item - plan.whole;
+            // a run's first item has the run's first slot, its last the second
+            const bool first = plan.s0 / plan.units == shared_item;
+            float *slot = a.slots + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * cap * kOuts;
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * cap;
-            for (int c = 0; c < tl.z; c += 8) {
-                uint32_t d[8];
-                tmem_ld8(src + c, d);
-                tc_wait_ld();
+            for (int c = 0; c < tl.z; c += 32) {
+                uint32_t d[4][8];
+                const int here = min(32, tl.z - c);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (c + j >= tl.z) continue;
-                    const float v = __uint_as_float(d[j]);
-                    if (!whole) {
-                        slot[(c + j) * kOuts + r] = v;
-                    } else if (there) {
-                        const int64_t pos = (int64_t)tl.y + c + j;
-                        const int64_t p = a.order ? a.order[pos] : pos;
-                        store(a, p * a.out_features + out0 + r, v);
+                for (int j = 0; j < 4; ++j)
+                    if (8 * j < here) tmem_ld8(src + c + 8 * j, d[j]);
+                tc_wait_ld();
+                if (whole) {
+                    const int64_t base = row_base(a, tl, c, lane);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (j >= here) break;
+                        const int64_t at = __shfl_sync(0xffffffffu, base, j);
+                        if (there) store(a, at + out0 + r, __uint_as_float(d[j >> 3][j & 7]));
                     }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < here) slot[(c + j) * kOuts + r] = __uint_as_float(d[j >> 3][j & 7]);
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&dempty[acc]);
             if (whole) continue;
-            // A shared item: the CTA that finishes last adds every part, in order.
-            const int64_t first_unit = shared_item * plan.units;
-            const int64_t last_unit = first_unit + plan.units - 1;
-            const int64_t all = (plan.items - plan.whole) * plan.units;
-            auto owner = [&](int64_t unit) {  // the CTA whose run holds the unit
-                int64_t c = unit * gridDim.x / all;
-                while (plan.start(c + 1) <= unit) ++c;
-                while (plan.start(c) > unit) --c;
-                return c;
+            // A shared item: the CTA that finishes last adds every part, in order
+            // (each warp for its 32 outputs: no warp waits for another).
+            const uint32_t first_unit = shared_item * plan.units;
+            auto owner = [&](uint32_t unit) {  // the CTA whose run holds the unit
+                uint32_t o = unit * plan.runs / plan.all;
+                while (plan.start(o + 1) <= unit) ++o;
+                while (plan.start(o) > unit) --o;
+                return o;
             };
-            const int64_t c0 = owner(first_unit), c1 = owner(last_unit);
-            // (each warp for its 32 outputs: no warp waits for another)
+            const uint32_t o0 = owner(first_unit), o1 = owner(first_unit + plan.units - 1);
             __threadfence();
             __syncwarp();
-            int last = 0;
-            if (lane == 0) {
-                int parts = 0;  // CTAs from c0 to c1 with a unit or more
-                for (int64_t c = c0; c <= c1; ++c) parts += plan.start(c + 1) > plan.start(c);
-                last = atomicAdd(&a.tickets[shared_item * 4 + quarter], 1) == parts - 1;
-            }
-            if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+            uint32_t done = 0;
+            if (lane == 0) done = (uint32_t)atomicAdd(&a.tickets[shared_item * 4 + quarter], 1);
+            if (__shfl_sync(0xffffffffu, done, 0) != o1 - o0) continue;
             __threadfence();
-            if (!there) continue;
-            for (int c = 0; c < tl.z; ++c) {
-                float v = 0.f;
-                for (int64_t o = c0; o <= c1; ++o) {
-                    const int64_t begin = plan.start(o);
-                    if (plan.start(o + 1) == begin) continue;
-                    v += __ldcg(a.slots + (o * 2 + (begin / plan.units == shared_item ? 0 : 1)) *
-                                              cap * kOuts + c * kOuts + r);
+            // the first owner's run may have begun in an earlier item
+            const bool early = plan.start(o0) / plan.units != shared_item;
+            for (int c = 0; c < tl.z; c += 8) {
+                float v[8] = {};
+                const int here = min(8, tl.z - c);
+#pragma unroll 2
+                for (uint32_t o = o0; o <= o1; ++o) {
+                    const float *part = a.slots +
+                        ((int64_t)o * 2 + (o == o0 && early ? 1 : 0)) * cap * kOuts + c * kOuts + r;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < here) v[j] += __ldcg(part + j * kOuts);
                 }
-                const int64_t pos = (int64_t)tl.y + c;
-                const int64_t p = a.order ? a.order[pos] : pos;
-                store(a, p * a.out_features + out0 + r, v);
+                const int64_t base = row_base(a, tl, c, lane);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t at = __shfl_sync(0xffffffffu, base, j);
+                    if (j < here && there) store(a, at + out0 + r, v[j]);
+                }
             }
         }
     }
@@ -462,12 +474,15 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
         off += (bytes + 255) & ~size_t(255);
         return at;
     };
-    // Rows of a tile: enough that an expert's rows mostly fit one (its matrix
-    // is then read once), and few for few rows, which leaves shared memory for
-    // more stages of the matrix.
+    // Rows of a tile. Enough that an expert's rows mostly fit one tile, whose
+    // matrix is then read once (an expert has `mean` rows or so), and fewer
+    // while the call has less than an item for each SM: small tiles spread over
+    // more SMs and have less to join.
+    const int64_t nblocks = (out_features + kOuts - 1) / kOuts;
+    const int64_t used = num_experts < pairs ? num_experts : pairs;
     const int64_t mean = pairs / num_experts;
-    L.cap = num_experts == 1 ? (pairs <= 16 ? 16 : pairs <= 64 ? 64 : 128)
-                             : (mean < 4 ? 16 : mean < 24 ? 64 : 128);
+    L.cap = num_experts == 1 || mean >= 24 ? 128 : mean >= 12 ? 64 : mean >= 4 ? 32 : 16;
+    while (L.cap > 16 && (used + (pairs - used) / L.cap) * nblocks < kMaxCtas) L.cap /= 2;
     L.pitch = (width / kMxBlock + 15) / 16 * 16;
     L.max_tiles = (num_experts < pairs ? num_experts : pairs) + pairs / L.cap + 1;
     L.hdr = take(64);
