@@ -239,7 +239,11 @@ def check_current(device: torch.device) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream as a handle; the raw query makes no Stream
+    object (0.1 us for 2.2 us a call)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if index is None else index)
 
 
 _PTR_ARRAYS: dict[tuple, ctypes.Array] = {}
@@ -544,37 +548,52 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def route(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int, renormalize: bool,
-          scale: float, indices, balance: bool):
-    """``iqk_route`` / ``iqk_route_balanced`` over logits ``rows [tokens, experts]``:
-    ``(indices, weights, loss, counts, slope)``, the last three None without
-    ``balance``. ``indices`` given (a choice already made): weights are None."""
-    lib, dev = library(), rows.device
+@functools.lru_cache(maxsize=1024)
+def balance_workspace_bytes(tokens: int, experts: int, segments: int) -> int:
+    return int(library().iqk_balance_workspace_bytes(tokens, experts, segments))
+
+
+def route(rows: torch.Tensor, mask, top_k: int, scoring: int, renormalize: bool, scale: float):
+    """``iqk_route`` over logits ``rows [tokens, experts]``: ``(indices, weights)``."""
+    dev = rows.device
     tokens, experts = rows.shape
+    indices = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    status = library().iqk_route(
+        rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
+        top_k, scoring, renormalize, scale, indices.data_ptr(), weights.data_ptr(),
+        stream_handle(dev))
+    if status:
+        raise_for_status(status, "iqk_route")
+    return indices, weights
+
+
+def route_balanced(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
+                   renormalize: bool, scale: float, indices=None):
+    """``iqk_route_balanced``: ``(indices, weights, loss, counts, slope)``. With
+    ``indices`` given (a choice already made) weights are None. ``slope``, which
+    the backward call reads, is a (pointer, owner) pair: it lies in the call's
+    workspace, one allocation for both."""
+    dev = rows.device
+    tokens, experts = rows.shape
+    segments = 1 if offsets is None else offsets.numel() - 1
     weights = None
     if indices is None:
         indices = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
         weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-    stream = stream_handle(dev)
-    if not balance:
-        status = lib.iqk_route(rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts,
-                               rows.stride(0), _ptr(mask), top_k, scoring, renormalize, scale,
-                               indices.data_ptr(), weights.data_ptr(), stream)
-        raise_for_status(status, "iqk_route")
-        return indices, weights, None, None, None
-    segments = 1 if offsets is None else offsets.numel() - 1
-    need = int(lib.iqk_balance_workspace_bytes(tokens, experts, segments))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    need = balance_workspace_bytes(tokens, experts, segments)
+    ws = torch.empty(need + 4 * segments * experts, dtype=torch.uint8, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty((segments, experts), dtype=torch.int32, device=dev)
-    slope = torch.empty((segments, experts), dtype=torch.float32, device=dev)
-    status = lib.iqk_route_balanced(
+    base = ws.data_ptr()
+    status = library().iqk_route_balanced(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         _ptr(offsets), segments, top_k, scoring, renormalize, scale, indices.data_ptr(),
-        _ptr(weights), loss.data_ptr(), counts.data_ptr(), slope.data_ptr(), ws.data_ptr(), need,
-        stream)
-    raise_for_status(status, "iqk_route_balanced")
-    return indices, weights, loss, counts, slope
+        _ptr(weights), loss.data_ptr(), counts.data_ptr(), base + need, base, need,
+        stream_handle(dev))
+    if status:
+        raise_for_status(status, "iqk_route_balanced")
+    return indices, weights, loss, counts, (base + need, ws)
 
 
 def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
@@ -590,19 +609,21 @@ def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
     status = library().iqk_route_backward(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         _ptr(offsets), 1 if offsets is None else offsets.numel() - 1, top_k, scoring, renormalize,
-        scale, indices.data_ptr(), _ptr(grad_weights), _ptr(slope), _ptr(grad_loss),
-        grad.data_ptr(), stream_handle(rows.device))
-    raise_for_status(status, "iqk_route_backward")
+        scale, indices.data_ptr(), _ptr(grad_weights), slope[0] if slope else None,
+        _ptr(grad_loss), grad.data_ptr(), stream_handle(rows.device))
+    if status:
+        raise_for_status(status, "iqk_route_backward")
     return grad
 
 
-def mx_quantize(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
-                scale_stride: int) -> None:
-    """``iqk_mx_quantize``: float rows ``[rows, width]`` into ``codes`` and ``scales``."""
+def mx_quantize(x: torch.Tensor, rows: int, row_stride: int, codes: torch.Tensor,
+                scales: torch.Tensor, scale_stride: int) -> None:
+    """``iqk_mx_quantize``: ``rows`` rows of ``x``, ``row_stride`` elements apart."""
     status = library().iqk_mx_quantize(
-        rows.data_ptr(), DTYPE_IDS[rows.dtype], rows.shape[0], rows.shape[1], rows.stride(0),
-        codes.data_ptr(), scales.data_ptr(), scale_stride, stream_handle(rows.device))
-    raise_for_status(status, "iqk_mx_quantize")
+        x.data_ptr(), DTYPE_IDS[x.dtype], rows, x.shape[-1], row_stride, codes.data_ptr(),
+        scales.data_ptr(), scale_stride, stream_handle(x.device))
+    if status:
+        raise_for_status(status, "iqk_mx_quantize")
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, scale_stride: int,
@@ -612,7 +633,8 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, scale_stride: int,
     status = library().iqk_mx_dequantize(
         codes.data_ptr(), scales.data_ptr(), scale_stride, out.numel() // width, width,
         out.data_ptr(), DTYPE_IDS[out.dtype], stream_handle(out.device))
-    raise_for_status(status, "iqk_mx_dequantize")
+    if status:
+        raise_for_status(status, "iqk_mx_dequantize")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -620,33 +642,36 @@ def mx_workspace_bytes(pairs: int, num_experts: int, width: int, out_features: i
     return int(library().iqk_mx_workspace_bytes(pairs, num_experts, width, out_features))
 
 
-def mx_linear(rows: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, scale_stride: int,
-              out_features: int, y: torch.Tensor) -> None:
-    """``iqk_mx_linear``: ``y [rows, out] = q(rows) W^T``."""
-    count, width = rows.shape
-    need = mx_workspace_bytes(count, 1, width, out_features)
-    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
+def mx_linear(x: torch.Tensor, rows: int, row_stride: int, codes: torch.Tensor,
+              scales: torch.Tensor, scale_stride: int, y: torch.Tensor) -> None:
+    """``iqk_mx_linear``: ``y [rows, out] = q(x) W^T``."""
+    width, out_features = x.shape[-1], codes.shape[0]
+    need = mx_workspace_bytes(rows, 1, width, out_features)
+    ws = torch.empty(need, dtype=torch.uint8, device=y.device)
     status = library().iqk_mx_linear(
-        rows.data_ptr(), DTYPE_IDS[rows.dtype], count, rows.stride(0), codes.data_ptr(),
-        scales.data_ptr(), scale_stride, out_features, width, y.data_ptr(), DTYPE_IDS[y.dtype],
-        ws.data_ptr(), ws.numel(), stream_handle(y.device))
-    raise_for_status(status, "iqk_mx_linear")
+        x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, codes.data_ptr(), scales.data_ptr(),
+        scale_stride, out_features, width, y.data_ptr(), DTYPE_IDS[y.dtype], ws.data_ptr(), need,
+        stream_handle(y.device))
+    if status:
+        raise_for_status(status, "iqk_mx_linear")
 
 
-def mx_routed(rows: torch.Tensor, sel: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
-              scale_stride: int, y: torch.Tensor, workspace: torch.Tensor | None = None) -> None:
+def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
+              codes: torch.Tensor, scales: torch.Tensor, scale_stride: int, y: torch.Tensor,
+              workspace: torch.Tensor | None = None) -> None:
     """``iqk_mx_routed``: ``y [pairs, out]`` through the stacked matrices."""
-    pairs, width = sel.numel(), rows.shape[1]
+    pairs, width = sel.numel(), x.shape[-1]
     experts, out_features = codes.shape[0], codes.shape[1]
     if workspace is None:
         need = mx_workspace_bytes(pairs, experts, width, out_features)
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
     status = library().iqk_mx_routed(
-        rows.data_ptr(), DTYPE_IDS[rows.dtype], rows.shape[0], rows.stride(0), sel.data_ptr(),
-        pairs, codes.data_ptr(), scales.data_ptr(), scale_stride, experts, out_features, width,
+        x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, sel.data_ptr(), pairs,
+        codes.data_ptr(), scales.data_ptr(), scale_stride, experts, out_features, width,
         y.data_ptr(), DTYPE_IDS[y.dtype], workspace.data_ptr(), workspace.numel(),
         stream_handle(y.device))
-    raise_for_status(status, "iqk_mx_routed")
+    if status:
+        raise_for_status(status, "iqk_mx_routed")
 
 
 def mx_read_error(workspace: torch.Tensor) -> int:

@@ -37,23 +37,28 @@ MX_BLOCK = 32
 
 
 def _rows(x, what="x"):
-    """``x`` as float rows ``[rows, width]`` whose columns are adjacent."""
+    """``(x, rows, row_stride)`` of float rows whose columns are adjacent: ``x``
+    itself, or a copy where its layout is not one of evenly spaced rows."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise IqkRuntimeError(f"{what} must be a tensor on the GPU")
     if x.dtype not in K.DTYPE_IDS:
         raise IqkRuntimeError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise IqkRuntimeError(f"the MXFP4 operators carry no gradient: detach {what}")
-    if x.dim() < 1 or x.shape[-1] <= 0 or x.shape[-1] % MX_BLOCK:
+    width = x.shape[-1] if x.dim() else 0
+    if width <= 0 or width % MX_BLOCK:
         raise IqkKernelError(
             f"{what} must have a width that is a positive multiple of {MX_BLOCK}, "
             f"got shape {tuple(x.shape)}")
     K.check_current(x.device)
-    rows = x.reshape(-1, x.shape[-1])
-    if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]
-                               and rows.stride(0) != 0):
-        rows = rows.contiguous()
-    return rows
+    count = x.numel() // width
+    if x.is_contiguous():
+        return x, count, width
+    rows = x.reshape(-1, width)
+    step, inner = rows.stride()
+    if inner != 1 or (count > 1 and 0 != step < width):
+        return rows.contiguous(), count, width
+    return rows, count, step
 
 
 def _matrix(codes, scales, dims, device=None):
@@ -65,31 +70,26 @@ def _matrix(codes, scales, dims, device=None):
             raise IqkRuntimeError(f"{name} must be uint8, got {t.dtype}")
     if codes.device != scales.device or (device is not None and codes.device != device):
         raise IqkRuntimeError("codes, scales and activations must be on one device")
-    if codes.dim() < 1 or (dims and codes.dim() != dims):
-        raise IqkRuntimeError(f"codes must have {dims or 'at least 1'} axes, got {codes.dim()}")
-    blocks = scales.shape[-1] if scales.dim() else 0
-    if scales.shape[:-1] != codes.shape[:-1] or codes.shape[-1] != blocks * MX_BLOCK // 2 \
-            or blocks == 0:
+    shape, lead = codes.shape, scales.shape
+    if not shape or (dims and len(shape) != dims):
+        raise IqkRuntimeError(f"codes must have {dims or 'at least 1'} axes, got {len(shape)}")
+    blocks = lead[-1] if lead else 0
+    if lead[:-1] != shape[:-1] or shape[-1] != blocks * MX_BLOCK // 2 or blocks == 0:
         raise IqkRuntimeError(
-            f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not belong "
+            f"codes {tuple(shape)} and scales {tuple(lead)} do not belong "
             f"together: {MX_BLOCK // 2} code bytes to a scale")
     if not codes.is_contiguous() or codes.data_ptr() % 16:
         raise IqkRuntimeError("codes must be contiguous and 16-byte aligned")
-    if scales.numel() == blocks:  # one row: any stride will do
-        stride = (blocks + 15) // 16 * 16
-        packed = True
-    else:
-        stride, packed = None, True
-        step = None
-        for axis in range(scales.dim() - 2, -1, -1):
-            if scales.shape[axis] == 1:
-                continue
-            if step is None:
-                stride = step = scales.stride(axis)
-            packed = packed and scales.stride(axis) == step
-            step = step * scales.shape[axis]
-    if blocks > 1 and scales.stride(-1) != 1 or not packed or stride % 16 \
-            or stride < blocks or scales.data_ptr() % 16:
+    steps = scales.stride()
+    stride, step, packed = (blocks + 15) // 16 * 16, None, blocks == 1 or steps[-1] == 1
+    for axis in range(len(lead) - 2, -1, -1):  # one row, or no axis longer than 1: any stride
+        if lead[axis] == 1:
+            continue
+        if step is None:
+            stride = step = steps[axis]
+        packed = packed and steps[axis] == step
+        step *= lead[axis]
+    if not packed or stride % 16 or stride < blocks or scales.data_ptr() % 16:
         raise IqkRuntimeError(
             "scale rows must be evenly spaced and start on 16-byte boundaries "
             "(mx_aligned_scales lays packed scales out so)")
@@ -118,11 +118,11 @@ def mx_quantize(x):
     (``2^-127`` at least); values round to the nearest code, ties to the even
     one, and hold at 6 beyond it. A block with a NaN or an infinity gets scale
     byte 255: all of it reads NaN."""
-    rows = _rows(x)
-    width = x.shape[-1]
-    codes = torch.empty(x.shape[:-1] + (width // 2,), dtype=torch.uint8, device=x.device)
-    scales = _scale_rows(x.shape[:-1], width // MX_BLOCK, x.device)
-    K.mx_quantize(rows, codes, scales, (width // MX_BLOCK + 15) // 16 * 16)
+    rows, count, step = _rows(x)
+    *lead, width = x.shape
+    codes = torch.empty((*lead, width // 2), dtype=torch.uint8, device=x.device)
+    scales = _scale_rows(lead, width // MX_BLOCK, x.device)
+    K.mx_quantize(rows, count, step, codes, scales, (width // MX_BLOCK + 15) // 16 * 16)
     return codes, scales
 
 
@@ -133,8 +133,8 @@ def mx_dequantize(codes, scales, dtype: torch.dtype = torch.float32) -> torch.Te
     if dtype not in K.DTYPE_IDS:
         raise IqkRuntimeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     K.check_current(codes.device)
-    width = codes.shape[-1] * 2
-    out = torch.empty(codes.shape[:-1] + (width,), dtype=dtype, device=codes.device)
+    *lead, half = codes.shape
+    out = torch.empty((*lead, half * 2), dtype=dtype, device=codes.device)
     K.mx_dequantize(codes, scales, stride, out)
     return out
 
@@ -149,14 +149,15 @@ def _out_dtype(x, out_dtype):
 def mx_linear(x, codes, scales, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``q(x) W^T`` ``[..., out]`` for ``x [..., width]`` and ``W`` = ``codes [out,
     width / 2]``, ``scales [out, width / 32]``; ``q`` is :func:`mx_quantize`."""
-    rows = _rows(x)
+    rows, count, step = _rows(x)
     stride = _matrix(codes, scales, 2, x.device)
-    if codes.shape[-1] * 2 != x.shape[-1]:
-        raise IqkRuntimeError(f"x of width {x.shape[-1]} meets a matrix of {codes.shape[-1] * 2}")
-    out = codes.shape[0]
-    y = torch.empty(x.shape[:-1] + (out,), dtype=_out_dtype(x, out_dtype), device=x.device)
-    if y.numel():
-        K.mx_linear(rows, codes, scales, stride, out, y)
+    out, half = codes.shape
+    *lead, width = x.shape
+    if half * 2 != width:
+        raise IqkRuntimeError(f"x of width {width} meets a matrix of {half * 2}")
+    y = torch.empty((*lead, out), dtype=_out_dtype(x, out_dtype), device=x.device)
+    if count and out:
+        K.mx_linear(rows, count, step, codes, scales, stride, y)
     return y
 
 
@@ -173,25 +174,25 @@ def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = 
     experts, which also sets ``DEVERR_EXPERT`` in a caller's ``workspace``
     (uint8, ``kernels.mx_workspace_bytes``), read by
     ``kernels.mx_read_error``."""
-    rows = _rows(x)
+    rows, count, step = _rows(x)
     stride = _matrix(codes, scales, 3, x.device)
     if not isinstance(indices, torch.Tensor) or indices.device != x.device \
             or indices.dtype not in (torch.int32, torch.int64):
         raise IqkRuntimeError("indices must be an int32 or int64 tensor beside x")
-    if codes.shape[-1] * 2 != x.shape[-1]:
-        raise IqkRuntimeError(f"x of width {x.shape[-1]} meets matrices of {codes.shape[-1] * 2}")
+    experts, out, half = codes.shape
+    if half * 2 != x.shape[-1]:
+        raise IqkRuntimeError(f"x of width {x.shape[-1]} meets matrices of {half * 2}")
     sel = indices.to(torch.int32).contiguous()
-    pairs, out = sel.numel(), codes.shape[1]
-    y = torch.empty(tuple(indices.shape) + (1, out), dtype=_out_dtype(x, out_dtype),
-                    device=x.device)
-    if pairs and (rows.shape[0] == 0 or pairs % rows.shape[0]):
+    pairs = sel.numel()
+    if pairs and (count == 0 or pairs % count):
         raise IqkRuntimeError(
-            f"{pairs} token-expert pairs do not tile {rows.shape[0]} activation "
+            f"{pairs} token-expert pairs do not tile {count} activation "
             f"row(s); the operand and the routing disagree")
-    if y.numel():
-        if codes.shape[0] == 0:
+    y = torch.empty((*indices.shape, 1, out), dtype=_out_dtype(x, out_dtype), device=x.device)
+    if pairs and out:
+        if experts == 0:
             return y.zero_()
-        K.mx_routed(rows, sel, codes, scales, stride, y, workspace)
+        K.mx_routed(rows, count, step, sel, codes, scales, stride, y, workspace)
     return y
 
 

@@ -68,41 +68,46 @@ def _check(logits, top_k, scoring, mask, offsets=None):
 
 
 class _Route(torch.autograd.Function):
-    """Choice and balance loss with one gradient kernel. ``indices`` None: chosen here."""
+    """Choice and, with ``balance``, balance loss: one gradient kernel for both.
+    ``given`` holds what is no input of the graph: the logits as rows, a choice
+    already made (or None), mask and offsets; ``call`` the plain arguments."""
 
     @staticmethod
-    def forward(ctx, logits, rows, indices, top_k, scoring, renormalize, scale, mask, offsets,
-                balance):
+    def forward(ctx, logits, given, call, balance):
         ctx.set_materialize_grads(False)
+        rows, indices, mask, offsets = given
         choose = indices is None
-        indices, weights, loss, counts, slope = K.route(
-            rows, mask, offsets, top_k, scoring, renormalize, scale, indices, balance)
-        ctx.call = (top_k, scoring, renormalize, scale, logits.shape)
-        ctx.save_for_backward(rows, mask, offsets, indices, slope)
-        ctx.mark_non_differentiable(*(t for t in (indices if choose else None, counts)
-                                      if t is not None))
+        if balance:
+            indices, weights, loss, counts, ctx.slope = K.route_balanced(
+                rows, mask, offsets, *call, indices)
+            ctx.mark_non_differentiable(*((indices, counts) if choose else (counts,)))
+        else:
+            indices, weights = K.route(rows, mask, *call)
+            loss = counts = ctx.slope = None
+            ctx.mark_non_differentiable(indices)
+        ctx.call = call
+        ctx.save_for_backward(logits, indices, mask, offsets)
+        # rows is logits itself, or the copy that made its columns adjacent
+        ctx.rows = None if rows is logits else rows
         return (indices if choose else None), weights, loss, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, _indices, grad_weights, grad_loss, _counts):
-        rows, mask, offsets, indices, slope = ctx.saved_tensors
-        top_k, scoring, renormalize, scale, shape = ctx.call
-        if grad_loss is None:
-            slope = None
+        logits, indices, mask, offsets = ctx.saved_tensors
+        slope = None if grad_loss is None else ctx.slope
         if grad_weights is None and slope is None:
-            return (None,) * 10
-        grad = K.route_backward(rows, mask, offsets, top_k, scoring, renormalize, scale, indices,
-                                grad_weights, slope, grad_loss)
-        return (grad.view(shape),) + (None,) * 9
+            return None, None, None, None
+        grad = K.route_backward(logits if ctx.rows is None else ctx.rows, mask, offsets,
+                                *ctx.call, indices, grad_weights, slope, grad_loss)
+        return grad if logits.dim() == 2 else grad.view(logits.shape), None, None, None
 
 
-def _run(logits, indices, top_k, scoring, renormalize, scale, mask, offsets, balance):
-    rows, mask, offsets, scoring = _check(logits, top_k, scoring, mask, offsets)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _Route.apply(logits, rows.detach(), indices, top_k, scoring, renormalize, scale,
-                            mask, offsets, balance)
-    return K.route(rows, mask, offsets, top_k, scoring, renormalize, scale, indices, balance)[:4]
+def _shaped(logits, top_k, indices, weights):
+    if logits.dim() == 2:
+        return indices, weights
+    shape = logits.shape[:-1] + (top_k,)
+    return indices.view(shape), weights.view(shape)
 
 
 def route(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = True,
@@ -111,24 +116,26 @@ def route(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = T
     [..., experts]``: the ``top_k`` largest in falling order (equal ones by
     index), and ``scale`` times their scores, divided by the scores' sum when
     ``renormalize``. Differentiable in ``logits`` through the weights."""
-    indices, weights, _, _ = _run(logits, None, top_k, scoring, renormalize, scale, mask, None,
-                                  False)
-    if logits.dim() == 2:
-        return indices, weights
-    shape = logits.shape[:-1] + (top_k,)
-    return indices.view(shape), weights.view(shape)
+    rows, mask, _, scoring = _check(logits, top_k, scoring, mask)
+    call = (top_k, scoring, renormalize, scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _Route.apply(logits, (rows, None, mask, None), call, False)
+    else:
+        out = K.route(rows, mask, *call)
+    return _shaped(logits, top_k, out[0], out[1])
 
 
 def route_balanced(logits, top_k: int, *, scoring: str = "softmax", renormalize: bool = True,
                    scale: float = 1.0, mask=None, offsets=None):
     """``(indices, weights, loss, counts)``: :func:`route` and :func:`balance_loss`
     in one pass over the logits, forward and backward."""
-    indices, weights, loss, counts = _run(logits, None, top_k, scoring, renormalize, scale, mask,
-                                          offsets, True)
-    if logits.dim() != 2:
-        shape = logits.shape[:-1] + (top_k,)
-        indices, weights = indices.view(shape), weights.view(shape)
-    return indices, weights, loss, counts
+    rows, mask, offsets, scoring = _check(logits, top_k, scoring, mask, offsets)
+    call = (top_k, scoring, renormalize, scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = _Route.apply(logits, (rows, None, mask, offsets), call, True)
+    else:
+        out = K.route_balanced(rows, mask, offsets, *call)
+    return *_shaped(logits, top_k, out[0], out[1]), out[2], out[3]
 
 
 def balance_loss(logits, indices, *, scoring: str = "softmax", mask=None, offsets=None):
@@ -150,8 +157,12 @@ def balance_loss(logits, indices, *, scoring: str = "softmax", mask=None, offset
     if indices.device != logits.device:
         raise IqkRuntimeError("indices must be on the logits' device")
     top_k = indices.shape[-1]
+    rows, mask, offsets, scoring = _check(logits, top_k, scoring, mask, offsets)
     sel = indices.to(torch.int32).contiguous()
-    return _run(logits, sel, top_k, scoring, True, 1.0, mask, offsets, True)[2:]
+    call = (top_k, scoring, True, 1.0)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, (rows, sel, mask, offsets), call, True)[2:]
+    return K.route_balanced(rows, mask, offsets, *call, sel)[2:4]
 
 
 __all__ = ["MAX_EXPERTS", "MAX_TOP_K", "balance_loss", "route", "route_balanced"]
