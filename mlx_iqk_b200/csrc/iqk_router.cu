@@ -1,8 +1,7 @@
 // Expert router: top-k choice with router weights, per-expert counts and the
 // balance loss, and their gradient (sm_100a).
 //
-// One token's logits z[0..E) are one warp's registers (lane l holds experts
-// l, l + 32, ...). With u(z) = exp(z) for softmax scoring and the logistic
+// One token's logits z[0..E) are one warp's registers. With u(z) = exp(z) for softmax scoring and the logistic
 // function for sigmoid scoring, every quantity of a row is a ratio of
 //
 //   r_e = u(z_e) / u(c),  c the row's largest logit (softmax) or min(it, 0)
@@ -27,8 +26,9 @@
 //   sigmoid        dz_i_j += scale q_j (1 - q_j) g_j
 //
 // Sums over rows are joined in a fixed order: a block writes one record per
-// segment that it meets, and the finishing kernel adds the records in block
-// order, so a result does not depend on which block ran first.
+// segment that it meets, and the finishing kernel adds the records in an order
+// that its launch alone decides, so a result repeats bit for bit.
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include "iqk_common.cuh"
@@ -56,7 +56,7 @@ struct RouteArgs {
     float *rec_score;        // [records, experts]
     int32_t *rec_count;      // [records, experts]
     int32_t *rec_rows;       // [records]
-    int64_t per_block;       // rows of one block
+    int64_t per_block;       // rows of one block (backward: of one warp)
 };
 
 __device__ __forceinline__ float logistic(float z) { return 1.f / (1.f + expf(-z)); }
@@ -86,6 +86,22 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
 }
 
+// A 16-bit logit's ordered bits in the upper 22 of a word (the low ten are
+// free for the expert), and back.
+template <typename T> __device__ __forceinline__ uint32_t key16(float z, uint32_t key) {
+    if (sizeof(T) == 4) return key;
+    if (z != z) return 0xffff0000u;
+    const T v = from_float<T>(z + 0.f);
+    const uint32_t b = *reinterpret_cast<const uint16_t *>(&v);
+    return ((b >> 15) ? (~b & 0xffffu) : (b | 0x8000u)) << 16;
+}
+template <typename T> __device__ __forceinline__ float value16(uint32_t key) {
+    const uint32_t k = key >> 16;
+    if (sizeof(T) == 4 || k == 0xffffu) return CUDART_NAN_F;
+    const uint16_t b = (uint16_t)((k >> 15) ? k & 0x7fffu : ~k);
+    return to_float<T>(*reinterpret_cast<const T *>(&b));
+}
+
 // The segment of row t and the row after that segment's end: the largest g
 // with offsets[g] <= t. -1 or `segments`: no segment.
 __device__ __forceinline__ int segment_of(const int32_t *offsets, int segments, int64_t t,
@@ -101,14 +117,32 @@ __device__ __forceinline__ int segment_of(const int32_t *offsets, int segments, 
     return lo - 1;
 }
 
-// Lane l's experts l + 32 i of one row; places past E read -inf.
-template <typename T, int V>
+// Value i of lane l is expert (i / N) 32 N + l N + i % N: N values to a load
+// (16 bytes where rows allow it, else one).
+template <int N> __device__ __forceinline__ int expert_of(int lane, int i) {
+    return (i / N) * 32 * N + lane * N + i % N;
+}
+
+// One row; places past E read -inf.
+template <typename T, int V, int N>
 __device__ __forceinline__ void load_row(const RouteArgs &a, int64_t t, int lane, float (&z)[V]) {
     const T *row = static_cast<const T *>(a.logits) + t * a.stride;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int e = lane + 32 * i;
-        z[i] = e < a.experts ? to_float<T>(row[e]) : -CUDART_INF_F;
+    for (int i = 0; i < V; i += N) {
+        const int e = expert_of<N>(lane, i);
+        if constexpr (N == 1) {
+            z[i] = e < a.experts ? to_float<T>(row[e]) : -CUDART_INF_F;
+        } else {  // E is a multiple of N
+            if (e < a.experts) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(row + e);
+                const T *v = reinterpret_cast<const T *>(&u);
+#pragma unroll
+                for (int j = 0; j < N; ++j) z[i + j] = to_float<T>(v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) z[i + j] = -CUDART_INF_F;
+            }
+        }
     }
 }
 
@@ -120,12 +154,19 @@ template <int V> __device__ __forceinline__ uint32_t row_peak(const float (&z)[V
 }
 
 // The top_k largest of the row: lane j gets choice j (index -1 past the last).
-template <int V>
+// 16-bit logits have 16-bit keys: key and 1023 - expert share a word, and one
+// warp maximum finds the largest and, among equals, the first. 32-bit keys take
+// a second one for the expert.
+template <typename T, int V, int N>
 __device__ __forceinline__ void choose(const RouteArgs &a, const float (&z)[V], int lane,
                                        int &index, float &value) {
+    constexpr bool kPacked = sizeof(T) == 2;
     uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
+    for (int i = 0; i < V; ++i) {
+        key[i] = key_of(z[i]);
+        if (kPacked && key[i]) key[i] = key16<T>(z[i], key[i]) | (1023u - expert_of<N>(lane, i));
+    }
     index = -1;
     value = -CUDART_INF_F;
     for (int j = 0; j < a.top_k; ++j) {
@@ -134,22 +175,30 @@ __device__ __forceinline__ void choose(const RouteArgs &a, const float (&z)[V], 
         for (int i = 0; i < V; ++i) best = max(best, key[i]);
         const uint32_t top = __reduce_max_sync(kFull, best);
         if (top == 0) break;
-        int first = kMaxExperts;
+        int first;
+        if (kPacked) {
+            first = 1023 - (int)(top & 1023u);
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i)
-            if (key[i] == top) first = lane + 32 * i;
-        first = __reduce_min_sync(kFull, first);
+            for (int i = 0; i < V; ++i)
+                if (key[i] == top) key[i] = 0;
+        } else {
+            first = kMaxExperts;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (first == lane + 32 * i) key[i] = 0;
+            for (int i = V - 1; i >= 0; --i)
+                if (key[i] == top) first = expert_of<N>(lane, i);
+            first = __reduce_min_sync(kFull, first);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (first == expert_of<N>(lane, i)) key[i] = 0;
+        }
         if (lane == j) {
             index = first;
-            value = value_of(top);
+            value = kPacked ? value16<T>(top) : value_of(top);
         }
     }
 }
 
-template <typename T, int V, bool CHOOSE, bool BALANCE>
+template <typename T, int V, int N, bool CHOOSE, bool BALANCE>
 __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lane,
                                           float (&score)[V], int &index) {
     const int k = a.top_k;
@@ -161,7 +210,7 @@ __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lan
         return false;
     }
     float z[V];
-    load_row<T, V>(a, t, lane, z);
+    load_row<T, V, N>(a, t, lane, z);
     const uint32_t peak = row_peak<V>(z);
     const float top = value_of(peak);
     const float c = a.sigmoid ? fminf(top, 0.f) : top;
@@ -177,7 +226,7 @@ __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lan
     }
     if (CHOOSE) {
         float value, w;
-        choose<V>(a, z, lane, index, value);
+        choose<T, V, N>(a, z, lane, index, value);
         if (a.renormalize) {
             const float r = index >= 0 ? ratio(value, c, a.sigmoid) : 0.f;
             w = r / warp_sum(r);
@@ -200,21 +249,26 @@ __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lan
 }
 
 // A warp a row.
-template <typename T, int V> __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
+template <typename T, int V, int N>
+__global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     const int lane = threadIdx.x & 31;
     const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
     for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.tokens;
          t += step) {
         float score[V];
         int index;
-        route_row<T, V, true, false>(a, t, lane, score, index);
+        route_row<T, V, N, true, false>(a, t, lane, score, index);
     }
 }
 
 // A block takes per_block rows in a run; its warps share the rows of each
 // segment part, and the part's sums become one record.
-template <typename T, int V, bool CHOOSE>
-__global__ void __launch_bounds__(256) balance_kernel(RouteArgs a) {
+// Warps of a balance block: a row's registers and the warps' sums (48 KB of
+// shared memory at most) bound them.
+__host__ __device__ constexpr int balance_warps(int v) { return v <= 8 ? 32 : v <= 16 ? 16 : 8; }
+
+template <typename T, int V, int N, bool CHOOSE>
+__global__ void __launch_bounds__(32 * balance_warps(V)) balance_kernel(RouteArgs a) {
     extern __shared__ float sums[];  // [warps, experts], then the counts
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int32_t *counts = reinterpret_cast<int32_t *>(sums + warps * a.experts);
@@ -234,7 +288,7 @@ __global__ void __launch_bounds__(256) balance_kernel(RouteArgs a) {
         for (int64_t t = t0 + warp; t < t1; t += warps) {
             float score[V];
             int index = -1;
-            if (!route_row<T, V, CHOOSE, true>(a, t, lane, score, index)) continue;
+            if (!route_row<T, V, N, CHOOSE, true>(a, t, lane, score, index)) continue;
             ++mine;
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] += score[i];
@@ -243,7 +297,8 @@ __global__ void __launch_bounds__(256) balance_kernel(RouteArgs a) {
         if (lane == 0) atomicAdd(&rows, mine);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (lane + 32 * i < a.experts) sums[warp * a.experts + lane + 32 * i] = acc[i];
+            if (expert_of<N>(lane, i) < a.experts)
+                sums[warp * a.experts + expert_of<N>(lane, i)] = acc[i];
         __syncthreads();
         if (g >= 0 && g < a.segments) {
             const int64_t rec = blockIdx.x + g;
@@ -260,61 +315,94 @@ __global__ void __launch_bounds__(256) balance_kernel(RouteArgs a) {
     }
 }
 
-// The rows [first, last] of blocks that hold a part of segment g.
-__device__ __forceinline__ bool blocks_of(const RouteArgs &a, int g, int64_t &first,
-                                          int64_t &last) {
+// The blocks [first, last] that hold a part of segment g; false: no row.
+__device__ __forceinline__ bool blocks_of(const RouteArgs &a, int g, int &first, int &last) {
     const int64_t lo = a.offsets ? max(a.offsets[g], 0) : 0;
     const int64_t hi = a.offsets ? min((int64_t)a.offsets[g + 1], a.tokens) : a.tokens;
     if (lo >= hi) return false;
-    first = lo / a.per_block;
-    last = (hi - 1) / a.per_block;
+    first = (int)(lo / a.per_block);
+    last = (int)((hi - 1) / a.per_block);
     return true;
 }
 
-// One block: counts, mean scores, the loss, and slope_ge = f_ge / (N_g G').
-__global__ void __launch_bounds__(1024)
+constexpr int kFinishCtas = 8, kFinishWarps = 16;
+
+// The rows of segment g that count, summed by a whole warp.
+__device__ __forceinline__ int rows_of(const RouteArgs &a, int g, int lane) {
+    int first, last, n = 0;
+    if (!blocks_of(a, g, first, last)) return 0;
+    for (int b = first + lane; b <= last; b += 32) n += a.rec_rows[b + g];
+    return __reduce_add_sync(kFull, n);
+}
+
+// Counts, mean scores, the loss, and slope_ge = f_ge / (N_g G'). A cluster of
+// eight CTAs shares the experts; in a CTA `share` warps split a segment's
+// records (all 16 for one segment, one for 16 or more) and lanes are experts.
+__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(32 * kFinishWarps)
 balance_finish_kernel(RouteArgs a, float *loss, int32_t *counts, float *slope) {
-    __shared__ float red[32];
+    __shared__ float scores[kFinishWarps][32], part_sum[kFinishWarps], total;
+    __shared__ int32_t picked[kFinishWarps][32];
     __shared__ int filled;
-    const int tid = threadIdx.x, nt = blockDim.x;
-    if (tid == 0) filled = 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) filled = 0;
     __syncthreads();
     int mine = 0;
-    for (int g = tid; g < a.segments; g += nt) {
-        int64_t b0, b1, n = 0;
-        if (!blocks_of(a, g, b0, b1)) continue;
-        for (int64_t b = b0; b <= b1; ++b) n += a.rec_rows[b + g];
-        mine += n > 0;
-    }
-    if (mine) atomicAdd(&filled, mine);
+    for (int g = warp; g < a.segments; g += kFinishWarps) mine += rows_of(a, g, lane) > 0;
+    if (lane == 0 && mine) atomicAdd(&filled, mine);
     __syncthreads();
-    const float share = 1.f / (float)max(filled, 1);
+    const float mean = 1.f / (float)max(filled, 1);
+    int share = kFinishWarps;
+    while (share > 1 && share * a.segments > kFinishWarps) share >>= 1;
+    const int sub = warp % share;
     float part = 0.f;
-    for (int g = 0; g < a.segments; ++g) {
-        int64_t b0 = 0, b1 = -1, n = 0;
-        blocks_of(a, g, b0, b1);
-        for (int64_t b = b0; b <= b1; ++b) n += a.rec_rows[b + g];
+    for (int g0 = 0; g0 < a.segments; g0 += kFinishWarps / share) {
+        const int g = g0 + warp / share;
+        int first = 0, last = -1, n = 0;
+        if (g < a.segments && blocks_of(a, g, first, last)) n = rows_of(a, g, lane);
         const float inv = n > 0 ? 1.f / (float)n : 0.f;
-        for (int e = tid; e < a.experts; e += nt) {
+        for (int e0 = blockIdx.x * 32; e0 < a.experts; e0 += kFinishCtas * 32) {
+            const int e = e0 + lane;
             float s = 0.f;
-            int64_t c = 0;
-            for (int64_t b = b0; b <= b1; ++b) {
-                s += a.rec_score[(b + g) * a.experts + e];
-                c += a.rec_count[(b + g) * a.experts + e];
+            int c = 0;
+            if (e < a.experts) {
+#pragma unroll 4
+                for (int b = first + sub; b <= last; b += share) {
+                    s += a.rec_score[(int64_t)(b + g) * a.experts + e];
+                    c += a.rec_count[(int64_t)(b + g) * a.experts + e];
+                }
             }
-            const float f = (float)c * (float)a.experts * inv / (float)a.top_k;
-            part += f * s * inv;
-            counts[(int64_t)g * a.experts + e] = (int32_t)c;
-            slope[(int64_t)g * a.experts + e] = f * inv * share;
+            scores[warp][lane] = s;
+            picked[warp][lane] = c;
+            __syncthreads();
+            if (sub == 0 && g < a.segments && e < a.experts) {
+                for (int w = 1; w < share; ++w) {
+                    s += scores[warp + w][lane];
+                    c += picked[warp + w][lane];
+                }
+                const float f = (float)c * (float)a.experts * inv / (float)a.top_k;
+                part += f * s * inv;
+                counts[(int64_t)g * a.experts + e] = c;
+                slope[(int64_t)g * a.experts + e] = f * inv * mean;
+            }
+            __syncthreads();
         }
     }
     part = warp_sum(part);
-    if ((tid & 31) == 0) red[tid >> 5] = part;
+    if (lane == 0) part_sum[warp] = part;
     __syncthreads();
-    if (tid < 32) {
-        part = warp_sum(tid < (nt >> 5) ? red[tid] : 0.f);
-        if (tid == 0) *loss = part * share;
+    if (threadIdx.x == 0) {
+        float v = 0.f;
+        for (int w = 0; w < kFinishWarps; ++w) v += part_sum[w];
+        total = v * mean;
     }
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        float v = 0.f;
+        for (int c = 0; c < kFinishCtas; ++c) v += *cluster.map_shared_rank(&total, c);
+        *loss = v;
+    }
+    cluster.sync();  // a CTA's shared memory stays until it is read
 }
 
 struct RouteGrad {
@@ -324,96 +412,125 @@ struct RouteGrad {
     void *logits;          // out, [tokens, experts]
 };
 
-template <typename T, int V>
+// A warp takes a run of rows, so that a segment's slopes stay in registers
+// until it ends. Shared memory holds a row for what goes by expert: the chosen
+// logits and the chosen experts' part of the gradient.
+template <typename T, int V, int N>
 __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, RouteGrad d) {
-    extern __shared__ float rows[];  // [warps, experts]
+    extern __shared__ __align__(16) float rows[];  // [warps, 32 V]
     const int lane = threadIdx.x & 31, k = a.top_k;
-    float *row = rows + (threadIdx.x >> 5) * a.experts;
-    const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
+    float *row = rows + (threadIdx.x >> 5) * 32 * V;
+    const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int64_t t0 = w * a.per_block, t1 = min(t0 + a.per_block, a.tokens);
     const float up = d.slope ? *d.loss : 0.f;
-    for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.tokens;
-         t += step) {
+    const bool softmax_all = d.weights && !a.renormalize && !a.sigmoid;
+    float slope[V];
+    int64_t end = t0;  // of the segment in `slope`
+    bool there = false;
+    for (int64_t t = t0; t < t1; ++t) {
         T *out = static_cast<T *>(d.logits) + t * a.experts;
-        uint32_t peak = 0;
+        // every load of the row, before anything waits for one
+        const bool keep = !a.mask || a.mask[t];
         float z[V], dz[V];
-        if (!a.mask || a.mask[t]) {
-            load_row<T, V>(a, t, lane, z);
-            peak = row_peak<V>(z);
-        }
-        if (peak == 0) {  // no expert: nothing depends on this row
-            for (int e = lane; e < a.experts; e += 32) out[e] = from_float<T>(0.f);
-            continue;
-        }
-        const float top = value_of(peak);
-        const float c = a.sigmoid ? fminf(top, 0.f) : top;
-        const bool dense = d.slope || (d.weights && !a.renormalize && !a.sigmoid);
-        float total = 1.f;
-        if (dense) {
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                dz[i] = ratio(z[i], c, a.sigmoid);
-                part += dz[i];
-            }
-            total = warp_sum(part);
-        }
-        const float inv = 1.f / total;
-        // the choice's part: lane j adds `own` at its index, and every expert
-        // takes -s_e * shared (softmax that is not renormalised)
-        float own = 0.f, shared = 0.f;
+        load_row<T, V, N>(a, t, lane, z);
         int index = -1;
-        if (d.weights) {
-            index = lane < k ? a.indices[t * k + lane] : -1;
-            if (index >= a.experts) index = -1;
-            const float g = index >= 0 ? d.weights[t * k + lane] * a.scale : 0.f;
-            const float zi = index >= 0
-                ? to_float<T>(static_cast<const T *>(a.logits)[t * a.stride + index])
-                : -CUDART_INF_F;
-            const float r = index >= 0 ? ratio(zi, c, a.sigmoid) : 0.f;
-            const float h = a.sigmoid ? logistic(-zi) : 1.f;
-            if (a.renormalize) {
-                const float q = r / warp_sum(r);
-                const float dot = warp_sum(q * g);
-                own = index >= 0 ? q * h * (g - dot) : 0.f;
-            } else if (a.sigmoid) {
-                own = index >= 0 ? logistic(zi) * h * g : 0.f;
-            } else {
-                own = r * inv * g;
-                shared = warp_sum(own);
-            }
+        float g = 0.f;
+        if (d.weights && lane < k) {
+            index = a.indices[t * k + lane];
+            g = d.weights[t * k + lane];
         }
-        float dot = 0.f;
-        const float *slope = nullptr;
-        if (d.slope) {
-            int64_t end = a.tokens;
-            const int g = segment_of(a.offsets, a.segments, t, end);
-            if (g >= 0 && g < a.segments) slope = d.slope + (int64_t)g * a.experts;
-        }
-        if (slope) {
+        if (d.slope && t >= end) {
+            end = a.tokens;
+            const int s = segment_of(a.offsets, a.segments, t, end);
+            there = s >= 0 && s < a.segments;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int e = lane + 32 * i;
-                if (e < a.experts) dot += dz[i] * inv * slope[e];
+                const int e = expert_of<N>(lane, i);
+                slope[i] = there && e < a.experts ? up * d.slope[(int64_t)s * a.experts + e] : 0.f;
             }
-            dot = warp_sum(dot);
+        }
+        const uint32_t peak = keep ? row_peak<V>(z) : 0u;
+        if (peak == 0) {  // no expert: nothing depends on this row
+#pragma unroll
+            for (int i = 0; i < V; ++i) dz[i] = 0.f;
+        } else {
+            const float top = value_of(peak);
+            const float c = a.sigmoid ? fminf(top, 0.f) : top;
+            float inv = 1.f;
+            if (there || softmax_all) {
+                float part = 0.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dz[i] = ratio(z[i], c, a.sigmoid);
+                    part += dz[i];
+                }
+                inv = 1.f / warp_sum(part);
+            }
+            // the choice's part: lane j adds `own` at its expert, and every
+            // expert takes -s_e * shared (softmax that is not renormalised)
+            float own = 0.f, shared = 0.f;
+            const bool chosen = index >= 0 && index < a.experts;
+            if (d.weights) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) row[expert_of<N>(lane, i)] = z[i];
+                __syncwarp();
+                const float zi = chosen ? row[index] : -CUDART_INF_F;
+                __syncwarp();
+                const float r = chosen ? ratio(zi, c, a.sigmoid) : 0.f;
+                const float h = a.sigmoid ? logistic(-zi) : 1.f;
+                g = chosen ? g * a.scale : 0.f;
+                if (a.renormalize) {
+                    const float q = r / warp_sum(r);
+                    const float dot = warp_sum(q * g);
+                    own = chosen ? q * h * (g - dot) : 0.f;
+                } else if (a.sigmoid) {
+                    own = chosen ? logistic(zi) * h * g : 0.f;
+                } else {
+                    own = r * inv * g;
+                    shared = warp_sum(own);
+                }
+            }
+            float dot = 0.f;
+            if (there) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) dot += dz[i] * slope[i];
+                dot = warp_sum(dot) * inv;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = 0.f;
+                if (there) {
+                    const float h = a.sigmoid ? logistic(-z[i]) : 1.f;
+                    v = dz[i] * inv * h * (slope[i] - dot);
+                }
+                if (softmax_all) v -= dz[i] * inv * shared;
+                dz[i] = v;
+            }
+            if (d.weights) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) row[expert_of<N>(lane, i)] = dz[i];
+                __syncwarp();
+                if (chosen) row[index] += own;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < V; ++i) dz[i] = row[expert_of<N>(lane, i)];
+                __syncwarp();
+            }
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = lane + 32 * i;
+        for (int i = 0; i < V; i += N) {
+            const int e = expert_of<N>(lane, i);
             if (e >= a.experts) continue;
-            float v = 0.f;
-            if (slope) {
-                const float h = a.sigmoid ? logistic(-z[i]) : 1.f;
-                v = dz[i] * inv * h * up * (slope[e] - dot);
+            if constexpr (N == 1) {
+                out[e] = from_float<T>(dz[i]);
+            } else {
+                uint4 u;
+                T *v = reinterpret_cast<T *>(&u);
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = from_float<T>(dz[i + j]);
+                *reinterpret_cast<uint4 *>(out + e) = u;
             }
-            if (shared != 0.f) v -= dz[i] * inv * shared;
-            row[e] = v;
         }
-        __syncwarp();
-        if (index >= 0) row[index] += own;
-        __syncwarp();
-        for (int e = lane; e < a.experts; e += 32) out[e] = from_float<T>(row[e]);
-        __syncwarp();
     }
 }
 
@@ -422,11 +539,11 @@ struct RouteLayout {
     int64_t blocks, per_block;
 };
 
-// Blocks of the balance kernel: one per SM, eight rows or more each.
+// Blocks of the balance kernel: one per SM, 32 rows (one a warp) or more each.
 RouteLayout route_layout(int64_t tokens, int64_t experts, int64_t segments) {
     RouteLayout L{};
     L.per_block = (tokens + 147) / 148;
-    if (L.per_block < 8) L.per_block = 8;
+    if (L.per_block < 32) L.per_block = 32;
     L.blocks = (tokens + L.per_block - 1) / L.per_block;
     const int64_t records = L.blocks + segments;
     size_t off = 0;
@@ -442,42 +559,53 @@ RouteLayout route_layout(int64_t tokens, int64_t experts, int64_t segments) {
     return L;
 }
 
-template <typename T, int V>
+template <typename T, int V, int N>
 cudaError_t launch_choice(const RouteArgs &a, int sms, cudaStream_t s) {
     const int64_t want = (a.tokens + 7) / 8;
     const int64_t most = (int64_t)sms * 8;
-    route_kernel<T, V><<<(unsigned)(want < most ? want : most), 256, 0, s>>>(a);
+    route_kernel<T, V, N><<<(unsigned)(want < most ? want : most), 256, 0, s>>>(a);
     return cudaGetLastError();
 }
 
-template <typename T, int V>
+template <typename T, int V, int N>
 cudaError_t launch_balance(const RouteArgs &a, bool choose, int64_t blocks, cudaStream_t s) {
-    const size_t smem = (size_t)(8 + 1) * a.experts * 4;
-    if (choose) balance_kernel<T, V, true><<<(unsigned)blocks, 256, smem, s>>>(a);
-    else balance_kernel<T, V, false><<<(unsigned)blocks, 256, smem, s>>>(a);
+    constexpr int warps = balance_warps(V);
+    static_assert((warps + 1) * 32 * V * 4 <= 48 * 1024, "the warps' sums fit shared memory");
+    const size_t smem = (size_t)(warps + 1) * a.experts * 4;
+    if (choose) balance_kernel<T, V, N, true><<<(unsigned)blocks, 32 * warps, smem, s>>>(a);
+    else balance_kernel<T, V, N, false><<<(unsigned)blocks, 32 * warps, smem, s>>>(a);
     return cudaGetLastError();
 }
 
-template <typename T, int V>
-cudaError_t launch_backward(const RouteArgs &a, const RouteGrad &d, int sms, cudaStream_t s) {
-    const int64_t want = (a.tokens + 7) / 8;
-    const int64_t most = (int64_t)sms * 6;
-    route_backward_kernel<T, V>
-        <<<(unsigned)(want < most ? want : most), 256, (size_t)8 * a.experts * 4, s>>>(a, d);
+template <typename T, int V, int N>
+cudaError_t launch_backward(RouteArgs a, const RouteGrad &d, int sms, cudaStream_t s) {
+    // rows of a warp: one while that fills the SMs once (32 warps each)
+    const int64_t warps = (int64_t)sms * 32;
+    a.per_block = (a.tokens + warps - 1) / warps;
+    const int64_t used = (a.tokens + a.per_block - 1) / a.per_block;
+    route_backward_kernel<T, V, N>
+        <<<(unsigned)((used + 7) / 8), 256, (size_t)8 * 32 * V * 4, s>>>(a, d);
     return cudaGetLastError();
 }
 
-// F(T, V): V values a lane cover E experts.
-#define IQK_ROUTE_V(T, F)                      \
-    (a.experts <= 64    ? F(T, 2)              \
-     : a.experts <= 128 ? F(T, 4)              \
-     : a.experts <= 256 ? F(T, 8)              \
-     : a.experts <= 512 ? F(T, 16)             \
-                        : F(T, 32))
-#define IQK_ROUTE_TV(dtype, F)                       \
-    ((dtype) == IQK_F32   ? IQK_ROUTE_V(float, F)    \
-     : (dtype) == IQK_F16 ? IQK_ROUTE_V(__half, F)   \
-                          : IQK_ROUTE_V(__nv_bfloat16, F))
+// Rows may be read and written 16 bytes at a time.
+template <typename T> bool wide(const RouteArgs &a, const void *out) {
+    const int n = 16 / (int)sizeof(T);
+    return a.experts % n == 0 && a.stride * (int64_t)sizeof(T) % 16 == 0 &&
+           aligned(a.logits, 16) && aligned(out, 16);
+}
+
+// F(T, V, N): V values a lane cover E experts, N to a load.
+#define IQK_ROUTE_V(T, W, F)                                             \
+    (a.experts <= 64    ? F(T, 2, 1)                                      \
+     : a.experts <= 128 ? ((W) && sizeof(T) == 4 ? F(T, 4, 4) : F(T, 4, 1)) \
+     : a.experts <= 256 ? ((W) ? F(T, 8, (16 / sizeof(T))) : F(T, 8, 1))  \
+     : a.experts <= 512 ? ((W) ? F(T, 16, (16 / sizeof(T))) : F(T, 16, 1)) \
+                        : ((W) ? F(T, 32, (16 / sizeof(T))) : F(T, 32, 1)))
+#define IQK_ROUTE_TV(dtype, out, F)                                          \
+    ((dtype) == IQK_F32   ? IQK_ROUTE_V(float, wide<float>(a, out), F)       \
+     : (dtype) == IQK_F16 ? IQK_ROUTE_V(__half, wide<__half>(a, out), F)     \
+                          : IQK_ROUTE_V(__nv_bfloat16, wide<__nv_bfloat16>(a, out), F))
 
 size_t element(int dtype) { return dtype == IQK_F32 ? 4 : 2; }
 
@@ -530,8 +658,8 @@ int iqk_route(const void *logits, int dtype, int64_t tokens, int64_t num_experts
     a.weights = weights;
     const int sms = num_sms_current();
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define IQK_F(T, V) launch_choice<T, V>(a, sms, s)
-    return cuda_status(IQK_ROUTE_TV(dtype, IQK_F));
+#define IQK_F(T, V, N) launch_choice<T, V, N>(a, sms, s)
+    return cuda_status(IQK_ROUTE_TV(dtype, nullptr, IQK_F));
 #undef IQK_F
 }
 
@@ -571,11 +699,11 @@ int iqk_route_balanced(const void *logits, int dtype, int64_t tokens, int64_t nu
     a.rec_rows = reinterpret_cast<int32_t *>(w + L.rows);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
-#define IQK_F(T, V) launch_balance<T, V>(a, weights != nullptr, L.blocks, s)
-    if (tokens) err = IQK_ROUTE_TV(dtype, IQK_F);
+#define IQK_F(T, V, N) launch_balance<T, V, N>(a, weights != nullptr, L.blocks, s)
+    if (tokens) err = IQK_ROUTE_TV(dtype, nullptr, IQK_F);
 #undef IQK_F
     if (err != cudaSuccess) return cuda_status(err);
-    balance_finish_kernel<<<1, 1024, 0, s>>>(a, loss, counts, slope);
+    balance_finish_kernel<<<kFinishCtas, 32 * kFinishWarps, 0, s>>>(a, loss, counts, slope);
     return cuda_status(cudaGetLastError());
 }
 
@@ -602,8 +730,8 @@ int iqk_route_backward(const void *logits, int dtype, int64_t tokens, int64_t nu
     const RouteGrad d{grad_weights, slope, grad_loss, grad_logits};
     const int sms = num_sms_current();
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define IQK_F(T, V) launch_backward<T, V>(a, d, sms, s)
-    return cuda_status(IQK_ROUTE_TV(dtype, IQK_F));
+#define IQK_F(T, V, N) launch_backward<T, V, N>(a, d, sms, s)
+    return cuda_status(IQK_ROUTE_TV(dtype, grad_logits, IQK_F));
 #undef IQK_F
 }
 

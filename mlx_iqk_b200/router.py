@@ -92,8 +92,13 @@ class _Route(torch.autograd.Function):
         return (indices if choose else None), weights, loss, counts
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, _indices, grad_weights, grad_loss, _counts):
+    def backward(ctx, *grads):
+        # the wrapper that refuses a second derivative costs more than the
+        # kernel, and only create_graph needs it
+        return (_refuse_twice if torch.is_grad_enabled() else _Route.gradient)(ctx, *grads)
+
+    @staticmethod
+    def gradient(ctx, _indices, grad_weights, grad_loss, _counts):
         logits, indices, mask, offsets = ctx.saved_tensors
         slope = None if grad_loss is None else ctx.slope
         if grad_weights is None and slope is None:
@@ -101,6 +106,9 @@ class _Route(torch.autograd.Function):
         grad = K.route_backward(logits if ctx.rows is None else ctx.rows, mask, offsets,
                                 *ctx.call, indices, grad_weights, slope, grad_loss)
         return grad if logits.dim() == 2 else grad.view(logits.shape), None, None, None
+
+
+_refuse_twice = once_differentiable(_Route.gradient)
 
 
 def _shaped(logits, top_k, indices, weights):
