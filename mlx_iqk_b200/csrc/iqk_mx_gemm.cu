@@ -25,8 +25,11 @@
 //               consecutive outputs of one row)
 // Accumulators and scale buffers are double-buffered.
 //
-// Work: item = (128 outputs, tile of rows), rows innermost, so that the tiles
-// of one expert read its matrix from L2. Full waves of items go to the CTAs in
+// Work: item = (128 outputs, tile of rows). One matrix: rows innermost, so that
+// it is read from memory once. Routed: outputs innermost, so that CTAs that run
+// together read one matrix's rows next to each other (the other order strides
+// by whole matrices and reads slower); an expert's next tile finds its matrix
+// in L2. Full waves of items go to the CTAs in
 // turn; what is left (under two waves) is cut into equal runs of units, and
 // the parts of a shared item meet in f32 slots of the workspace: the last CTA
 // to finish adds them in order, so results repeat bit for bit.
@@ -85,7 +88,7 @@ struct Maps {
 // The items of a call and how they are dealt to the CTAs.
 struct Plan {
     uint32_t items, whole;   // whole: items dealt in full waves
-    uint32_t tiles, units;   // units of an item
+    uint32_t tiles, nblocks, units;  // units of an item
     uint32_t all, runs;      // units of the shared items, CTAs that take a run of them
     uint32_t s0, s1;         // this CTA's run
     __device__ uint32_t start(uint32_t cta) const { return all * min(cta, runs) / runs; }
@@ -93,10 +96,11 @@ struct Plan {
 
 __device__ __forceinline__ Plan make_plan(const ProductArgs &a) {
     Plan p;
-    const uint32_t nblocks = (uint32_t)((a.out_features + kOuts - 1) / kOuts), ctas = gridDim.x;
+    const uint32_t ctas = gridDim.x;
+    p.nblocks = (uint32_t)((a.out_features + kOuts - 1) / kOuts);
     p.tiles = a.tiles ? (uint32_t)a.hdr[1] : (uint32_t)((a.pairs + a.cap - 1) / a.cap);
     p.units = (uint32_t)((a.width + kUnit - 1) / kUnit);
-    p.items = p.tiles * nblocks;
+    p.items = p.tiles * p.nblocks;
     const uint32_t waves = p.items / ctas;
     p.whole = p.items % ctas == 0 ? p.items : waves > 1 ? (waves - 1) * ctas : 0;
     // under two waves of items, at most 2^11 units each: 32 bits hold all * runs
@@ -131,9 +135,12 @@ __device__ __forceinline__ bool part_of(const Plan &p, uint32_t i, Part &q) {
 
 __device__ __forceinline__ int4 tile_of(const ProductArgs &a, const Plan &p, uint32_t item,
                                         int &out0) {
+    if (a.tiles) {
+        out0 = (int)(item % p.nblocks) * kOuts;
+        return a.tiles[item / p.nblocks];
+    }
     const uint32_t t = item % p.tiles;
     out0 = (int)(item / p.tiles) * kOuts;
-    if (a.tiles) return a.tiles[t];
     return make_int4(0, (int)(t * a.cap), (int)min((int64_t)a.cap, a.pairs - (int64_t)t * a.cap), 0);
 }
 
@@ -161,6 +168,49 @@ __device__ __forceinline__ int64_t row_base(const ProductArgs &a, const int4 &ti
     if (c + lane >= tile.z) return 0;
     const int64_t pos = (int64_t)tile.y + c + lane;
     return (a.order ? a.order[pos] : pos) * a.out_features;
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t v, int from) {
+    return (int64_t)(((uint64_t)__shfl_sync(0xffffffffu, (uint32_t)((uint64_t)v >> 32), from) << 32) |
+                     __shfl_sync(0xffffffffu, (uint32_t)(uint64_t)v, from));
+}
+
+// Columns [0, n) of v, each one row of y; lanes are 32 consecutive outputs from
+// `out`. 16-bit outputs leave in pairs: lanes 2i and 2i + 1 swap halves, the
+// even one stores both outputs of row j and the odd one of row j + 1 (4 bytes
+// a lane; `pairs` says that rows of y begin on 4 bytes).
+template <typename YT, int C>
+__device__ __forceinline__ void store_columns(const ProductArgs &a, const float (&v)[C], int n,
+                                              int64_t base, int lane, int out, bool pairs) {
+    YT *y = static_cast<YT *>(a.y);
+    const bool there = out < a.out_features;
+    if (sizeof(YT) == 4 || !pairs) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const int64_t at = shfl64(base, j);
+            if (j < n && there) y[at + out] = from_float<YT>(v[j]);
+        }
+    } else {
+        const int odd = lane & 1;
+#pragma unroll
+        for (int j = 0; j < C; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+            const int64_t at = shfl64(base, j + odd);
+            struct __align__(4) Two { YT x, y; };
+            const Two two{from_float<YT>(odd ? other : v[j]), from_float<YT>(odd ? v[j + 1] : other)};
+            // out_features is even: an output and its neighbour exist together
+            if (j + odd < n && there)
+                *reinterpret_cast<Two *>(y + at + (out & ~1)) = two;
+        }
+    }
+}
+
+template <int C>
+__device__ __forceinline__ void store_columns(const ProductArgs &a, const float (&v)[C], int n,
+                                              int64_t base, int lane, int out, bool pairs) {
+    if (a.y_dtype == IQK_F32) store_columns<float, C>(a, v, n, base, lane, out, pairs);
+    else if (a.y_dtype == IQK_F16) store_columns<__half, C>(a, v, n, base, lane, out, pairs);
+    else store_columns<__nv_bfloat16, C>(a, v, n, base, lane, out, pairs);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -347,6 +397,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
     } else if (warp >= kEpi0) {
         const int quarter = warp & 3;
         const int r = 32 * quarter + lane;  // this thread's output of the item
+        const bool pairs = a.out_features % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % 4 == 0;
         int n = 0;
         Part q;
         for (uint32_t i = 0; part_of(plan, i, q); ++i, ++n) {
@@ -360,31 +411,27 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
             }
             tc_fence_after();
             const bool whole = (uint32_t)(q.u1 - q.u0) == plan.units;
-            const bool there = out0 + r < a.out_features;
             const uint32_t shared_item = q.item - plan.whole;
             // a run's first item has the run's first slot, its last the second
             const bool first = plan.s0 / plan.units == shared_item;
             float *slot = a.slots + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * cap * kOuts;
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * cap;
-            for (int c = 0; c < tl.z; c += 32) {
-                uint32_t d[4][8];
-                const int here = min(32, tl.z - c);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (8 * j < here) tmem_ld8(src + c + 8 * j, d[j]);
+            for (int c = 0; c < tl.z; c += 16) {
+                uint32_t d[2][8];
+                const int here = min(16, tl.z - c);
+                const int64_t base = whole ? row_base(a, tl, c, lane) : 0;
+                tmem_ld8(src + c, d[0]);  // accumulators have a multiple of 16 columns
+                tmem_ld8(src + c + 8, d[1]);
                 tc_wait_ld();
-                if (whole) {
-                    const int64_t base = row_base(a, tl, c, lane);
+                float v[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j >= here) break;
-                        const int64_t at = __shfl_sync(0xffffffffu, base, j);
-                        if (there) store(a, at + out0 + r, __uint_as_float(d[j >> 3][j & 7]));
-                    }
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(d[j >> 3][j & 7]);
+                if (whole) {
+                    store_columns<16>(a, v, here, base, lane, out0 + r, pairs);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (j < here) slot[(c + j) * kOuts + r] = __uint_as_float(d[j >> 3][j & 7]);
+                    for (int j = 0; j < 16; ++j)
+                        if (j < here) slot[(c + j) * kOuts + r] = v[j];
                 }
             }
             tc_fence_before();
@@ -420,12 +467,7 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
                     for (int j = 0; j < 8; ++j)
                         if (j < here) v[j] += __ldcg(part + j * kOuts);
                 }
-                const int64_t base = row_base(a, tl, c, lane);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t at = __shfl_sync(0xffffffffu, base, j);
-                    if (j < here && there) store(a, at + out0 + r, v[j]);
-                }
+                store_columns<8>(a, v, here, row_base(a, tl, c, lane), lane, out0 + r, pairs);
             }
         }
     }
