@@ -63,27 +63,26 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax, float &inv) {
     return field == 255u ? 255u : byte;
 }
 
-// Row r of the output is row r of x, or with `order` row order[r] / per_row
-// (a pair's activation row) for the first *count of them. Block 0 clears the
-// words that the product kernel counts in.
+// Row r of the output is row r of x; with `place`, row r of x goes to the rows
+// place[r * copies ..] of its `copies` pairs (-1: none), so that a token's row
+// is read and rounded once. Block 0 clears the words that the product kernel
+// counts in.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const T *__restrict__ x, int64_t rows, int64_t width, int64_t row_stride,
                    uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
-                   int64_t scale_stride, const int32_t *__restrict__ order,
-                   const int32_t *__restrict__ count, int64_t per_row,
+                   int64_t scale_stride, const int32_t *__restrict__ place, int copies,
                    int32_t *__restrict__ zero, int zero_words) {
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero[i] = 0;
     const int64_t per = width / 8;  // threads of a row
-    const int64_t all = (order ? (int64_t)*count : rows) * per;
+    const int64_t all = rows * per;
     // whole groups of four lanes run or stop together: `per` is a multiple of 4
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all;
          i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / per, c = i % per;
-        const int64_t src = order ? order[r] / per_row : r;
         float v[8];
-        load8<T, WIDE>(x + src * row_stride + c * 8, v);
+        load8<T, WIDE>(x + r * row_stride + c * 8, v);
         uint32_t amax = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -92,8 +91,13 @@ mx_quantize_kernel(const T *__restrict__ x, int64_t rows, int64_t width, int64_t
         amax = max(amax, __shfl_xor_sync(group, amax, 2));
         float inv;
         const uint32_t byte = scale_byte(amax, inv);
-        *reinterpret_cast<uint32_t *>(codes + r * (width / 2) + c * 4) = codes8(v, inv);
-        if ((c & 3) == 0) scales[r * scale_stride + c / 4] = (uint8_t)byte;
+        const uint32_t packed = codes8(v, inv);
+        for (int j = 0; j < copies; ++j) {
+            const int64_t to = place ? place[r * copies + j] : r;
+            if (to < 0) continue;
+            *reinterpret_cast<uint32_t *>(codes + to * (width / 2) + c * 4) = packed;
+            if ((c & 3) == 0) scales[to * scale_stride + c / 4] = (uint8_t)byte;
+        }
     }
 }
 
@@ -130,9 +134,11 @@ mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restric
 }
 
 // Pairs by expert: one block counts, cuts each expert's run into tiles of at
-// most L.cap rows and scatters the pairs; those without an expert go to the
-// tail. The order of an expert's pairs changes no result: each is a row of
-// its own.
+// most L.cap rows and gives every pair its place; those without an expert go
+// to the tail of `order` and have place -1. Counting hands out the ranks, so
+// the second pass needs no atomics. The order of an expert's pairs changes no
+// result: each is a row of its own. Latency bounds it (one SM): a thread loads
+// and stores four pairs at a time.
 __global__ void __launch_bounds__(1024)
 mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLayout L,
                char *ws) {
@@ -141,15 +147,37 @@ mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLa
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, wid = tid >> 5;
     int32_t *hdr = reinterpret_cast<int32_t *>(ws + L.hdr);
     int32_t *order = reinterpret_cast<int32_t *>(ws + L.order);
+    int32_t *place = reinterpret_cast<int32_t *>(ws + L.place);
     int4 *tiles = reinterpret_cast<int4 *>(ws + L.tiles);
     for (int e = tid; e < num_experts; e += nt) cnt[e] = 0;
     for (int i = tid; i < L.zeroed(); i += nt) hdr[i] = 0;
-    if (tid == 0) bad = 0;
+    if (tid == 0) bad = tail = 0;
+    const bool quads = (reinterpret_cast<uintptr_t>(sel) & 15) == 0;
+    // the experts of pairs p .. p + 3 (-1 past the last and for any that is none)
+    auto experts4 = [&](int p, int (&e)[4]) {
+        if (quads && p + 3 < pairs) {
+            const int4 v = *reinterpret_cast<const int4 *>(sel + p);
+            e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = p + j < pairs ? sel[p + j] : -1;
+        }
+    };
+    auto is_expert = [&](int e) { return e >= 0 && e < num_experts; };
     __syncthreads();
-    for (int p = tid; p < pairs; p += nt) {
-        const int e = sel[p];
-        if (e >= 0 && e < num_experts) atomicAdd(&cnt[e], 1);
-        else if (e != -1) bad = IQK_DEVERR_EXPERT;
+    for (int p = 4 * tid; p < pairs; p += 4 * nt) {
+        int e[4];
+        experts4(p, e);
+        int4 rank;  // within the expert, or among those without one
+        int *r = &rank.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            r[j] = 0;
+            if (p + j >= pairs) continue;
+            r[j] = atomicAdd(is_expert(e[j]) ? &cnt[e[j]] : &tail, 1);
+            if (e[j] < -1 || e[j] >= num_experts) bad = IQK_DEVERR_EXPERT;
+        }
+        *reinterpret_cast<int4 *>(place + p) = rank;  // whole quads: see the layout
     }
     __syncthreads();
     // exclusive sums of rows and tiles over the experts, `per` a thread
@@ -185,12 +213,21 @@ mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLa
         hdr[0] = bad;
         hdr[1] = all_tiles;
         hdr[2] = all_rows;
-        tail = all_rows;
     }
     __syncthreads();
-    for (int p = tid; p < pairs; p += nt) {
-        const int e = sel[p];
-        order[e >= 0 && e < num_experts ? atomicAdd(&cnt[e], 1) : atomicAdd(&tail, 1)] = p;
+    for (int p = 4 * tid; p < pairs; p += 4 * nt) {
+        int e[4];
+        experts4(p, e);
+        int4 to = *reinterpret_cast<const int4 *>(place + p);
+        int *r = &to.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (p + j >= pairs) continue;
+            r[j] += is_expert(e[j]) ? cnt[e[j]] : all_rows;
+            order[r[j]] = p + j;
+            if (!is_expert(e[j])) r[j] = -1;
+        }
+        *reinterpret_cast<int4 *>(place + p) = to;
     }
 }
 
@@ -226,8 +263,8 @@ bool mx_items_ok(const MxProduct &p) {
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
                                int64_t row_stride, uint8_t *codes, uint8_t *scales,
-                               int64_t scale_stride, const int32_t *order, const int32_t *count,
-                               int64_t per_row, int32_t *zero, int zero_words,
+                               int64_t scale_stride, const int32_t *place, int copies,
+                               int32_t *zero, int zero_words,
                                cudaStream_t stream, int sms) {
     const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)sms * 16;
     const unsigned blocks = (unsigned)(want < most ? want : most);
@@ -235,8 +272,8 @@ cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t w
 #define IQK_Q(T, W)                                                                           \
     mx_quantize_kernel<T, W><<<blocks, 256, 0, stream>>>(static_cast<const T *>(x), rows,     \
                                                          width, row_stride, codes, scales,    \
-                                                         scale_stride, order, count, per_row,    \
-                                                         zero, zero_words)
+                                                         scale_stride, place, copies, zero,   \
+                                                         zero_words)
     if (dtype == IQK_F32) {
         if (wide) IQK_Q(float, true);
         else IQK_Q(float, false);
@@ -263,7 +300,7 @@ int iqk_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width, int64
     if (st == IQK_OK) st = check_rows(x, dtype, rows, width, row_stride);
     if (st != IQK_OK || rows == 0) return st;
     return cuda_status(launch_mx_quantize(x, dtype, rows, width, row_stride, codes, scales,
-                                          scale_stride, nullptr, nullptr, 1, nullptr, 0,
+                                          scale_stride, nullptr, 1, nullptr, 0,
                                           reinterpret_cast<cudaStream_t>(stream),
                                           num_sms_current()));
 }
@@ -320,9 +357,8 @@ int iqk_mx_linear(const void *x, int x_dtype, int64_t rows, int64_t row_stride,
     const int sms = num_sms_current();
     cudaError_t err = launch_mx_quantize(x, x_dtype, rows, width, row_stride,
                              reinterpret_cast<uint8_t *>(p.ws + p.L.codes),
-                             reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch, nullptr,
-                             nullptr, 1, reinterpret_cast<int32_t *>(p.ws + p.L.hdr),
-                             p.L.zeroed(), s, sms);
+                             reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch, nullptr, 1,
+                             reinterpret_cast<int32_t *>(p.ws + p.L.hdr), p.L.zeroed(), s, sms);
     if (err != cudaSuccess) return cuda_status(err);
     return cuda_status(launch_mx_product(p, s, sms));
 }
@@ -355,12 +391,11 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
         sel, (int)pairs, (int)num_experts, p.L, p.ws);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return cuda_status(err);
-    err = launch_mx_quantize(x, x_dtype, pairs, width, row_stride,
+    err = launch_mx_quantize(x, x_dtype, x_rows, width, row_stride,
                              reinterpret_cast<uint8_t *>(p.ws + p.L.codes),
                              reinterpret_cast<uint8_t *>(p.ws + p.L.scales), p.L.pitch,
-                             reinterpret_cast<const int32_t *>(p.ws + p.L.order),
-                             reinterpret_cast<const int32_t *>(p.ws + p.L.hdr) + 2,
-                             pairs / x_rows, nullptr, 0, s, sms);
+                             reinterpret_cast<const int32_t *>(p.ws + p.L.place),
+                             (int)(pairs / x_rows), nullptr, 0, s, sms);
     if (err != cudaSuccess) return cuda_status(err);
     return cuda_status(launch_mx_product(p, s, sms));
 }

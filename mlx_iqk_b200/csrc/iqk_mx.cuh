@@ -12,12 +12,13 @@ constexpr int kMxBlock = 32;  // values under one scale
 //   tickets  int32: parts that are done of each item that CTAs share,
 //          per 32 outputs
 //   order  [pairs] int32: sorted position -> pair (the others at the tail)
+//   place  [pairs, in whole quads] int32: pair -> sorted position, or -1
 //   tiles  [max_tiles] int4: {expert, first position, rows (<= cap), 0}
 //   codes  [pairs, width / 2], scales [pairs, pitch]: the activations in
 //          sorted order
 //   slots  f32: shared items' parts
 struct MxLayout {
-    size_t hdr, tickets, order, tiles, codes, scales, slots, total;
+    size_t hdr, tickets, order, place, tiles, codes, scales, slots, total;
     int64_t max_tiles, pitch;
     int cap;  // rows of a tile, a row box of the product kernel
     __host__ __device__ int zeroed() const { return (int)((order - hdr) / 4); }  // words that start at 0
@@ -39,8 +40,8 @@ struct MxProduct {
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
                                int64_t row_stride, uint8_t *codes, uint8_t *scales,
-                               int64_t scale_stride, const int32_t *order, const int32_t *count,
-                               int64_t per_row, int32_t *zero, int zero_words,
+                               int64_t scale_stride, const int32_t *place, int copies,
+                               int32_t *zero, int zero_words,
                                cudaStream_t stream, int sms);
 cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms);
 

@@ -530,6 +530,7 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
     L.hdr = take(64);
     L.tickets = take(sizeof(int32_t) * 4 * 2 * kMaxCtas);
     L.order = take(sizeof(int32_t) * (size_t)pairs);
+    L.place = take(sizeof(int32_t) * (size_t)((pairs + 3) / 4 * 4));
     L.tiles = take(16 * (size_t)L.max_tiles);
     L.codes = take((size_t)pairs * (size_t)(width / 2));
     L.scales = take((size_t)pairs * (size_t)L.pitch);
