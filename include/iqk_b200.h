@@ -535,6 +535,26 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
 
 int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream);
 
+/*
+ * iqk_mx_few: iqk_mx_routed, or with sel NULL iqk_mx_linear (num_experts 1,
+ * pairs = x_rows), of few rows in one launch; the same products and f32 sums
+ * (a long row's sum may be cut at other columns).
+ * iqk_mx_few_fits says whether a call is one (up to 64 pairs, or 16 rows of
+ * one matrix, 64 of a small one). The first 8192 bytes of `state`
+ * (iqk_mx_few_state_bytes) must be zero before its first call; each call leaves it ready for the next one on
+ * the same stream. Calls that may overlap in time need a state each.
+ * iqk_mx_read_error reads its error bits.
+ */
+size_t iqk_mx_few_state_bytes(void);
+
+int iqk_mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
+                    int routed);
+
+int iqk_mx_few(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride, const int32_t *sel,
+               int64_t pairs, const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+               int64_t num_experts, int64_t out_features, int64_t width, void *y, int y_dtype,
+               void *state, size_t state_bytes, iqk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,52 +16,10 @@
 // 16-byte accesses.
 #include "iqk_host.cuh"
 #include "iqk_mx.cuh"
+#include "iqk_mx_block.cuh"
 
 namespace iqk {
 namespace {
-
-// Eight consecutive values as f32.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    if constexpr (!WIDE) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j]);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0];
-        const float4 b = reinterpret_cast<const float4 *>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(e[j]);
-    }
-}
-
-// Two values to two codes, `lo` in the low nibble.
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8], float inv) {
-    uint32_t r;
-    asm("{\n .reg .b8 a, b, c, d;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
-        " cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
-        " mov.b32 %0, {a, b, c, d};\n}\n"
-        : "=r"(r)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv),
-          "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
-    return r;
-}
-
-// The scale byte of a block whose magnitudes' largest bit pattern is `amax`,
-// and the factor that its values are multiplied with.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t amax, float &inv) {
-    const uint32_t field = amax >> 23;  // floor(log2) + 127; 255: NaN or infinity
-    const uint32_t byte = field <= 2u ? 0u : field - 2u;
-    inv = __uint_as_float((254u - byte) << 23);
-    return field == 255u ? 255u : byte;
-}
 
 // Row r of the output is row r of x; with `place`, row r of x goes to the rows
 // place[r * copies ..] of its `copies` pairs (-1: none), so that a token's row
@@ -404,11 +362,44 @@ int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream
     if (!workspace || !flags) return IQK_ERR_ARGUMENT;
     *flags = 0;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int32_t word = 0;
-    cudaError_t err = cudaMemcpyAsync(&word, workspace, sizeof(word), cudaMemcpyDeviceToHost, s);
+    int32_t word[4] = {};
+    cudaError_t err = cudaMemcpyAsync(word, workspace, sizeof(word), cudaMemcpyDeviceToHost, s);
     if (err == cudaSuccess) err = cudaStreamSynchronize(s);
-    if (err == cudaSuccess) *flags = word;
+    if (err == cudaSuccess) *flags = word[0] | word[3];
     return cuda_status(err);
+}
+
+size_t iqk_mx_few_state_bytes(void) { return mx_few_state_bytes(); }
+
+int iqk_mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
+                    int routed) {
+    return pairs > 0 && num_experts > 0 && out_features > 0 && width > 0 &&
+           mx_few_fits(pairs, num_experts, out_features, width, routed != 0);
+}
+
+int iqk_mx_few(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride, const int32_t *sel,
+               int64_t pairs, const uint8_t *codes, const uint8_t *scales, int64_t scale_stride,
+               int64_t num_experts, int64_t out_features, int64_t width, void *y, int y_dtype,
+               void *state, size_t state_bytes, iqk_stream_t stream) {
+    if (out_features <= 0 || num_experts <= 0 || num_experts > 4096) return IQK_ERR_GEOMETRY;
+    if (!sel && num_experts != 1) return IQK_ERR_GEOMETRY;
+    if (out_features > ((int64_t)1 << 31) / num_experts) return IQK_ERR_GEOMETRY;
+    int st = check_matrix(codes, scales, scale_stride, num_experts * out_features, width);
+    if (st == IQK_OK) st = check_rows(x, x_dtype, x_rows, width, row_stride);
+    if (st != IQK_OK) return st;
+    if (!dtype_ok(y_dtype)) return IQK_ERR_ARGUMENT;
+    if (pairs < 0 || !mx_few_fits(pairs, num_experts, out_features, width, sel != nullptr))
+        return IQK_ERR_GEOMETRY;
+    if (pairs == 0) return IQK_OK;
+    if (x_rows <= 0 || pairs % x_rows || (!sel && pairs != x_rows)) return IQK_ERR_GEOMETRY;
+    if (!y || !state) return IQK_ERR_ARGUMENT;
+    if (!aligned(y, element(y_dtype)) || !aligned(state, 256) || !aligned(sel, 4))
+        return IQK_ERR_ALIGNMENT;
+    if (state_bytes < mx_few_state_bytes()) return IQK_ERR_WORKSPACE;
+    const MxFew p{x, x_dtype, x_rows, row_stride, sel, pairs, codes, scales, scale_stride,
+                  num_experts, out_features, width, y, y_dtype, static_cast<char *>(state)};
+    return cuda_status(launch_mx_few(p, reinterpret_cast<cudaStream_t>(stream),
+                                     num_sms_current()));
 }
 
 }  // extern "C"

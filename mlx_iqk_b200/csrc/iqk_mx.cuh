@@ -8,7 +8,8 @@ namespace iqk {
 constexpr int kMxBlock = 32;  // values under one scale
 
 // Workspace of one product, written by its preparation:
-//   hdr    [16] int32: [0] device error bits, [1] work tiles, [2] routable pairs
+//   hdr    [16] int32: [0] routing error bits, [1] work tiles, [2] routable
+//          pairs, [3] error bits of the product
 //   tickets  int32: parts that are done of each item that CTAs share,
 //          per 32 outputs
 //   order  [pairs] int32: sorted position -> pair (the others at the tail)
@@ -37,6 +38,26 @@ struct MxProduct {
     void *y;
     int y_dtype;
 };
+
+// The product of few rows in one launch; `state` keeps the counters of shared
+// items (0 between calls) and their parts.
+struct MxFew {
+    const void *x;
+    int x_dtype;
+    int64_t x_rows, x_stride;
+    const int32_t *sel;  // null: one matrix
+    int64_t pairs;
+    const uint8_t *codes, *scales;
+    int64_t scale_stride, num_experts, out_features, width;
+    void *y;
+    int y_dtype;
+    char *state;
+};
+
+size_t mx_few_state_bytes();
+bool mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
+                 bool routed);
+cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms);
 
 cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width,
                                int64_t row_stride, uint8_t *codes, uint8_t *scales,

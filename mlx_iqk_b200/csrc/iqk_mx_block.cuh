@@ -1,0 +1,51 @@
+// One block of MXFP4: values in, codes and scale out (device helpers).
+#pragma once
+
+#include "iqk_common.cuh"
+
+namespace iqk {
+
+// Eight consecutive values as f32.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    if constexpr (!WIDE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j]);
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0];
+        const float4 b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(e[j]);
+    }
+}
+
+// Two values to two codes, `lo` in the low nibble.
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8], float inv) {
+    uint32_t r;
+    asm("{\n .reg .b8 a, b, c, d;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        " mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(r)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv),
+          "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+    return r;
+}
+
+// The scale byte of a block whose magnitudes' largest bit pattern is `amax`,
+// and the factor that its values are multiplied with.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax, float &inv) {
+    const uint32_t field = amax >> 23;  // floor(log2) + 127; 255: NaN or infinity
+    const uint32_t byte = field <= 2u ? 0u : field - 2u;
+    inv = __uint_as_float((254u - byte) << 23);
+    return field == 255u ? 255u : byte;
+}
+
+}  // namespace iqk

@@ -23,6 +23,13 @@
 //               columns
 //   warps 8-11  epilogue: tcgen05.ld, y stored (a warp's lanes are 32
 //               consecutive outputs of one row)
+//   warps 12-15 (few rows only) activations: the rows' 512 columns read from x,
+//               rounded and written where TMA would have put them, so that
+//               such a call is one launch; each CTA also sorts its (at most
+//               64) pairs by itself. With up to 4 rows a tile each warp takes
+//               every fourth unit, so that four units' loads are under way
+//               (8 tokens' down projection 52 -> 39 us); with more, the warps
+//               share each unit (37 rows 14.2 -> 12 us)
 // Accumulators and scale buffers are double-buffered.
 //
 // Work: item = (128 outputs, tile of rows). One matrix: rows innermost, so that
@@ -41,6 +48,7 @@
 
 #include "iqk_host.cuh"
 #include "iqk_mx.cuh"
+#include "iqk_mx_block.cuh"
 #include "iqk_sync.cuh"
 
 namespace iqk {
@@ -48,8 +56,9 @@ namespace {
 
 using namespace dev;
 
-constexpr int kThreads = 384;
-constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kMover0 = 4, kEpi0 = 8;
+constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kSortWarp = 3, kMover0 = 4, kEpi0 = 8,
+              kRound0 = 12;
+__host__ __device__ constexpr int threads_of(bool few) { return few ? 512 : 384; }
 constexpr int kOuts = 128;              // outputs of an item (the MMA's M)
 constexpr int kUnit = 512;              // columns of a pipeline stage
 constexpr int kAtomA = kOuts * 128;     // one swizzle atom: 256 columns of 128 outputs
@@ -57,6 +66,8 @@ constexpr int kBoxes = 4;               // row boxes: 16, 32, 64, 128
 constexpr int kMaxStages = 5;
 constexpr int kSmemCap = 227 * 1024;
 constexpr int kBarBytes = 256;
+constexpr int kFewCap = 16, kFewPairs = 64;          // one launch: rows of a tile, routed pairs
+constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap);  // tiles; pairs, rows of x
 constexpr int kMaxCtas = 148;
 
 // Shared memory of a stage: codes of the matrix, codes of the rows, scales.
@@ -64,7 +75,7 @@ __host__ __device__ constexpr int stage_bytes(int cap) {
     return 2 * kAtomA + 2 * cap * 128 + kOuts * 16 + cap * 16;
 }
 __host__ __device__ constexpr int stages_for(int cap) {
-    const int n = (kSmemCap - 1024 - kBarBytes) / ((stage_bytes(cap) + 1023) & ~1023);
+    const int n = (kSmemCap - 1024 - kBarBytes - kFewTable) / ((stage_bytes(cap) + 1023) & ~1023);
     return n < kMaxStages ? n : kMaxStages;
 }
 
@@ -78,6 +89,12 @@ struct ProductArgs {
     float *slots;          // [ctas, 2, cap, 128]
     void *y;
     int y_dtype;
+    // few rows: the activations themselves, row p / per_row for pair p
+    const void *x;
+    int64_t x_stride;
+    const int32_t *sel;    // null: one matrix
+    int per_row, experts, wide;
+    int spread;            // the four rounding warps share each unit, else take turns
 };
 
 struct Maps {
@@ -94,11 +111,11 @@ struct Plan {
     __device__ uint32_t start(uint32_t cta) const { return all * min(cta, runs) / runs; }
 };
 
-__device__ __forceinline__ Plan make_plan(const ProductArgs &a) {
+__device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles) {
     Plan p;
     const uint32_t ctas = gridDim.x;
     p.nblocks = (uint32_t)((a.out_features + kOuts - 1) / kOuts);
-    p.tiles = a.tiles ? (uint32_t)a.hdr[1] : (uint32_t)((a.pairs + a.cap - 1) / a.cap);
+    p.tiles = a.tiles ? (uint32_t)routed_tiles : (uint32_t)((a.pairs + a.cap - 1) / a.cap);
     p.units = (uint32_t)((a.width + kUnit - 1) / kUnit);
     p.items = p.tiles * p.nblocks;
     const uint32_t waves = p.items / ctas;
@@ -156,10 +173,66 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     return v;
 }
 
-__device__ __forceinline__ void store(const ProductArgs &a, int64_t i, float v) {
-    if (a.y_dtype == IQK_F32) static_cast<float *>(a.y)[i] = v;
-    else if (a.y_dtype == IQK_F16) static_cast<__half *>(a.y)[i] = from_float<__half>(v);
-    else static_cast<__nv_bfloat16 *>(a.y)[i] = from_float<__nv_bfloat16>(v);
+__device__ __forceinline__ void store_zero(const ProductArgs &a, int64_t i) {
+    if (a.y_dtype == IQK_F32) static_cast<float *>(a.y)[i] = 0.f;
+    else static_cast<uint16_t *>(a.y)[i] = 0;
+}
+
+// Few pairs, sorted by one warp (lane l: pairs l and l + 32): a pair's rank is
+// the number of earlier pairs of its expert, every 16th rank opens a tile, and
+// the pair's row is its rank in the tile. Returns the tiles; `bad` says that an
+// index is neither an expert nor -1.
+__device__ __forceinline__ int sort_few(const ProductArgs &a, int lane, int4 *tiles,
+                                        int32_t *pairs, int32_t *rows, bool &bad) {
+    int e[2], rank[2] = {0, 0}, count[2] = {0, 0}, tile[2];
+    bad = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int p = lane + 32 * h;
+        e[h] = p < a.pairs ? a.sel[p] : -1;
+        if (e[h] < 0 || e[h] >= a.experts) {
+            bad |= e[h] != -1;
+            e[h] = -1;
+        }
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    const int n = (int)a.pairs;
+    for (int q = 0; q < n; ++q) {
+        const int other = __shfl_sync(0xffffffffu, q < 32 ? e[0] : e[1], q & 31);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            count[h] += other == e[h];
+            rank[h] += other == e[h] && q < lane + 32 * h;
+        }
+    }
+    const bool opens0 = e[0] >= 0 && rank[0] % kFewCap == 0;
+    const bool opens1 = e[1] >= 0 && rank[1] % kFewCap == 0;
+    const uint32_t m0 = __ballot_sync(0xffffffffu, opens0), m1 = __ballot_sync(0xffffffffu, opens1);
+    const uint32_t below = (1u << lane) - 1u;
+    tile[0] = opens0 ? __popc(m0 & below) : -1;
+    tile[1] = opens1 ? __popc(m0) + __popc(m1 & below) : -1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (tile[h] >= 0)
+            tiles[tile[h]] = make_int4(e[h], tile[h] * kFewCap, min(kFewCap, count[h] - rank[h]), 0);
+    int mine[2] = {tile[0], tile[1]};
+    for (int q = 0; q < n; ++q) {  // the tile that a pair's leader opened
+        const bool hi = q >= 32;
+        const int oe = __shfl_sync(0xffffffffu, hi ? e[1] : e[0], q & 31);
+        const int orank = __shfl_sync(0xffffffffu, hi ? rank[1] : rank[0], q & 31);
+        const int ot = __shfl_sync(0xffffffffu, hi ? tile[1] : tile[0], q & 31);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (ot >= 0 && oe == e[h] && orank == rank[h] / kFewCap * kFewCap) mine[h] = ot;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (e[h] >= 0) {
+            const int at = mine[h] * kFewCap + rank[h] % kFewCap, p = lane + 32 * h;
+            pairs[at] = p;
+            rows[at] = p / a.per_row;
+        }
+    return __popc(m0) + __popc(m1);
 }
 
 // Where the output row of the tile's row c + lane begins.
@@ -213,8 +286,11 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, const float 
     else store_columns<__nv_bfloat16, C>(a, v, n, base, lane, out, pairs);
 }
 
-__global__ void __launch_bounds__(kThreads, 1)
-mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
+// FEW: activations of type XT, rounded in the kernel; else from the workspace.
+template <bool FEW, typename XT>
+__global__ void __launch_bounds__(threads_of(FEW), 1)
+mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constant__ Maps maps) {
+    ProductArgs a = args;
     extern __shared__ char smem_raw[];
     // swizzle atoms repeat every 1024 bytes of shared memory
     const uint32_t raw = saddr(smem_raw);
@@ -228,11 +304,15 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
     uint64_t *dfull = sfree + 2, *dempty = dfull + 2, *drain = dempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
+    int *tile_count = reinterpret_cast<int *>(tmem_slot + 2);
+    int4 *few_tiles = reinterpret_cast<int4 *>(bars + kBarBytes);
+    int32_t *few_pairs = reinterpret_cast<int32_t *>(few_tiles + kFewPairs);
+    int32_t *few_rows = few_pairs + kFewPairs * kFewCap;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            bar_init(&full[i], 1);
+            bar_init(&full[i], !FEW ? 1 : a.spread ? 5 : 2);
             bar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -250,12 +330,31 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
         tmem_relinquish();
         tc_fence_before();
     }
-    if (a.tiles) {  // rows of pairs without an expert
+    if (FEW && a.sel) {
+        if (warp == kSortWarp) {
+            bool bad;
+            const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows, bad);
+            if (lane == 0) {
+                *tile_count = n;
+                if (blockIdx.x == 0) a.hdr[0] = bad ? IQK_DEVERR_EXPERT : 0;
+            }
+        }
+        // rows of pairs without an expert
+        for (int p = blockIdx.x; p < a.pairs; p += gridDim.x) {
+            const int e = a.sel[p];
+            if (e >= 0 && e < a.experts) continue;
+            for (int64_t i = threadIdx.x; i < a.out_features; i += blockDim.x)
+                store_zero(a, p * a.out_features + i);
+        }
+        a.tiles = few_tiles;
+        a.order = few_pairs;
+    }
+    if (!FEW && a.tiles) {
         const int64_t routed = a.hdr[2], tail = (a.pairs - routed) * a.out_features;
         for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tail;
              i += (int64_t)gridDim.x * blockDim.x)
-            store(a, a.order[routed + i / a.out_features] * a.out_features + i % a.out_features,
-                  0.f);
+            store_zero(a, a.order[routed + i / a.out_features] * a.out_features +
+                              i % a.out_features);
     }
     __syncthreads();
     tc_fence_after();
@@ -263,12 +362,12 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
     // columns: two accumulators of `cap`, then the scale buffers, 16 columns
     // a side and buffer (four words a row group, 128 rows)
     const uint32_t scale_col = tmem + 2 * cap;
-    const Plan plan = make_plan(a);
+    const Plan plan = make_plan(a, !a.tiles ? 0 : FEW ? *tile_count : a.hdr[1]);
 
     auto give_up = [&]() {
         if (!*abort_flag) {
             *abort_flag = 1;
-            atomicOr(a.hdr, IQK_DEVERR_TIMEOUT);
+            atomicOr(a.hdr + 3, IQK_DEVERR_TIMEOUT);
         }
     };
     const uint32_t off_b = 2 * kAtomA, off_sa = off_b + 2 * cap * 128, off_sb = off_sa + kOuts * 16;
@@ -291,16 +390,18 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
                     }
                     // the second half of the last unit may lie past the width
                     const int atoms = (int)min((int64_t)2, (a.width - (int64_t)u * kUnit + 255) / 256);
-                    bar_expect_tx(&full[s], (uint32_t)(atoms * (kAtomA + rows * 128) +
-                                                       (kOuts + rows) * 16));
+                    const int xrows = FEW ? 0 : rows;  // few rows: written by the rounding warps
+                    bar_expect_tx(&full[s], (uint32_t)(atoms * (kAtomA + xrows * 128) +
+                                                       (kOuts + xrows) * 16));
                     const uint32_t st = smem + s * stage;
                     for (int t = 0; t < atoms; ++t) {
                         tma_2d(st + t * kAtomA, &maps.w, u * 256 + t * 128, row0, &full[s]);
-                        tma_2d(st + off_b + t * rows * 128, &maps.x[box], u * 256 + t * 128, tl.y,
-                               &full[s]);
+                        if (!FEW)
+                            tma_2d(st + off_b + t * rows * 128, &maps.x[box], u * 256 + t * 128,
+                                   tl.y, &full[s]);
                     }
                     tma_2d(st + off_sa, &maps.ws, u * 16, row0, &full[s]);
-                    tma_2d(st + off_sb, &maps.xs[box], u * 16, tl.y, &full[s]);
+                    if (!FEW) tma_2d(st + off_sb, &maps.xs[box], u * 16, tl.y, &full[s]);
                 }
             }
             if (!ok) give_up();
@@ -394,7 +495,63 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
             }
         }
         if (!ok) give_up();
-    } else if (warp >= kEpi0) {
+    } else if (FEW && warp >= kRound0) {
+        // lane: the 32 columns lane % 16 of every other row of this warp's
+        const int block = lane & 15, turn = warp - kRound0;
+        const int first = (lane >> 4) + (a.spread ? 2 * turn : 0), step = a.spread ? 8 : 2;
+        int g = 0;
+        bool ok = true;
+        Part q;
+        for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
+            int out0;
+            const int4 tl = tile_of(a, plan, q.item, out0);
+            for (int u = q.u0; u < q.u1; ++u, ++g) {
+                if (!a.spread && (g & 3) != turn) continue;
+                const int s = g % S;
+                ok = bar_wait(&empty[s], ((uint32_t)(g / S) & 1u) ^ 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t st = smem + s * stage;
+                const int64_t col = (int64_t)u * kUnit + block * kMxBlock;
+#pragma unroll 2
+                for (int r = first; r < tl.z; r += step) {
+                    uint32_t w[4] = {0u, 0u, 0u, 0u}, byte = 0u;
+                    if (col < a.width) {
+                        const int64_t row = a.tiles ? few_rows[tl.y + r] : tl.y + r;
+                        const XT *src = static_cast<const XT *>(a.x) + row * a.x_stride + col;
+                        float v[4][8];
+                        uint32_t amax = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (a.wide) load8<XT, true>(src + 8 * j, v[j]);
+                            else load8<XT, false>(src + 8 * j, v[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            amax = max(amax, __float_as_uint(v[j >> 3][j & 7]) & 0x7fffffffu);
+                        float inv;
+                        byte = scale_byte(amax, inv);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = codes8(v[j], inv);
+                    }
+                    // row r of the swizzle atom of 256 columns, its 16-byte chunk block % 8
+                    const uint32_t at = st + off_b + (block >> 3) * kFewCap * 128 + r * 128 +
+                                        ((uint32_t)((block & 7) ^ (r & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[0]),
+                                 "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                 : "memory");
+                    asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(st + off_sb + r * 16 + block),
+                                 "r"(byte)
+                                 : "memory");
+                }
+                // the MMA reads shared memory through the asynchronous proxy
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&full[s]);
+            }
+        }
+        if (!ok) give_up();
+    } else if (warp >= kEpi0 && warp < kEpi0 + 4) {
         const int quarter = warp & 3;
         const int r = 32 * quarter + lane;  // this thread's output of the item
         const bool pairs = a.out_features % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % 4 == 0;
@@ -454,6 +611,8 @@ mx_product_kernel(ProductArgs a, const __grid_constant__ Maps maps) {
             if (lane == 0) done = (uint32_t)atomicAdd(&a.tickets[shared_item * 4 + quarter], 1);
             if (__shfl_sync(0xffffffffu, done, 0) != o1 - o0) continue;
             __threadfence();
+            // no part is left to count: the ticket is 0 again for the next call
+            if (lane == 0) a.tickets[shared_item * 4 + quarter] = 0;
             // the first owner's run may have begun in an earlier item
             const bool early = plan.start(o0) / plan.units != shared_item;
             for (int c = 0; c < tl.z; c += 8) {
@@ -539,6 +698,37 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
     return L;
 }
 
+namespace {
+
+template <bool FEW, typename XT>
+cudaError_t launch_kernel(const ProductArgs &a, const Maps &maps, int sms, cudaStream_t stream) {
+    static std::atomic<bool> attr_done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
+    if (dev < 0 || !attr_done[dev].load()) {
+        const cudaError_t err = cudaFuncSetAttribute(
+            mx_product_kernel<FEW, XT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap);
+        if (err != cudaSuccess) return err;
+        if (dev >= 0) attr_done[dev].store(true);
+    }
+    const int smem = 1024 + a.stages * ((stage_bytes(a.cap) + 1023) & ~1023) + kBarBytes + kFewTable;
+    const int grid = sms < kMaxCtas ? sms : kMaxCtas;
+    mx_product_kernel<FEW, XT><<<(unsigned)grid, threads_of(FEW), smem, stream>>>(a, maps);
+    return cudaGetLastError();
+}
+
+cudaError_t encode_matrix(Maps &maps, const uint8_t *codes, const uint8_t *scales,
+                          int64_t scale_stride, int64_t rows, int64_t width) {
+    const uint64_t code_row = (uint64_t)width / 2, scale_row = (uint64_t)width / kMxBlock;
+    const cudaError_t err =
+        encode_rows(&maps.w, codes, code_row, (uint64_t)rows, code_row, 128, kOuts, true);
+    if (err != cudaSuccess) return err;
+    return encode_rows(&maps.ws, scales, scale_row, (uint64_t)rows, (uint64_t)scale_stride, 16,
+                       kOuts, false);
+}
+
+}  // namespace
+
 cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) {
     ProductArgs a{};
     a.out_features = p.out_features;
@@ -556,13 +746,11 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     a.y = p.y;
     a.y_dtype = p.y_dtype;
     Maps maps;
-    const uint64_t rows = (uint64_t)(p.num_experts * p.out_features);
+    cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
+                                    p.num_experts * p.out_features, p.width);
+    // boxes up to the tile's rows; a lone matrix's tiles are full but the last
     const uint64_t code_row = (uint64_t)p.width / 2, scale_row = (uint64_t)p.width / kMxBlock;
-    cudaError_t err = encode_rows(&maps.w, p.codes, code_row, rows, code_row, 128, kOuts, true);
-    if (err == cudaSuccess)
-        err = encode_rows(&maps.ws, p.scales, scale_row, rows, (uint64_t)p.scale_stride, 16, kOuts,
-                          false);
-    for (int i = 0; i < kBoxes && err == cudaSuccess; ++i) {
+    for (int i = 0; i < kBoxes && err == cudaSuccess && (16 << i) <= a.cap; ++i) {
         err = encode_rows(&maps.x[i], p.ws + p.L.codes, code_row, (uint64_t)p.pairs, code_row, 128,
                           16u << i, true);
         if (err == cudaSuccess)
@@ -570,19 +758,58 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
                               (uint64_t)p.L.pitch, 16, 16u << i, false);
     }
     if (err != cudaSuccess) return err;
-    const int smem = 1024 + a.stages * ((stage_bytes(a.cap) + 1023) & ~1023) + kBarBytes;
-    static std::atomic<bool> attr_done[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
-    if (dev < 0 || !attr_done[dev].load()) {
-        err = cudaFuncSetAttribute(mx_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   kSmemCap);
-        if (err != cudaSuccess) return err;
-        if (dev >= 0) attr_done[dev].store(true);
-    }
-    const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    mx_product_kernel<<<(unsigned)grid, kThreads, smem, stream>>>(a, maps);
-    return cudaGetLastError();
+    return launch_kernel<false, float>(a, maps, sms, stream);
+}
+
+// State of the one-launch product: hdr, tickets, slots.
+constexpr size_t kStateTickets = 256;
+constexpr size_t kStateSlots = kStateTickets + (sizeof(int32_t) * 4 * 2 * kMaxCtas + 255) / 256 * 256;
+
+static_assert(kStateSlots <= 8192, "the caller clears 8192 bytes");
+
+size_t mx_few_state_bytes() {
+    return kStateSlots + sizeof(float) * 2 * kMaxCtas * kOuts * kFewCap;
+}
+
+// One launch serves few rows: each CTA rounds the rows that it needs, and sorts
+// the pairs, by itself. A lone matrix of up to 16 rows is read once either way;
+// above that (64 at most) its tiles read it again, and this form is taken while
+// the call has under four units of work a CTA, where launches cost more.
+bool mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
+                 bool routed) {
+    if (pairs > kFewPairs) return false;
+    if (routed || pairs <= kFewCap) return true;
+    const int64_t items = (pairs + kFewCap - 1) / kFewCap * ((out_features + kOuts - 1) / kOuts);
+    return items * ((width + kUnit - 1) / kUnit) <= 4 * kMaxCtas;
+}
+
+cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
+    ProductArgs a{};
+    a.out_features = p.out_features;
+    a.width = p.width;
+    a.pairs = p.pairs;
+    a.cap = kFewCap;
+    a.stages = stages_for(a.cap);
+    a.hdr = reinterpret_cast<int32_t *>(p.state);
+    a.tickets = reinterpret_cast<int32_t *>(p.state + kStateTickets);
+    a.slots = reinterpret_cast<float *>(p.state + kStateSlots);
+    a.y = p.y;
+    a.y_dtype = p.y_dtype;
+    a.x = p.x;
+    a.x_stride = p.x_stride;
+    a.sel = p.sel;
+    a.per_row = (int)(p.pairs / p.x_rows);
+    a.experts = (int)p.num_experts;
+    const size_t item = p.x_dtype == IQK_F32 ? 4 : 2;
+    a.spread = !p.sel && p.pairs > 4;
+    a.wide = aligned(p.x, 16) && p.x_stride * (int64_t)item % 16 == 0;
+    Maps maps;
+    const cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
+                                          p.num_experts * p.out_features, p.width);
+    if (err != cudaSuccess) return err;
+    if (p.x_dtype == IQK_F32) return launch_kernel<true, float>(a, maps, sms, stream);
+    if (p.x_dtype == IQK_F16) return launch_kernel<true, __half>(a, maps, sms, stream);
+    return launch_kernel<true, __nv_bfloat16>(a, maps, sms, stream);
 }
 
 }  // namespace iqk

@@ -174,6 +174,12 @@ def library() -> ctypes.CDLL:
     lib.iqk_mx_routed.argtypes = [vp, i32, i64, i64, vp, i64, vp, vp, i64, i64, i64, i64, vp, i32,
                                   vp, sz, vp]
     lib.iqk_mx_routed.restype = i32
+    lib.iqk_mx_few_state_bytes.argtypes = []
+    lib.iqk_mx_few_state_bytes.restype = sz
+    lib.iqk_mx_few_fits.argtypes = [i64, i64, i64, i64, i32]
+    lib.iqk_mx_few_fits.restype = i32
+    lib.iqk_mx_few.argtypes = lib.iqk_mx_routed.argtypes
+    lib.iqk_mx_few.restype = i32
     lib.iqk_mx_read_error.argtypes = [vp, ctypes.POINTER(ctypes.c_int32), vp]
     lib.iqk_mx_read_error.restype = i32
     _LIB = lib
@@ -195,7 +201,8 @@ def exported_symbols() -> list[str]:
             "iqk_dense_dequant", "iqk_dense_gemv",
             "iqk_route", "iqk_balance_workspace_bytes", "iqk_route_balanced",
             "iqk_route_backward", "iqk_mx_quantize", "iqk_mx_dequantize",
-            "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error"]
+            "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error",
+            "iqk_mx_few_state_bytes", "iqk_mx_few_fits", "iqk_mx_few"]
 
 
 def check_bounded_wait(limit_ns: int, device: torch.device) -> int:
@@ -642,10 +649,52 @@ def mx_workspace_bytes(pairs: int, num_experts: int, width: int, out_features: i
     return int(library().iqk_mx_workspace_bytes(pairs, num_experts, width, out_features))
 
 
+@functools.lru_cache(maxsize=4096)
+def mx_few_fits(pairs: int, num_experts: int, out_features: int, width: int, routed: bool) -> bool:
+    return bool(library().iqk_mx_few_fits(pairs, num_experts, out_features, width, routed))
+
+
+_FEW_STATES: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def mx_few_state(device: torch.device, stream: int) -> torch.Tensor:
+    """Zeroed state of the one-launch product, kept per device and stream (stream
+    order keeps a call after the one before); fresh under graph capture, where
+    its clearing is part of the graph."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    state = None if capturing else _FEW_STATES.get((device.index, stream))
+    if state is None:
+        state = torch.empty(int(library().iqk_mx_few_state_bytes()), dtype=torch.uint8,
+                            device=device)
+        state[:8192].zero_()
+        if not capturing:
+            if len(_FEW_STATES) >= 64:
+                _FEW_STATES.clear()
+            _FEW_STATES[device.index, stream] = state
+    return state
+
+
+def mx_few(x: torch.Tensor, rows: int, row_stride: int, sel, pairs: int, codes: torch.Tensor,
+           scales: torch.Tensor, scale_stride: int, experts: int, out_features: int,
+           y: torch.Tensor) -> None:
+    """``iqk_mx_few``: the product of few rows; ``sel`` None for one matrix."""
+    stream = stream_handle(y.device)
+    state = mx_few_state(y.device, stream)
+    status = library().iqk_mx_few(
+        x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, _ptr(sel), pairs, codes.data_ptr(),
+        scales.data_ptr(), scale_stride, experts, out_features, x.shape[-1], y.data_ptr(),
+        DTYPE_IDS[y.dtype], state.data_ptr(), state.numel(), stream)
+    if status:
+        raise_for_status(status, "iqk_mx_few")
+
+
 def mx_linear(x: torch.Tensor, rows: int, row_stride: int, codes: torch.Tensor,
               scales: torch.Tensor, scale_stride: int, y: torch.Tensor) -> None:
     """``iqk_mx_linear``: ``y [rows, out] = q(x) W^T``."""
     width, out_features = x.shape[-1], codes.shape[0]
+    if mx_few_fits(rows, 1, out_features, width, False):
+        mx_few(x, rows, row_stride, None, rows, codes, scales, scale_stride, 1, out_features, y)
+        return
     need = mx_workspace_bytes(rows, 1, width, out_features)
     ws = torch.empty(need, dtype=torch.uint8, device=y.device)
     status = library().iqk_mx_linear(
@@ -663,6 +712,10 @@ def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
     pairs, width = sel.numel(), x.shape[-1]
     experts, out_features = codes.shape[0], codes.shape[1]
     if workspace is None:
+        if mx_few_fits(pairs, experts, out_features, width, True):
+            mx_few(x, rows, row_stride, sel, pairs, codes, scales, scale_stride, experts,
+                   out_features, y)
+            return
         need = mx_workspace_bytes(pairs, experts, width, out_features)
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
     status = library().iqk_mx_routed(
