@@ -214,7 +214,7 @@ int check_rows(const void *x, int dtype, int64_t rows, int64_t width, int64_t ro
 
 // The product kernel counts its items in 32 bits.
 bool mx_items_ok(const MxProduct &p) {
-    return p.L.max_tiles * ((p.out_features + 127) / 128) < (int64_t)1 << 31;
+    return p.L.max_tiles * ((p.out_features + p.L.outs - 1) / p.L.outs) < (int64_t)1 << 31;
 }
 
 }  // namespace

@@ -21,7 +21,7 @@ constexpr int kMxBlock = 32;  // values under one scale
 struct MxLayout {
     size_t hdr, tickets, order, place, tiles, codes, scales, slots, total;
     int64_t max_tiles, pitch;
-    int cap;  // rows of a tile, a row box of the product kernel
+    int cap, outs;  // rows of a tile, outputs of an item
     __host__ __device__ int zeroed() const { return (int)((order - hdr) / 4); }  // words that start at 0
 };
 

@@ -32,14 +32,16 @@
 //               share each unit (37 rows 14.2 -> 12 us)
 // Accumulators and scale buffers are double-buffered.
 //
-// Work: item = (128 outputs, tile of rows). One matrix: rows innermost, so that
+// Work: item = (128 outputs, tile of rows); a call of few items takes 64 or 32
+// outputs to an item and leaves the MMA's other rows unused, which spreads the
+// matrix over more SMs. One matrix: rows innermost, so that
 // it is read from memory once. Routed: outputs innermost, so that CTAs that run
 // together read one matrix's rows next to each other (the other order strides
 // by whole matrices and reads slower); an expert's next tile finds its matrix
-// in L2. Full waves of items go to the CTAs in
-// turn; what is left (under two waves) is cut into equal runs of units, and
-// the parts of a shared item meet in f32 slots of the workspace: the last CTA
-// to finish adds them in order, so results repeat bit for bit.
+// in L2. The CTAs take items in turn. Where the last round would leave many of
+// them idle over a wide matrix, its items are cut into equal runs of units, and
+// the parts of an item meet in f32 slots of the workspace: the last CTA to
+// finish adds them in order, so results repeat bit for bit.
 //
 // Every wait is bounded (2 s): a wait that expires sets IQK_DEVERR_TIMEOUT and
 // an abort flag that ends the others, copies in flight land, and tensor memory
@@ -59,7 +61,7 @@ using namespace dev;
 constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kSortWarp = 3, kMover0 = 4, kEpi0 = 8,
               kRound0 = 12;
 __host__ __device__ constexpr int threads_of(bool few) { return few ? 512 : 384; }
-constexpr int kOuts = 128;              // outputs of an item (the MMA's M)
+constexpr int kOuts = 128;              // outputs of an item at most (the MMA's M)
 constexpr int kUnit = 512;              // columns of a pipeline stage
 constexpr int kAtomA = kOuts * 128;     // one swizzle atom: 256 columns of 128 outputs
 constexpr int kBoxes = 4;               // row boxes: 16, 32, 64, 128
@@ -67,8 +69,9 @@ constexpr int kMaxStages = 5;
 constexpr int kSmemCap = 227 * 1024;
 constexpr int kBarBytes = 256;
 constexpr int kFewCap = 16, kFewPairs = 64;          // one launch: rows of a tile, routed pairs
-constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap);  // tiles; pairs, rows of x
+constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap + 4);  // tiles; pairs, rows of x; experts
 constexpr int kMaxCtas = 148;
+constexpr uint32_t kSaved = 14;
 
 // Shared memory of a stage: codes of the matrix, codes of the rows, scales.
 __host__ __device__ constexpr int stage_bytes(int cap) {
@@ -81,7 +84,7 @@ __host__ __device__ constexpr int stages_for(int cap) {
 
 struct ProductArgs {
     int64_t out_features, width, pairs;
-    int cap, stages;
+    int cap, outs, stages;
     int32_t *hdr;
     const int32_t *order;  // null: one matrix, row p is pair p
     const int4 *tiles;
@@ -114,13 +117,17 @@ struct Plan {
 __device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles) {
     Plan p;
     const uint32_t ctas = gridDim.x;
-    p.nblocks = (uint32_t)((a.out_features + kOuts - 1) / kOuts);
+    p.nblocks = (uint32_t)((a.out_features + a.outs - 1) / a.outs);
     p.tiles = a.tiles ? (uint32_t)routed_tiles : (uint32_t)((a.pairs + a.cap - 1) / a.cap);
     p.units = (uint32_t)((a.width + kUnit - 1) / kUnit);
     p.items = p.tiles * p.nblocks;
-    const uint32_t waves = p.items / ctas;
-    p.whole = p.items % ctas == 0 ? p.items : waves > 1 ? (waves - 1) * ctas : 0;
-    // under two waves of items, at most 2^11 units each: 32 bits hold all * runs
+    // The last round's items are shared when that saves kSaved units or more:
+    // joining parts costs 4 to 8 us (a fence, a counter and the sums), a unit
+    // 0.4 us for a CTA that has the memory to itself. Cutting every call of
+    // under one round cost a 4096-wide decode (8 units) 13 us for 9.
+    const uint32_t rest = p.items % ctas, run = (rest * p.units + ctas - 1) / ctas;
+    p.whole = p.units - run < kSaved ? p.items : p.items - rest;
+    // fewer items than CTAs, at most 2^11 units each: 32 bits hold all * runs
     p.all = (p.items - p.whole) * p.units;
     p.runs = max(1u, min(ctas, p.all));
     p.s0 = p.start(blockIdx.x);
@@ -153,17 +160,21 @@ __device__ __forceinline__ bool part_of(const Plan &p, uint32_t i, Part &q) {
 __device__ __forceinline__ int4 tile_of(const ProductArgs &a, const Plan &p, uint32_t item,
                                         int &out0) {
     if (a.tiles) {
-        out0 = (int)(item % p.nblocks) * kOuts;
+        out0 = (int)(item % p.nblocks) * a.outs;
         return a.tiles[item / p.nblocks];
     }
     const uint32_t t = item % p.tiles;
-    out0 = (int)(item / p.tiles) * kOuts;
+    out0 = (int)(item / p.tiles) * a.outs;
     return make_int4(0, (int)(t * a.cap), (int)min((int64_t)a.cap, a.pairs - (int64_t)t * a.cap), 0);
 }
 
 // The smallest box that holds `rows`.
 __device__ __forceinline__ int box_of(int rows) {
     return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -173,18 +184,27 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     return v;
 }
 
-__device__ __forceinline__ void store_zero(const ProductArgs &a, int64_t i) {
-    if (a.y_dtype == IQK_F32) static_cast<float *>(a.y)[i] = 0.f;
-    else static_cast<uint16_t *>(a.y)[i] = 0;
+// Zeros to row p of y, by one warp, 16 bytes a lane where they are aligned.
+__device__ __forceinline__ void zero_row(const ProductArgs &a, int64_t p, int lane) {
+    const int64_t item = a.y_dtype == IQK_F32 ? 4 : 2;
+    char *row = static_cast<char *>(a.y) + p * a.out_features * item;
+    const int64_t bytes = a.out_features * item;
+    const int64_t head = min(bytes, (int64_t)(-reinterpret_cast<intptr_t>(row) & 15));
+    const int64_t body = (bytes - head) / 16;
+    for (int64_t i = 2 * lane; i < head; i += 64) *reinterpret_cast<uint16_t *>(row + i) = 0;
+    for (int64_t i = lane; i < body; i += 32)
+        reinterpret_cast<uint4 *>(row + head)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t i = head + 16 * body + 2 * lane; i < bytes; i += 64)
+        *reinterpret_cast<uint16_t *>(row + i) = 0;
 }
 
 // Few pairs, sorted by one warp (lane l: pairs l and l + 32): a pair's rank is
 // the number of earlier pairs of its expert, every 16th rank opens a tile, and
-// the pair's row is its rank in the tile. Returns the tiles; `bad` says that an
-// index is neither an expert nor -1.
+// the pair's row is its rank in the tile. `all` is scratch for the experts.
+// Returns the tiles; `bad` says that an index is neither an expert nor -1.
 __device__ __forceinline__ int sort_few(const ProductArgs &a, int lane, int4 *tiles,
-                                        int32_t *pairs, int32_t *rows, bool &bad) {
-    int e[2], rank[2] = {0, 0}, count[2] = {0, 0}, tile[2];
+                                        int32_t *pairs, int32_t *rows, int4 *all, bool &bad) {
+    int e[2], rank[2] = {0, 0}, count[2] = {0, 0}, lead[2] = {0, 0};
     bad = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -194,44 +214,38 @@ __device__ __forceinline__ int sort_few(const ProductArgs &a, int lane, int4 *ti
             bad |= e[h] != -1;
             e[h] = -1;
         }
+        reinterpret_cast<int32_t *>(all)[p] = e[h];
     }
     bad = __any_sync(0xffffffffu, bad);
-    const int n = (int)a.pairs;
-    for (int q = 0; q < n; ++q) {
-        const int other = __shfl_sync(0xffffffffu, q < 32 ? e[0] : e[1], q & 31);
+    __syncwarp();
+    for (int q = 0; q < (int)a.pairs; q += 4) {
+        const int4 four = all[q / 4];
+        const int other[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            count[h] += other == e[h];
-            rank[h] += other == e[h] && q < lane + 32 * h;
-        }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (other[j] == e[h]) {
+                    // the pair that opened this one's tile
+                    if (q + j <= lane + 32 * h && count[h] % kFewCap == 0) lead[h] = q + j;
+                    rank[h] += q + j < lane + 32 * h;
+                    ++count[h];
+                }
     }
-    const bool opens0 = e[0] >= 0 && rank[0] % kFewCap == 0;
-    const bool opens1 = e[1] >= 0 && rank[1] % kFewCap == 0;
-    const uint32_t m0 = __ballot_sync(0xffffffffu, opens0), m1 = __ballot_sync(0xffffffffu, opens1);
-    const uint32_t below = (1u << lane) - 1u;
-    tile[0] = opens0 ? __popc(m0 & below) : -1;
-    tile[1] = opens1 ? __popc(m0) + __popc(m1 & below) : -1;
+    const uint32_t m0 = __ballot_sync(0xffffffffu, e[0] >= 0 && lead[0] == lane);
+    const uint32_t m1 = __ballot_sync(0xffffffffu, e[1] >= 0 && lead[1] == lane + 32);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (tile[h] >= 0)
-            tiles[tile[h]] = make_int4(e[h], tile[h] * kFewCap, min(kFewCap, count[h] - rank[h]), 0);
-    int mine[2] = {tile[0], tile[1]};
-    for (int q = 0; q < n; ++q) {  // the tile that a pair's leader opened
-        const bool hi = q >= 32;
-        const int oe = __shfl_sync(0xffffffffu, hi ? e[1] : e[0], q & 31);
-        const int orank = __shfl_sync(0xffffffffu, hi ? rank[1] : rank[0], q & 31);
-        const int ot = __shfl_sync(0xffffffffu, hi ? tile[1] : tile[0], q & 31);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (ot >= 0 && oe == e[h] && orank == rank[h] / kFewCap * kFewCap) mine[h] = ot;
+    for (int h = 0; h < 2; ++h) {
+        if (e[h] < 0) continue;
+        const int p = lane + 32 * h;
+        const uint32_t below = (1u << (lead[h] & 31)) - 1u;
+        const int tile = lead[h] < 32 ? __popc(m0 & below) : __popc(m0) + __popc(m1 & below);
+        const int at = tile * kFewCap + rank[h] % kFewCap;
+        if (lead[h] == p)
+            tiles[tile] = make_int4(e[h], tile * kFewCap, min(kFewCap, count[h] - rank[h]), 0);
+        pairs[at] = p;
+        rows[at] = p / a.per_row;
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (e[h] >= 0) {
-            const int at = mine[h] * kFewCap + rank[h] % kFewCap, p = lane + 32 * h;
-            pairs[at] = p;
-            rows[at] = p / a.per_row;
-        }
     return __popc(m0) + __popc(m1);
 }
 
@@ -325,6 +339,10 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
         *abort_flag = 0;
         bar_fence_init();
     }
+    if (warp == kProducer && lane == 1) {
+        prefetch_map(&maps.w);
+        prefetch_map(&maps.ws);
+    }
     if (warp == kTmemWarp) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -333,28 +351,15 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
     if (FEW && a.sel) {
         if (warp == kSortWarp) {
             bool bad;
-            const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows, bad);
+            const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows,
+                                   reinterpret_cast<int4 *>(few_rows + kFewPairs * kFewCap), bad);
             if (lane == 0) {
                 *tile_count = n;
                 if (blockIdx.x == 0) a.hdr[0] = bad ? IQK_DEVERR_EXPERT : 0;
             }
         }
-        // rows of pairs without an expert
-        for (int p = blockIdx.x; p < a.pairs; p += gridDim.x) {
-            const int e = a.sel[p];
-            if (e >= 0 && e < a.experts) continue;
-            for (int64_t i = threadIdx.x; i < a.out_features; i += blockDim.x)
-                store_zero(a, p * a.out_features + i);
-        }
         a.tiles = few_tiles;
         a.order = few_pairs;
-    }
-    if (!FEW && a.tiles) {
-        const int64_t routed = a.hdr[2], tail = (a.pairs - routed) * a.out_features;
-        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tail;
-             i += (int64_t)gridDim.x * blockDim.x)
-            store_zero(a, a.order[routed + i / a.out_features] * a.out_features +
-                              i % a.out_features);
     }
     __syncthreads();
     tc_fence_after();
@@ -391,8 +396,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
                     // the second half of the last unit may lie past the width
                     const int atoms = (int)min((int64_t)2, (a.width - (int64_t)u * kUnit + 255) / 256);
                     const int xrows = FEW ? 0 : rows;  // few rows: written by the rounding warps
-                    bar_expect_tx(&full[s], (uint32_t)(atoms * (kAtomA + xrows * 128) +
-                                                       (kOuts + xrows) * 16));
+                    bar_expect_tx(&full[s], (uint32_t)((atoms * 128 + 16) * (a.outs + xrows)));
                     const uint32_t st = smem + s * stage;
                     for (int t = 0; t < atoms; ++t) {
                         tma_2d(st + t * kAtomA, &maps.w, u * 256 + t * 128, row0, &full[s]);
@@ -554,6 +558,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
     } else if (warp >= kEpi0 && warp < kEpi0 + 4) {
         const int quarter = warp & 3;
         const int r = 32 * quarter + lane;  // this thread's output of the item
+        const bool active = 32 * quarter < a.outs;
         const bool pairs = a.out_features % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % 4 == 0;
         int n = 0;
         Part q;
@@ -573,7 +578,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             const bool first = plan.s0 / plan.units == shared_item;
             float *slot = a.slots + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * cap * kOuts;
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * cap;
-            for (int c = 0; c < tl.z; c += 16) {
+            for (int c = 0; active && c < tl.z; c += 16) {
                 uint32_t d[2][8];
                 const int here = min(16, tl.z - c);
                 const int64_t base = whole ? row_base(a, tl, c, lane) : 0;
@@ -594,7 +599,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&dempty[acc]);
-            if (whole) continue;
+            if (whole || !active) continue;
             // A shared item: the CTA that finishes last adds every part, in order
             // (each warp for its 32 outputs: no warp waits for another).
             const uint32_t first_unit = shared_item * plan.units;
@@ -615,19 +620,27 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             if (lane == 0) a.tickets[shared_item * 4 + quarter] = 0;
             // the first owner's run may have begun in an earlier item
             const bool early = plan.start(o0) / plan.units != shared_item;
-            for (int c = 0; c < tl.z; c += 8) {
-                float v[8] = {};
-                const int here = min(8, tl.z - c);
-#pragma unroll 2
+            for (int c = 0; c < tl.z; c += 32) {
+                float v[32] = {};
+                const int here = min(32, tl.z - c);
                 for (uint32_t o = o0; o <= o1; ++o) {
                     const float *part = a.slots +
                         ((int64_t)o * 2 + (o == o0 && early ? 1 : 0)) * cap * kOuts + c * kOuts + r;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 32; ++j)
                         if (j < here) v[j] += __ldcg(part + j * kOuts);
                 }
-                store_columns<8>(a, v, here, row_base(a, tl, c, lane), lane, out0 + r, pairs);
+                store_columns<32>(a, v, here, row_base(a, tl, c, lane), lane, out0 + r, pairs);
             }
+        }
+    }
+    if (warp == kTmemWarp || warp == kSortWarp) {  // rows of pairs without an expert
+        const int64_t at = blockIdx.x * 2 + (warp == kSortWarp), step = gridDim.x * 2;
+        if (FEW && a.sel) {
+            for (int64_t p = at; p < a.pairs; p += step)
+                if (a.sel[p] < 0 || a.sel[p] >= a.experts) zero_row(a, p, lane);
+        } else if (a.tiles) {
+            for (int64_t i = a.hdr[2] + at; i < a.pairs; i += step) zero_row(a, a.order[i], lane);
         }
     }
     __syncthreads();
@@ -667,6 +680,42 @@ cudaError_t encode_rows(CUtensorMap *map, const void *base, uint64_t row_used, u
 
 }  // namespace
 
+namespace {
+
+// The shape of an item: `cap` rows, `outs` outputs. A CTA's time goes by the
+// bytes that it loads, (rows + outputs) of each column block, times the rounds
+// of items. Large items load least in all; small ones fill the SMs. A smaller
+// shape is taken where it saves a tenth or more.
+struct Shape {
+    int cap, outs;
+};
+
+Shape shape_of(int64_t pairs, int64_t experts, int64_t out_features, int most) {
+    const int64_t used = experts < pairs ? experts : pairs;
+    const int64_t mean = (pairs + used - 1) / used;  // rows of an expert
+    Shape best{0, 0};
+    double least = 0;
+    for (int cap = most; cap >= 16; cap /= 2) {
+        // an expert's rows vary: below twice the mean many experts would take a
+        // second tile, above it the tile's rows (and its stages) are wasted
+        if (cap > 16 && cap / 2 >= 2 * mean) continue;
+        const int64_t tiles = experts == 1 ? (pairs + cap - 1) / cap
+                                           : used + (pairs - used) / cap;
+        const int64_t rows = mean < cap ? mean : cap;
+        for (int outs = kOuts; outs >= 32; outs /= 2) {
+            const int64_t items = tiles * ((out_features + outs - 1) / outs);
+            const double cost = (double)((items + kMaxCtas - 1) / kMaxCtas) * (double)(rows + outs);
+            if (!best.cap || cost < 0.9 * least) {
+                best = Shape{cap, outs};
+                least = cost;
+            }
+        }
+    }
+    return best;
+}
+
+}  // namespace
+
 MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t out_features) {
     MxLayout L{};
     size_t off = 0;
@@ -675,15 +724,9 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
         off += (bytes + 255) & ~size_t(255);
         return at;
     };
-    // Rows of a tile. Enough that an expert's rows mostly fit one tile, whose
-    // matrix is then read once (an expert has `mean` rows or so), and fewer
-    // while the call has less than an item for each SM: small tiles spread over
-    // more SMs and have less to join.
-    const int64_t nblocks = (out_features + kOuts - 1) / kOuts;
-    const int64_t used = num_experts < pairs ? num_experts : pairs;
-    const int64_t mean = pairs / num_experts;
-    L.cap = num_experts == 1 || mean >= 24 ? 128 : mean >= 12 ? 64 : mean >= 4 ? 32 : 16;
-    while (L.cap > 16 && (used + (pairs - used) / L.cap) * nblocks < kMaxCtas) L.cap /= 2;
+    const Shape shape = shape_of(pairs, num_experts, out_features, 128);
+    L.cap = shape.cap;
+    L.outs = shape.outs;
     L.pitch = (width / kMxBlock + 15) / 16 * 16;
     L.max_tiles = (num_experts < pairs ? num_experts : pairs) + pairs / L.cap + 1;
     L.hdr = take(64);
@@ -718,13 +761,13 @@ cudaError_t launch_kernel(const ProductArgs &a, const Maps &maps, int sms, cudaS
 }
 
 cudaError_t encode_matrix(Maps &maps, const uint8_t *codes, const uint8_t *scales,
-                          int64_t scale_stride, int64_t rows, int64_t width) {
+                          int64_t scale_stride, int64_t rows, int64_t width, int outs) {
     const uint64_t code_row = (uint64_t)width / 2, scale_row = (uint64_t)width / kMxBlock;
     const cudaError_t err =
-        encode_rows(&maps.w, codes, code_row, (uint64_t)rows, code_row, 128, kOuts, true);
+        encode_rows(&maps.w, codes, code_row, (uint64_t)rows, code_row, 128, (uint32_t)outs, true);
     if (err != cudaSuccess) return err;
     return encode_rows(&maps.ws, scales, scale_row, (uint64_t)rows, (uint64_t)scale_stride, 16,
-                       kOuts, false);
+                       (uint32_t)outs, false);
 }
 
 }  // namespace
@@ -735,6 +778,7 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     a.width = p.width;
     a.pairs = p.pairs;
     a.cap = p.L.cap;
+    a.outs = p.L.outs;
     a.stages = stages_for(a.cap);
     a.hdr = reinterpret_cast<int32_t *>(p.ws + p.L.hdr);
     if (p.routed) {
@@ -747,7 +791,7 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     a.y_dtype = p.y_dtype;
     Maps maps;
     cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
-                                    p.num_experts * p.out_features, p.width);
+                                    p.num_experts * p.out_features, p.width, a.outs);
     // boxes up to the tile's rows; a lone matrix's tiles are full but the last
     const uint64_t code_row = (uint64_t)p.width / 2, scale_row = (uint64_t)p.width / kMxBlock;
     for (int i = 0; i < kBoxes && err == cudaSuccess && (16 << i) <= a.cap; ++i) {
@@ -789,6 +833,7 @@ cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
     a.width = p.width;
     a.pairs = p.pairs;
     a.cap = kFewCap;
+    a.outs = shape_of(p.pairs, p.num_experts, p.out_features, kFewCap).outs;
     a.stages = stages_for(a.cap);
     a.hdr = reinterpret_cast<int32_t *>(p.state);
     a.tickets = reinterpret_cast<int32_t *>(p.state + kStateTickets);
@@ -805,7 +850,7 @@ cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
     a.wide = aligned(p.x, 16) && p.x_stride * (int64_t)item % 16 == 0;
     Maps maps;
     const cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
-                                          p.num_experts * p.out_features, p.width);
+                                          p.num_experts * p.out_features, p.width, a.outs);
     if (err != cudaSuccess) return err;
     if (p.x_dtype == IQK_F32) return launch_kernel<true, float>(a, maps, sms, stream);
     if (p.x_dtype == IQK_F16) return launch_kernel<true, __half>(a, maps, sms, stream);
