@@ -30,7 +30,7 @@
 //               every fourth unit, so that four units' loads are under way
 //               (8 tokens' down projection 52 -> 39 us); with more, the warps
 //               share each unit (37 rows 14.2 -> 12 us)
-// Accumulators and scale buffers are double-buffered.
+// Accumulators are double-buffered, scale buffers four deep.
 //
 // Work: item = (128 outputs, tile of rows); a call of few items takes 64 or 32
 // outputs to an item and leaves the MMA's other rows unused, which spreads the
@@ -63,22 +63,29 @@ constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kSortWarp = 3, kMover0 
 __host__ __device__ constexpr int threads_of(bool few) { return few ? 512 : 384; }
 constexpr int kOuts = 128;              // outputs of an item at most (the MMA's M)
 constexpr int kUnit = 512;              // columns of a pipeline stage
-constexpr int kAtomA = kOuts * 128;     // one swizzle atom: 256 columns of 128 outputs
+constexpr int kScales = 4;              // scale buffers in tensor memory
 constexpr int kBoxes = 4;               // row boxes: 16, 32, 64, 128
-constexpr int kMaxStages = 5;
+constexpr int kMaxStages = 12;
 constexpr int kSmemCap = 227 * 1024;
-constexpr int kBarBytes = 256;
+constexpr int kBarBytes = 384;
 constexpr int kFewCap = 16, kFewPairs = 64;          // one launch: rows of a tile, routed pairs
-constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap + 4);  // tiles; pairs, rows of x; experts
+constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap);  // tiles; pairs, rows of x
 constexpr int kMaxCtas = 148;
 constexpr uint32_t kSaved = 14;
 
-// Shared memory of a stage: codes of the matrix, codes of the rows, scales.
-__host__ __device__ constexpr int stage_bytes(int cap) {
-    return 2 * kAtomA + 2 * cap * 128 + kOuts * 16 + cap * 16;
+// Shared memory of a stage: codes of the matrix and of the rows (two swizzle
+// atoms of 256 columns each), scales; in whole kilobytes, as the swizzle is.
+__host__ __device__ constexpr int stage_bytes(int cap, int outs) {
+    return (2 * (outs + cap) * 128 + (outs + cap) * 16 + 1023) / 1024 * 1024;
 }
-__host__ __device__ constexpr int stages_for(int cap) {
-    const int n = (kSmemCap - 1024 - kBarBytes - kFewTable) / ((stage_bytes(cap) + 1023) & ~1023);
+// The MMA reads 128 outputs of an atom whatever an item has: what follows an
+// atom must be shared memory too.
+__host__ __device__ constexpr int spare_bytes(int outs) { return (kOuts - outs) * 128; }
+__host__ __device__ constexpr int smem_fixed(int outs) {
+    return 1024 + kBarBytes + kFewTable + spare_bytes(outs);
+}
+__host__ __device__ constexpr int stages_for(int cap, int outs) {
+    const int n = (kSmemCap - smem_fixed(outs)) / stage_bytes(cap, outs);
     return n < kMaxStages ? n : kMaxStages;
 }
 
@@ -200,46 +207,64 @@ __device__ __forceinline__ void zero_row(const ProductArgs &a, int64_t p, int la
 
 // Few pairs, sorted by one warp (lane l: pairs l and l + 32): a pair's rank is
 // the number of earlier pairs of its expert, every 16th rank opens a tile, and
-// the pair's row is its rank in the tile. `all` is scratch for the experts.
-// Returns the tiles; `bad` says that an index is neither an expert nor -1.
+// the pair's row is its rank in the tile. Returns the tiles; `bad` says that an
+// index is neither an expert nor -1.
 __device__ __forceinline__ int sort_few(const ProductArgs &a, int lane, int4 *tiles,
-                                        int32_t *pairs, int32_t *rows, int4 *all, bool &bad) {
-    int e[2], rank[2] = {0, 0}, count[2] = {0, 0}, lead[2] = {0, 0};
-    bad = false;
+                                        int32_t *pairs, int32_t *rows, bool &bad) {
+    constexpr uint32_t kAll = 0xffffffffu;
+    int e[2], rank[2], count[2], lead[2] = {0, 0};
+    bool stray = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int p = lane + 32 * h;
         e[h] = p < a.pairs ? a.sel[p] : -1;
         if (e[h] < 0 || e[h] >= a.experts) {
-            bad |= e[h] != -1;
+            stray |= e[h] != -1;
             e[h] = -1;
         }
-        reinterpret_cast<int32_t *>(all)[p] = e[h];
     }
-    bad = __any_sync(0xffffffffu, bad);
-    __syncwarp();
-    for (int q = 0; q < (int)a.pairs; q += 4) {
-        const int4 four = all[q / 4];
-        const int other[4] = {four.x, four.y, four.z, four.w};
+    bad = __any_sync(kAll, stray);
+    const bool two = a.pairs > 32;
+    const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (other[j] == e[h]) {
-                    // the pair that opened this one's tile
-                    if (q + j <= lane + 32 * h && count[h] % kFewCap == 0) lead[h] = q + j;
-                    rank[h] += q + j < lane + 32 * h;
-                    ++count[h];
-                }
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t same = __match_any_sync(kAll, e[h]);
+        rank[h] = __popc(same & below);
+        count[h] = __popc(same);
     }
-    const uint32_t m0 = __ballot_sync(0xffffffffu, e[0] >= 0 && lead[0] == lane);
-    const uint32_t m1 = __ballot_sync(0xffffffffu, e[1] >= 0 && lead[1] == lane + 32);
+    if (two) {
+#pragma unroll 8
+        for (int q = 0; q < 32; ++q) {
+            const int other0 = __shfl_sync(kAll, e[0], q), other1 = __shfl_sync(kAll, e[1], q);
+            const int in0 = other0 == e[1], in1 = other1 == e[0];
+            rank[1] += in0;
+            count[1] += in0;
+            count[0] += in1;
+        }
+    }
+    const uint32_t m0 = __ballot_sync(kAll, e[0] >= 0 && rank[0] % kFewCap == 0);
+    const uint32_t m1 = __ballot_sync(kAll, e[1] >= 0 && rank[1] % kFewCap == 0);
+    // the pair that opened this one's tile
+    const int from[2] = {rank[0] & -kFewCap, rank[1] & -kFewCap};
+#pragma unroll 8
+    for (int q = 0; q < 32; ++q) {
+        const int oe = __shfl_sync(kAll, e[0], q), orank = __shfl_sync(kAll, rank[0], q);
+        if (oe == e[0] && orank == from[0]) lead[0] = q;
+        if (oe == e[1] && orank == from[1]) lead[1] = q;
+    }
+    if (two) {
+#pragma unroll 8
+        for (int q = 0; q < 32; ++q) {
+            const int oe = __shfl_sync(kAll, e[1], q), orank = __shfl_sync(kAll, rank[1], q);
+            if (oe == e[1] && orank == from[1]) lead[1] = q + 32;
+        }
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (e[h] < 0) continue;
         const int p = lane + 32 * h;
-        const uint32_t below = (1u << (lead[h] & 31)) - 1u;
-        const int tile = lead[h] < 32 ? __popc(m0 & below) : __popc(m0) + __popc(m1 & below);
+        const uint32_t under = (1u << (lead[h] & 31)) - 1u;
+        const int tile = lead[h] < 32 ? __popc(m0 & under) : __popc(m0) + __popc(m1 & under);
         const int at = tile * kFewCap + rank[h] % kFewCap;
         if (lead[h] == p)
             tiles[tile] = make_int4(e[h], tile * kFewCap, min(kFewCap, count[h] - rank[h]), 0);
@@ -310,12 +335,12 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
     const uint32_t raw = saddr(smem_raw);
     const uint32_t smem = (raw + 1023u) & ~1023u;
     const int S = a.stages, cap = a.cap;
-    const uint32_t stage = (uint32_t)((stage_bytes(cap) + 1023) & ~1023);
+    const uint32_t stage = (uint32_t)stage_bytes(cap, a.outs);
     char *bars = smem_raw + (smem - raw) + S * stage;
     uint64_t *full = reinterpret_cast<uint64_t *>(bars);
     uint64_t *empty = full + kMaxStages;
-    uint64_t *sready = empty + kMaxStages, *sfree = sready + 2;
-    uint64_t *dfull = sfree + 2, *dempty = dfull + 2, *drain = dempty + 2;
+    uint64_t *sready = empty + kMaxStages, *sfree = sready + kScales;
+    uint64_t *dfull = sfree + kScales, *dempty = dfull + 2, *drain = dempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
     int *tile_count = reinterpret_cast<int *>(tmem_slot + 2);
@@ -329,9 +354,11 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             bar_init(&full[i], !FEW ? 1 : a.spread ? 5 : 2);
             bar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kScales; ++i) {
             bar_init(&sready[i], 4);
             bar_init(&sfree[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
             bar_init(&dfull[i], 1);
             bar_init(&dempty[i], 4);
         }
@@ -351,8 +378,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
     if (FEW && a.sel) {
         if (warp == kSortWarp) {
             bool bad;
-            const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows,
-                                   reinterpret_cast<int4 *>(few_rows + kFewPairs * kFewCap), bad);
+            const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows, bad);
             if (lane == 0) {
                 *tile_count = n;
                 if (blockIdx.x == 0) a.hdr[0] = bad ? IQK_DEVERR_EXPERT : 0;
@@ -375,7 +401,8 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             atomicOr(a.hdr + 3, IQK_DEVERR_TIMEOUT);
         }
     };
-    const uint32_t off_b = 2 * kAtomA, off_sa = off_b + 2 * cap * 128, off_sb = off_sa + kOuts * 16;
+    const uint32_t atom = (uint32_t)a.outs * 128;
+    const uint32_t off_b = 2 * atom, off_sa = off_b + 2 * cap * 128, off_sb = off_sa + a.outs * 16;
 
     if (warp == kProducer) {
         if (lane == 0) {
@@ -399,7 +426,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
                     bar_expect_tx(&full[s], (uint32_t)((atoms * 128 + 16) * (a.outs + xrows)));
                     const uint32_t st = smem + s * stage;
                     for (int t = 0; t < atoms; ++t) {
-                        tma_2d(st + t * kAtomA, &maps.w, u * 256 + t * 128, row0, &full[s]);
+                        tma_2d(st + t * atom, &maps.w, u * 256 + t * 128, row0, &full[s]);
                         if (!FEW)
                             tma_2d(st + off_b + t * rows * 128, &maps.x[box], u * 256 + t * 128,
                                    tl.y, &full[s]);
@@ -429,9 +456,9 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             for (int u = q.u0; u < q.u1; ++u, ++g) {
-                const int s = g % S, b = g & 1;
+                const int s = g % S, b = g % kScales;
                 ok = bar_wait_spin(&full[s], (uint32_t)(g / S) & 1u, abort_flag) &&
-                     bar_wait_spin(&sready[b], (uint32_t)(g >> 1) & 1u, abort_flag);
+                     bar_wait_spin(&sready[b], (uint32_t)(g / kScales) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);  // elect.sync needs the warp converged
                 if (!ok) break;
                 tc_fence_after();
@@ -441,7 +468,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
                     const uint32_t sa = scale_col + b * 32, sb = sa + 16;
                     for (int k = 0; k < steps; ++k) {
                         const uint32_t in = (uint32_t)(k & 3) * 32;
-                        tc_mma_mxf4(tmem + acc * cap, sw128_desc(st + (k >> 2) * kAtomA + in),
+                        tc_mma_mxf4(tmem + acc * cap, sw128_desc(st + (k >> 2) * atom + in),
                                     sw128_desc(st + off_b + (k >> 2) * rows * 128 + in),
                                     idesc_mxf4(kOuts, npad, (k & 1) * 2), sa + (k >> 1) * 4,
                                     sb + (k >> 1) * 4, (u > q.u0 || k > 0) ? 1u : 0u);
@@ -469,9 +496,10 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int rows = 16 << box_of(tl.z);
             for (int u = q.u0; u < q.u1; ++u, ++g) {
-                const int s = g % S, b = g & 1;
+                const int s = g % S, b = g % kScales;
                 ok = bar_wait(&full[s], (uint32_t)(g / S) & 1u, abort_flag) &&
-                     (g < 2 || bar_wait(&sfree[b], ((uint32_t)(g >> 1) & 1u) ^ 1u, abort_flag));
+                     (g < kScales ||
+                      bar_wait(&sfree[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag));
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
@@ -481,7 +509,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 32 * j + lane;
-                    w[j] = lds128(st + off_sa + r * 16);
+                    w[j] = r < a.outs ? lds128(st + off_sa + r * 16) : make_uint4(0u, 0u, 0u, 0u);
                     x[j] = r < rows ? lds128(st + off_sb + r * 16) : make_uint4(0u, 0u, 0u, 0u);
                 }
                 tmem_st4(dst + 0, w[0].x, w[1].x, w[2].x, w[3].x);
@@ -620,17 +648,18 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             if (lane == 0) a.tickets[shared_item * 4 + quarter] = 0;
             // the first owner's run may have begun in an earlier item
             const bool early = plan.start(o0) / plan.units != shared_item;
-            for (int c = 0; c < tl.z; c += 32) {
-                float v[32] = {};
-                const int here = min(32, tl.z - c);
+            constexpr int kBatch = FEW ? 16 : 32;  // loads under way
+            for (int c = 0; c < tl.z; c += kBatch) {
+                float v[kBatch] = {};
+                const int here = min(kBatch, tl.z - c);
                 for (uint32_t o = o0; o <= o1; ++o) {
                     const float *part = a.slots +
                         ((int64_t)o * 2 + (o == o0 && early ? 1 : 0)) * cap * kOuts + c * kOuts + r;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
+                    for (int j = 0; j < kBatch; ++j)
                         if (j < here) v[j] += __ldcg(part + j * kOuts);
                 }
-                store_columns<32>(a, v, here, row_base(a, tl, c, lane), lane, out0 + r, pairs);
+                store_columns<kBatch>(a, v, here, row_base(a, tl, c, lane), lane, out0 + r, pairs);
             }
         }
     }
@@ -682,10 +711,12 @@ cudaError_t encode_rows(CUtensorMap *map, const void *base, uint64_t row_used, u
 
 namespace {
 
-// The shape of an item: `cap` rows, `outs` outputs. A CTA's time goes by the
-// bytes that it loads, (rows + outputs) of each column block, times the rounds
-// of items. Large items load least in all; small ones fill the SMs. A smaller
-// shape is taken where it saves a tenth or more.
+// The shape of an item: `cap` rows, `outs` outputs. A round of items costs a
+// CTA, per unit, the bytes that it loads (512 columns of rows and outputs, 272
+// bytes each) at its share of the memory's 6500 bytes a ns, or at the 90 that
+// one SM can take, and 0.3 us at least for the steps from a load to the next.
+// Large items load least in all; small ones fill the SMs. A smaller shape is
+// taken where it saves a tenth or more.
 struct Shape {
     int cap, outs;
 };
@@ -704,7 +735,15 @@ Shape shape_of(int64_t pairs, int64_t experts, int64_t out_features, int most) {
         const int64_t rows = mean < cap ? mean : cap;
         for (int outs = kOuts; outs >= 32; outs /= 2) {
             const int64_t items = tiles * ((out_features + outs - 1) / outs);
-            const double cost = (double)((items + kMaxCtas - 1) / kMaxCtas) * (double)(rows + outs);
+            const double bytes = 272.0 * (double)(rows + outs);
+            auto round = [&](int64_t ctas) {
+                const double shared = bytes * (double)ctas / 6500.0, alone = bytes / 90.0;
+                const double ns = shared > alone ? shared : alone;
+                return ns > 300.0 ? ns : 300.0;
+            };
+            const int64_t rest = items % kMaxCtas;
+            const double cost = (double)(items / kMaxCtas) * round(kMaxCtas) +
+                                (rest ? round(rest) : 0.0);
             if (!best.cap || cost < 0.9 * least) {
                 best = Shape{cap, outs};
                 least = cost;
@@ -754,7 +793,7 @@ cudaError_t launch_kernel(const ProductArgs &a, const Maps &maps, int sms, cudaS
         if (err != cudaSuccess) return err;
         if (dev >= 0) attr_done[dev].store(true);
     }
-    const int smem = 1024 + a.stages * ((stage_bytes(a.cap) + 1023) & ~1023) + kBarBytes + kFewTable;
+    const int smem = smem_fixed(a.outs) + a.stages * stage_bytes(a.cap, a.outs);
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
     mx_product_kernel<FEW, XT><<<(unsigned)grid, threads_of(FEW), smem, stream>>>(a, maps);
     return cudaGetLastError();
@@ -779,7 +818,7 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     a.pairs = p.pairs;
     a.cap = p.L.cap;
     a.outs = p.L.outs;
-    a.stages = stages_for(a.cap);
+    a.stages = stages_for(a.cap, a.outs);
     a.hdr = reinterpret_cast<int32_t *>(p.ws + p.L.hdr);
     if (p.routed) {
         a.order = reinterpret_cast<const int32_t *>(p.ws + p.L.order);
@@ -834,7 +873,7 @@ cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
     a.pairs = p.pairs;
     a.cap = kFewCap;
     a.outs = shape_of(p.pairs, p.num_experts, p.out_features, kFewCap).outs;
-    a.stages = stages_for(a.cap);
+    a.stages = stages_for(a.cap, a.outs);
     a.hdr = reinterpret_cast<int32_t *>(p.state);
     a.tickets = reinterpret_cast<int32_t *>(p.state + kStateTickets);
     a.slots = reinterpret_cast<float *>(p.state + kStateSlots);
