@@ -12,8 +12,10 @@
 // field, so the maximum of the magnitudes' bit patterns finds it, and the
 // block's scale byte is 255 (NaN).
 //
-// Both kernels are bound by HBM: four threads a block, eight values each, in
-// 16-byte accesses.
+// Both kernels are bound by memory: every thread moves 16 bytes at a time and
+// starts kAhead of them before it waits for the first.
+#include <cooperative_groups.h>
+
 #include "iqk_host.cuh"
 #include "iqk_mx.cuh"
 #include "iqk_mx_block.cuh"
@@ -25,36 +27,52 @@ namespace {
 // place[r * copies ..] of its `copies` pairs (-1: none), so that a token's row
 // is read and rounded once. Block 0 clears the words that the product kernel
 // counts in.
-template <typename T, bool WIDE>
+// Four threads share a block, eight values each. I: an index type that holds
+// rows * width / 8.
+constexpr int kAhead = 4;
+
+template <typename T, bool WIDE, typename I>
 __global__ void __launch_bounds__(256)
-mx_quantize_kernel(const T *__restrict__ x, int64_t rows, int64_t width, int64_t row_stride,
+mx_quantize_kernel(const T *__restrict__ x, I rows, I width, int64_t row_stride,
                    uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
                    int64_t scale_stride, const int32_t *__restrict__ place, int copies,
                    int32_t *__restrict__ zero, int zero_words) {
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero[i] = 0;
-    const int64_t per = width / 8;  // threads of a row
-    const int64_t all = rows * per;
-    // whole groups of four lanes run or stop together: `per` is a multiple of 4
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / per, c = i % per;
-        float v[8];
-        load8<T, WIDE>(x + r * row_stride + c * 8, v);
-        uint32_t amax = 0;
+    const I per = width / 8, all = rows * per, wave = (I)blockDim.x * kAhead;
+    for (I i0 = (I)blockIdx.x * wave + threadIdx.x; i0 < all; i0 += (I)gridDim.x * wave) {
+        Raw8<T> raw[kAhead];
+        I row[kAhead], col[kAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
-        const unsigned group = 0xfu << (threadIdx.x & 28u);
-        amax = max(amax, __shfl_xor_sync(group, amax, 1));
-        amax = max(amax, __shfl_xor_sync(group, amax, 2));
-        float inv;
-        const uint32_t byte = scale_byte(amax, inv);
-        const uint32_t packed = codes8(v, inv);
-        for (int j = 0; j < copies; ++j) {
-            const int64_t to = place ? place[r * copies + j] : r;
-            if (to < 0) continue;
-            *reinterpret_cast<uint32_t *>(codes + to * (width / 2) + c * 4) = packed;
-            if ((c & 3) == 0) scales[to * scale_stride + c / 4] = (uint8_t)byte;
+        for (int h = 0; h < kAhead; ++h) {
+            const I i = i0 + (I)h * blockDim.x;
+            row[h] = i / per;
+            col[h] = i - row[h] * per;
+            if (i < all) load8<T, WIDE>(x + (int64_t)row[h] * row_stride + (int64_t)col[h] * 8, raw[h]);
+        }
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h) {
+            // `all` is a multiple of four: a block's four lanes stop together
+            if (i0 + (I)h * blockDim.x >= all) break;
+            float v[8];
+            raw[h].get(v);
+            uint32_t amax = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+            const unsigned group = 0xfu << (threadIdx.x & 28u);
+            amax = max(amax, __shfl_xor_sync(group, amax, 1));
+            amax = max(amax, __shfl_xor_sync(group, amax, 2));
+            float inv;
+            const uint32_t byte = scale_byte(amax, inv);
+            const uint32_t packed = codes8(v, inv);
+            for (int j = 0; j < copies; ++j) {
+                const int64_t to = place ? (int64_t)place[(int64_t)row[h] * copies + j] : (int64_t)row[h];
+                if (to < 0) continue;
+                *reinterpret_cast<uint32_t *>(codes + to * (int64_t)(width / 2) +
+                                              (int64_t)col[h] * 4) = packed;
+                if ((col[h] & 3) == 0)
+                    scales[to * scale_stride + (int64_t)(col[h] / 4)] = (uint8_t)byte;
+            }
         }
     }
 }
@@ -65,86 +83,127 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
 
-__device__ __forceinline__ float code_value(uint32_t code) {
-    // {0, 1, 2, 3, 4, 6, 8, 12} halves: 4-bit entries of one word
-    const float size = 0.5f * (float)((0xC8643210u >> (4 * (code & 7u))) & 15u);
-    return (code & 8u) ? -size : size;
+// Two codes of a byte to two values.
+__device__ __forceinline__ float2 code_values(uint32_t byte) {
+    uint32_t h;
+    asm("{\n .reg .b8 b, z;\n mov.b32 {b, z, z, z}, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n"
+        : "=r"(h) : "r"(byte));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-template <typename T>
+// A thread writes 16 bytes: four f32 or eight 16-bit values.
+template <typename T, typename I>
 __global__ void __launch_bounds__(256)
 mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                     int64_t scale_stride, int64_t rows, int64_t width, T *__restrict__ out) {
-    const int64_t per = width / 8, all = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / per, c = i % per;
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + r * (width / 2) + c * 4);
-        const float s = scale_value(scales[r * scale_stride + c / 4]);
-        T v[8];
+                     int64_t scale_stride, I rows, I width, T *__restrict__ out) {
+    constexpr int kN = 16 / (int)sizeof(T);
+    const I per = width / kN, all = rows * per, wave = (I)blockDim.x * kAhead;
+    for (I i0 = (I)blockIdx.x * wave + threadIdx.x; i0 < all; i0 += (I)gridDim.x * wave) {
+        uint32_t word[kAhead], byte[kAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from_float<T>(code_value((w >> (4 * j)) & 15u) * s);
-        uint4 *dst = reinterpret_cast<uint4 *>(out + r * width + c * 8);
+        for (int h = 0; h < kAhead; ++h) {
+            const I i = i0 + (I)h * blockDim.x;
+            if (i >= all) break;
+            const I r = i / per, c = i - r * per;
+            if constexpr (kN == 4) word[h] = reinterpret_cast<const uint16_t *>(codes)[i];
+            else word[h] = reinterpret_cast<const uint32_t *>(codes)[i];
+            byte[h] = scales[(int64_t)r * scale_stride + (int64_t)(c / (kMxBlock / kN))];
+        }
 #pragma unroll
-        for (int j = 0; j < (int)sizeof(T) / 2; ++j)
-            dst[j] = reinterpret_cast<const uint4 *>(v)[j];
+        for (int h = 0; h < kAhead; ++h) {
+            const I i = i0 + (I)h * blockDim.x;
+            if (i >= all) break;
+            const float s = scale_value(byte[h]);
+            uint4 u;
+            T *v = reinterpret_cast<T *>(&u);
+#pragma unroll
+            for (int j = 0; j < kN / 2; ++j) {
+                const float2 f = code_values((word[h] >> (8 * j)) & 0xffu);
+                v[2 * j] = from_float<T>(f.x * s);
+                v[2 * j + 1] = from_float<T>(f.y * s);
+            }
+            reinterpret_cast<uint4 *>(out)[i] = u;
+        }
     }
 }
 
-// Pairs by expert: one block counts, cuts each expert's run into tiles of at
-// most L.cap rows and gives every pair its place; those without an expert go
-// to the tail of `order` and have place -1. Counting hands out the ranks, so
-// the second pass needs no atomics. The order of an expert's pairs changes no
-// result: each is a row of its own. Latency bounds it (one SM): a thread loads
-// and stores four pairs at a time.
-__global__ void __launch_bounds__(1024)
+// Pairs by expert. A cluster of eight CTAs takes an eighth of the pairs each:
+// it counts its pairs by expert (counting hands out the ranks, so that the
+// second pass needs no atomics), reads the other CTAs' counts, and gives each
+// of its pairs its place behind those of the CTAs before it. Pairs without an
+// expert go to the tail of `order` and have place -1. The order of an expert's
+// pairs changes no result: each is a row of its own. CTA 0 cuts each expert's
+// run into tiles of at most L.cap rows. Latency bounds it: one CTA took 14 us
+// for 12288 pairs, most of it in shared-memory atomics.
+constexpr int kSortCtas = 8;
+
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(1024)
 mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLayout L,
                char *ws) {
-    extern __shared__ int32_t cnt[];
-    __shared__ int32_t warp_rows[32], warp_tiles[32], bad, tail;
+    extern __shared__ int32_t cnt[];  // [num_experts + 1]: the last has no expert
+    __shared__ int32_t warp_rows[32], warp_tiles[32], none_base;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, wid = tid >> 5;
+    const int rank = blockIdx.x;
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     int32_t *hdr = reinterpret_cast<int32_t *>(ws + L.hdr);
     int32_t *order = reinterpret_cast<int32_t *>(ws + L.order);
     int32_t *place = reinterpret_cast<int32_t *>(ws + L.place);
     int4 *tiles = reinterpret_cast<int4 *>(ws + L.tiles);
-    for (int e = tid; e < num_experts; e += nt) cnt[e] = 0;
-    for (int i = tid; i < L.zeroed(); i += nt) hdr[i] = 0;
-    if (tid == 0) bad = tail = 0;
+    for (int e = tid; e <= num_experts; e += nt) cnt[e] = 0;
+    if (rank == 0)
+        for (int i = tid; i < L.zeroed(); i += nt) hdr[i] = 0;
     const bool quads = (reinterpret_cast<uintptr_t>(sel) & 15) == 0;
-    // the experts of pairs p .. p + 3 (-1 past the last and for any that is none)
-    auto experts4 = [&](int p, int (&e)[4]) {
-        if (quads && p + 3 < pairs) {
+    const int chunk = ((pairs + kSortCtas - 1) / kSortCtas + 3) / 4 * 4;
+    const int p0 = rank * chunk, p1 = min(p0 + chunk, pairs);
+    // the buckets of pairs p .. p + 3
+    auto buckets = [&](int p, int (&e)[4]) {
+        if (quads && p + 3 < p1) {
             const int4 v = *reinterpret_cast<const int4 *>(sel + p);
             e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = p + j < pairs ? sel[p + j] : -1;
+            for (int j = 0; j < 4; ++j) e[j] = p + j < p1 ? sel[p + j] : -1;
         }
     };
     auto is_expert = [&](int e) { return e >= 0 && e < num_experts; };
+    int stray = 0;
     __syncthreads();
-    for (int p = 4 * tid; p < pairs; p += 4 * nt) {
+    for (int p = p0 + 4 * tid; p < p1; p += 4 * nt) {
         int e[4];
-        experts4(p, e);
-        int4 rank;  // within the expert, or among those without one
-        int *r = &rank.x;
+        buckets(p, e);
+        int4 ranks = make_int4(0, 0, 0, 0);
+        int *r = &ranks.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            r[j] = 0;
-            if (p + j >= pairs) continue;
-            r[j] = atomicAdd(is_expert(e[j]) ? &cnt[e[j]] : &tail, 1);
-            if (e[j] < -1 || e[j] >= num_experts) bad = IQK_DEVERR_EXPERT;
+            if (p + j >= p1) continue;
+            r[j] = atomicAdd(&cnt[is_expert(e[j]) ? e[j] : num_experts], 1);
+            stray |= !is_expert(e[j]) && e[j] != -1;
         }
-        *reinterpret_cast<int4 *>(place + p) = rank;  // whole quads: see the layout
+        *reinterpret_cast<int4 *>(place + p) = ranks;  // whole quads: see the layout
     }
-    __syncthreads();
+    stray = __syncthreads_or(stray);
+    cluster.sync();
     // exclusive sums of rows and tiles over the experts, `per` a thread
     const int per = (num_experts + nt - 1) / nt;
     const int e0 = min(tid * per, num_experts), e1 = min(e0 + per, num_experts);
-    int rows = 0, made = 0;
-    for (int e = e0; e < e1; ++e) {
-        rows += cnt[e];
-        made += (cnt[e] + L.cap - 1) / L.cap;
+    int rows = 0, made = 0, mine[4], total[4];  // per <= 4: at most 4096 experts
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        mine[k] = total[k] = 0;
+        if (e0 + k >= e1) continue;
+#pragma unroll
+        for (int c = 0; c < kSortCtas; ++c) {
+            const int n = cluster.map_shared_rank(cnt, c)[e0 + k];
+            mine[k] += c < rank ? n : 0;
+            total[k] += n;
+        }
+        rows += total[k];
+        made += (total[k] + L.cap - 1) / L.cap;
+    }
+    if (tid == 0) {
+        int n = 0;
+        for (int c = 0; c < rank; ++c) n += cluster.map_shared_rank(cnt, c)[num_experts];
+        none_base = n;
     }
     int at = rows, tile = made;
 #pragma unroll
@@ -153,40 +212,53 @@ mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLa
         if (lane >= o) at += a, tile += b;
     }
     if (lane == 31) warp_rows[wid] = at, warp_tiles[wid] = tile;
-    __syncthreads();
+    cluster.sync();  // every CTA has read the counts: they become cursors
     at -= rows, tile -= made;
     int all_rows = 0, all_tiles = 0;
-    for (int w = 0; w < (nt >> 5); ++w) {
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
         if (w == wid) at += all_rows, tile += all_tiles;
         all_rows += warp_rows[w], all_tiles += warp_tiles[w];
     }
-    for (int e = e0; e < e1; ++e) {
-        const int c = cnt[e];
-        for (int i = 0; i < c; i += L.cap)
-            tiles[tile++] = make_int4(e, at + i, min(L.cap, c - i), 0);
-        cnt[e] = at;
-        at += c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (e0 + k >= e1) continue;
+        if (rank == 0)
+            for (int i = 0; i < total[k]; i += L.cap)
+                tiles[tile++] = make_int4(e0 + k, at + i, min(L.cap, total[k] - i), 0);
+        cnt[e0 + k] = at + mine[k];
+        at += total[k];
     }
     if (tid == 0) {
-        hdr[0] = bad;
-        hdr[1] = all_tiles;
-        hdr[2] = all_rows;
+        cnt[num_experts] = all_rows + none_base;
+        if (rank == 0) {
+            hdr[1] = all_tiles;
+            hdr[2] = all_rows;
+        }
     }
     __syncthreads();
-    for (int p = 4 * tid; p < pairs; p += 4 * nt) {
+    // after the clearing of hdr: the cluster has synchronised twice since
+    if (tid == 0 && stray) atomicOr(hdr, IQK_DEVERR_EXPERT);
+    for (int p = p0 + 4 * tid; p < p1; p += 4 * nt) {
         int e[4];
-        experts4(p, e);
+        buckets(p, e);
         int4 to = *reinterpret_cast<const int4 *>(place + p);
         int *r = &to.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (p + j >= pairs) continue;
-            r[j] += is_expert(e[j]) ? cnt[e[j]] : all_rows;
+            if (p + j >= p1) continue;
+            r[j] += cnt[is_expert(e[j]) ? e[j] : num_experts];
             order[r[j]] = p + j;
             if (!is_expert(e[j])) r[j] = -1;
         }
         *reinterpret_cast<int4 *>(place + p) = to;
     }
+}
+
+// Blocks of a streaming kernel: eight an SM, fewer for fewer items.
+unsigned stream_blocks(int64_t items, int sms) {
+    const int64_t want = (items + 256 * kAhead - 1) / (256 * kAhead), most = (int64_t)sms * 8;
+    return (unsigned)(want < most ? want : most);
 }
 
 size_t element(int dtype) { return dtype == IQK_F32 ? 4 : 2; }
@@ -224,24 +296,24 @@ cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t w
                                int64_t scale_stride, const int32_t *place, int copies,
                                int32_t *zero, int zero_words,
                                cudaStream_t stream, int sms) {
-    const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)sms * 16;
-    const unsigned blocks = (unsigned)(want < most ? want : most);
+    const unsigned blocks = stream_blocks(rows * (width / 8), sms);
     const bool wide = aligned(x, 16) && row_stride * (int64_t)element(dtype) % 16 == 0;
-#define IQK_Q(T, W)                                                                           \
-    mx_quantize_kernel<T, W><<<blocks, 256, 0, stream>>>(static_cast<const T *>(x), rows,     \
-                                                         width, row_stride, codes, scales,    \
-                                                         scale_stride, place, copies, zero,   \
-                                                         zero_words)
-    if (dtype == IQK_F32) {
-        if (wide) IQK_Q(float, true);
-        else IQK_Q(float, false);
-    } else if (dtype == IQK_F16) {
-        if (wide) IQK_Q(__half, true);
-        else IQK_Q(__half, false);
-    } else {
-        if (wide) IQK_Q(__nv_bfloat16, true);
-        else IQK_Q(__nv_bfloat16, false);
-    }
+    const bool small = rows * (width / 8) < (int64_t)1 << 31;
+#define IQK_QI(T, W, I)                                                                         \
+    mx_quantize_kernel<T, W, I><<<blocks, 256, 0, stream>>>(                                    \
+        static_cast<const T *>(x), (I)rows, (I)width, row_stride, codes, scales, scale_stride,  \
+        place, copies, zero, zero_words)
+#define IQK_Q(T)                                        \
+    do {                                                \
+        if (wide && small) IQK_QI(T, true, uint32_t);   \
+        else if (small) IQK_QI(T, false, uint32_t);     \
+        else if (wide) IQK_QI(T, true, uint64_t);       \
+        else IQK_QI(T, false, uint64_t);                \
+    } while (0)
+    if (dtype == IQK_F32) IQK_Q(float);
+    else if (dtype == IQK_F16) IQK_Q(__half);
+    else IQK_Q(__nv_bfloat16);
+#undef IQK_QI
 #undef IQK_Q
     return cudaGetLastError();
 }
@@ -272,15 +344,22 @@ int iqk_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t scale
     if (rows == 0) return IQK_OK;
     if (!out) return IQK_ERR_ARGUMENT;
     if (!aligned(out, 16)) return IQK_ERR_ALIGNMENT;
-    const int64_t want = (rows * (width / 8) + 255) / 256, most = (int64_t)num_sms_current() * 16;
-    const unsigned blocks = (unsigned)(want < most ? want : most);
+    const int64_t items = rows * width * (int64_t)element(out_dtype) / 16;
+    const unsigned blocks = stream_blocks(items, num_sms_current());
+    const bool small = items < (int64_t)1 << 31;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define IQK_D(T)                                                                        \
-    mx_dequantize_kernel<T><<<blocks, 256, 0, s>>>(codes, scales, scale_stride, rows, width, \
-                                                   static_cast<T *>(out))
+#define IQK_DI(T, I)                                                                   \
+    mx_dequantize_kernel<T, I><<<blocks, 256, 0, s>>>(codes, scales, scale_stride, (I)rows, \
+                                                      (I)width, static_cast<T *>(out))
+#define IQK_D(T)                      \
+    do {                              \
+        if (small) IQK_DI(T, uint32_t); \
+        else IQK_DI(T, uint64_t);     \
+    } while (0)
     if (out_dtype == IQK_F32) IQK_D(float);
     else if (out_dtype == IQK_F16) IQK_D(__half);
     else IQK_D(__nv_bfloat16);
+#undef IQK_DI
 #undef IQK_D
     return cuda_status(cudaGetLastError());
 }
@@ -345,7 +424,7 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
     if (!mx_items_ok(p)) return IQK_ERR_GEOMETRY;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = num_sms_current();
-    mx_sort_kernel<<<1, 1024, sizeof(int32_t) * (size_t)num_experts, s>>>(
+    mx_sort_kernel<<<kSortCtas, 1024, sizeof(int32_t) * (size_t)(num_experts + 1), s>>>(
         sel, (int)pairs, (int)num_experts, p.L, p.ws);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return cuda_status(err);

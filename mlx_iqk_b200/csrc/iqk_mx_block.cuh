@@ -5,23 +5,31 @@
 
 namespace iqk {
 
-// Eight consecutive values as f32.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    if constexpr (!WIDE) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j]);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0];
-        const float4 b = reinterpret_cast<const float4 *>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const T *e = reinterpret_cast<const T *>(&u);
+// Eight consecutive values as loaded, and as f32.
+template <typename T> struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = to_float<T>(e[j]);
     }
+};
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *p, Raw8<T> &r) {
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) r.w[j] = reinterpret_cast<const uint4 *>(p)[j];
+    } else {
+        T *e = reinterpret_cast<T *>(r.w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = p[j];
+    }
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    Raw8<T> r;
+    load8<T, WIDE>(p, r);
+    r.get(v);
 }
 
 // Two values to two codes, `lo` in the low nibble.
