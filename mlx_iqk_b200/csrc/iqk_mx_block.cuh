@@ -13,6 +13,40 @@ template <typename T> struct Raw8 {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = to_float<T>(e[j]);
     }
+    // The largest magnitude's f32 bits (NaN above infinity above numbers):
+    // 16-bit types compare two magnitudes at a time.
+    __device__ __forceinline__ uint32_t peak() const {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t *b = reinterpret_cast<const uint32_t *>(w);
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, b[j] & 0x7fffffffu);
+            return m;
+        } else {
+            constexpr uint32_t kSize = 0x7fff7fffu;
+            const uint32_t m2 = __vmaxu2(__vmaxu2(w[0].x & kSize, w[0].y & kSize),
+                                         __vmaxu2(w[0].z & kSize, w[0].w & kSize));
+            const uint16_t m = (uint16_t)max(m2 & 0xffffu, m2 >> 16);
+            return __float_as_uint(to_float<T>(*reinterpret_cast<const T *>(&m))) & 0x7fffffffu;
+        }
+    }
+};
+
+// Row and column of an item that moves on by a fixed number of items: no
+// division after the first.
+template <typename I> struct Walk {
+    I row, col, per, rows_on, cols_on;
+    __device__ __forceinline__ Walk(I at, I per_row, I step)
+        : row(at / per_row), col(at % per_row), per(per_row), rows_on(step / per_row),
+          cols_on(step % per_row) {}
+    __device__ __forceinline__ void next() {
+        row += rows_on;
+        col += cols_on;
+        if (col >= per) {
+            col -= per;
+            ++row;
+        }
+    }
 };
 template <typename T, bool WIDE>
 __device__ __forceinline__ void load8(const T *p, Raw8<T> &r) {

@@ -48,6 +48,8 @@
 // is freed before the CTA exits.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "iqk_host.cuh"
 #include "iqk_mx.cuh"
 #include "iqk_mx_block.cuh"
@@ -107,10 +109,13 @@ struct ProductArgs {
     int spread;            // the four rounding warps share each unit, else take turns
 };
 
-struct Maps {
-    CUtensorMap w, ws;                // matrix codes, scales
+struct MatrixMaps {
+    CUtensorMap w, ws;  // matrix codes, scales
+};
+struct Maps : MatrixMaps {
     CUtensorMap x[kBoxes], xs[kBoxes];  // rows' codes, scales; boxes of 16 << i rows
 };
+template <bool FEW> using MapsOf = typename std::conditional<FEW, MatrixMaps, Maps>::type;
 
 // The items of a call and how they are dealt to the CTAs.
 struct Plan {
@@ -175,8 +180,10 @@ __device__ __forceinline__ int4 tile_of(const ProductArgs &a, const Plan &p, uin
     return make_int4(0, (int)(t * a.cap), (int)min((int64_t)a.cap, a.pairs - (int64_t)t * a.cap), 0);
 }
 
-// The smallest box that holds `rows`.
-__device__ __forceinline__ int box_of(int rows) {
+// The smallest box that holds the tile's rows; one matrix: the box of a full
+// tile, which the last one's rows beyond the activations read as zeros.
+__device__ __forceinline__ int box_of(const ProductArgs &a, const int4 &tile) {
+    const int rows = a.tiles ? tile.z : a.cap;
     return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
 }
 
@@ -328,7 +335,8 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, const float 
 // FEW: activations of type XT, rounded in the kernel; else from the workspace.
 template <bool FEW, typename XT>
 __global__ void __launch_bounds__(threads_of(FEW), 1)
-mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constant__ Maps maps) {
+mx_product_kernel(const __grid_constant__ ProductArgs args,
+                  const __grid_constant__ MapsOf<FEW> maps) {
     ProductArgs a = args;
     extern __shared__ char smem_raw[];
     // swizzle atoms repeat every 1024 bytes of shared memory
@@ -412,7 +420,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
             for (uint32_t i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
                 int out0;
                 const int4 tl = tile_of(a, plan, q.item, out0);
-                const int box = box_of(tl.z), rows = 16 << box;
+                const int box = box_of(a, tl), rows = 16 << box;
                 const int row0 = (int)((int64_t)tl.x * a.out_features + out0);
                 for (int u = q.u0; u < q.u1; ++u, ++g) {
                     const int s = g % S;
@@ -427,12 +435,12 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
                     const uint32_t st = smem + s * stage;
                     for (int t = 0; t < atoms; ++t) {
                         tma_2d(st + t * atom, &maps.w, u * 256 + t * 128, row0, &full[s]);
-                        if (!FEW)
+                        if constexpr (!FEW)
                             tma_2d(st + off_b + t * rows * 128, &maps.x[box], u * 256 + t * 128,
                                    tl.y, &full[s]);
                     }
                     tma_2d(st + off_sa, &maps.ws, u * 16, row0, &full[s]);
-                    if (!FEW) tma_2d(st + off_sb, &maps.xs[box], u * 16, tl.y, &full[s]);
+                    if constexpr (!FEW) tma_2d(st + off_sb, &maps.xs[box], u * 16, tl.y, &full[s]);
                 }
             }
             if (!ok) give_up();
@@ -449,7 +457,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i, ++n) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
-            const int rows = 16 << box_of(tl.z);
+            const int rows = 16 << box_of(a, tl);
             const int npad = (tl.z + 15) & ~15;
             const int acc = n & 1;
             ok = n < 2 || bar_wait_spin(&dempty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag);
@@ -494,7 +502,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args, const __grid_constan
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
-            const int rows = 16 << box_of(tl.z);
+            const int rows = 16 << box_of(a, tl);
             for (int u = q.u0; u < q.u1; ++u, ++g) {
                 const int s = g % S, b = g % kScales;
                 ok = bar_wait(&full[s], (uint32_t)(g / S) & 1u, abort_flag) &&
@@ -783,7 +791,8 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
 namespace {
 
 template <bool FEW, typename XT>
-cudaError_t launch_kernel(const ProductArgs &a, const Maps &maps, int sms, cudaStream_t stream) {
+cudaError_t launch_kernel(const ProductArgs &a, const MapsOf<FEW> &maps, int sms,
+                          cudaStream_t stream) {
     static std::atomic<bool> attr_done[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
@@ -799,7 +808,7 @@ cudaError_t launch_kernel(const ProductArgs &a, const Maps &maps, int sms, cudaS
     return cudaGetLastError();
 }
 
-cudaError_t encode_matrix(Maps &maps, const uint8_t *codes, const uint8_t *scales,
+cudaError_t encode_matrix(MatrixMaps &maps, const uint8_t *codes, const uint8_t *scales,
                           int64_t scale_stride, int64_t rows, int64_t width, int outs) {
     const uint64_t code_row = (uint64_t)width / 2, scale_row = (uint64_t)width / kMxBlock;
     const cudaError_t err =
@@ -831,9 +840,9 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     Maps maps;
     cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
                                     p.num_experts * p.out_features, p.width, a.outs);
-    // boxes up to the tile's rows; a lone matrix's tiles are full but the last
     const uint64_t code_row = (uint64_t)p.width / 2, scale_row = (uint64_t)p.width / kMxBlock;
     for (int i = 0; i < kBoxes && err == cudaSuccess && (16 << i) <= a.cap; ++i) {
+        if (!p.routed && (16 << i) != a.cap) continue;
         err = encode_rows(&maps.x[i], p.ws + p.L.codes, code_row, (uint64_t)p.pairs, code_row, 128,
                           16u << i, true);
         if (err == cudaSuccess)
@@ -887,7 +896,7 @@ cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
     const size_t item = p.x_dtype == IQK_F32 ? 4 : 2;
     a.spread = !p.sel && p.pairs > 4;
     a.wide = aligned(p.x, 16) && p.x_stride * (int64_t)item % 16 == 0;
-    Maps maps;
+    MatrixMaps maps;
     const cudaError_t err = encode_matrix(maps, p.codes, p.scales, p.scale_stride,
                                           p.num_experts * p.out_features, p.width, a.outs);
     if (err != cudaSuccess) return err;

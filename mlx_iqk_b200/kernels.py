@@ -564,8 +564,8 @@ def route(rows: torch.Tensor, mask, top_k: int, scoring: int, renormalize: bool,
     """``iqk_route`` over logits ``rows [tokens, experts]``: ``(indices, weights)``."""
     dev = rows.device
     tokens, experts = rows.shape
-    indices = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    indices = rows.new_empty((tokens, top_k), dtype=torch.int32)
+    weights = rows.new_empty((tokens, top_k), dtype=torch.float32)
     status = library().iqk_route(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         top_k, scoring, renormalize, scale, indices.data_ptr(), weights.data_ptr(),
@@ -586,12 +586,12 @@ def route_balanced(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
     segments = 1 if offsets is None else offsets.numel() - 1
     weights = None
     if indices is None:
-        indices = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+        indices = rows.new_empty((tokens, top_k), dtype=torch.int32)
+        weights = rows.new_empty((tokens, top_k), dtype=torch.float32)
     need = balance_workspace_bytes(tokens, experts, segments)
-    ws = torch.empty(need + 4 * segments * experts, dtype=torch.uint8, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    counts = torch.empty((segments, experts), dtype=torch.int32, device=dev)
+    ws = rows.new_empty(need + 4 * segments * experts, dtype=torch.uint8)
+    loss = rows.new_empty((), dtype=torch.float32)
+    counts = rows.new_empty((segments, experts), dtype=torch.int32)
     base = ws.data_ptr()
     status = library().iqk_route_balanced(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
@@ -612,7 +612,7 @@ def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
         grad_weights = grad_weights.to(torch.float32).contiguous()
     if grad_loss is not None:
         grad_loss = grad_loss.to(torch.float32).contiguous()
-    grad = torch.empty((tokens, experts), dtype=rows.dtype, device=rows.device)
+    grad = rows.new_empty((tokens, experts))
     status = library().iqk_route_backward(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         _ptr(offsets), 1 if offsets is None else offsets.numel() - 1, top_k, scoring, renormalize,
@@ -696,7 +696,7 @@ def mx_linear(x: torch.Tensor, rows: int, row_stride: int, codes: torch.Tensor,
         mx_few(x, rows, row_stride, None, rows, codes, scales, scale_stride, 1, out_features, y)
         return
     need = mx_workspace_bytes(rows, 1, width, out_features)
-    ws = torch.empty(need, dtype=torch.uint8, device=y.device)
+    ws = y.new_empty(need, dtype=torch.uint8)
     status = library().iqk_mx_linear(
         x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, codes.data_ptr(), scales.data_ptr(),
         scale_stride, out_features, width, y.data_ptr(), DTYPE_IDS[y.dtype], ws.data_ptr(), need,
@@ -717,7 +717,7 @@ def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
                    out_features, y)
             return
         need = mx_workspace_bytes(pairs, experts, width, out_features)
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=y.device)
+        workspace = y.new_empty(need, dtype=torch.uint8)
     status = library().iqk_mx_routed(
         x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, sel.data_ptr(), pairs,
         codes.data_ptr(), scales.data_ptr(), scale_stride, experts, out_features, width,

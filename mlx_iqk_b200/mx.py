@@ -61,8 +61,26 @@ def _rows(x, what="x"):
     return rows, count, step
 
 
-def _matrix(codes, scales, dims, device=None):
-    """Checks a matrix's two tensors; returns the byte stride of its scale rows."""
+def _matrix(codes, scales, dims, x=None):
+    """The byte stride of a matrix's scale rows; refuses what the kernels do not take."""
+    try:
+        shape, steps = scales.shape, scales.stride()
+        if codes.dtype is scales.dtype is torch.uint8 and len(shape) == dims \
+                and codes.get_device() == scales.get_device() >= 0 \
+                and (x is None or x.get_device() == codes.get_device()) \
+                and codes.is_contiguous() \
+                and codes.shape == shape[:-1] + (shape[-1] * (MX_BLOCK // 2),) \
+                and steps[-1] == 1 and shape[-2] > 1 and steps[-2] >= shape[-1] > 0 \
+                and (dims == 2 or steps[0] == steps[1] * shape[1]) \
+                and not (steps[-2] | codes.data_ptr() | scales.data_ptr()) % 16:
+            return steps[-2]
+    except (AttributeError, IndexError):
+        pass
+    return _check_matrix(codes, scales, dims, None if x is None else x.device)
+
+
+def _check_matrix(codes, scales, dims, device):
+    """Every check of :func:`_matrix` with its message, and the layouts off its fast path."""
     for t, name in ((codes, "codes"), (scales, "scales")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise IqkRuntimeError(f"{name} must be a tensor on the GPU")
@@ -100,15 +118,15 @@ def mx_aligned_scales(scales: torch.Tensor) -> torch.Tensor:
     """A copy of ``scales [..., rows, blocks]`` whose rows start on 16-byte boundaries."""
     if not isinstance(scales, torch.Tensor) or scales.dtype != torch.uint8 or scales.dim() < 1:
         raise IqkRuntimeError("scales must be a uint8 tensor")
-    out = _scale_rows(scales.shape[:-1], scales.shape[-1], scales.device)
+    out = _scale_rows(scales.shape[:-1], scales.shape[-1], scales)
     out.copy_(scales)
     return out
 
 
-def _scale_rows(lead, blocks, device) -> torch.Tensor:
+def _scale_rows(lead, blocks, like) -> torch.Tensor:
     pitch = (blocks + 15) // 16 * 16
-    t = torch.empty(tuple(lead) + (pitch,), dtype=torch.uint8, device=device)
-    return t if pitch == blocks else t[..., :blocks]
+    t = like.new_empty((*lead, pitch), dtype=torch.uint8)
+    return t if pitch == blocks else t.narrow(-1, 0, blocks)
 
 
 def mx_quantize(x):
@@ -120,8 +138,8 @@ def mx_quantize(x):
     byte 255: all of it reads NaN."""
     rows, count, step = _rows(x)
     *lead, width = x.shape
-    codes = torch.empty((*lead, width // 2), dtype=torch.uint8, device=x.device)
-    scales = _scale_rows(lead, width // MX_BLOCK, x.device)
+    codes = x.new_empty((*lead, width // 2), dtype=torch.uint8)
+    scales = _scale_rows(lead, width // MX_BLOCK, x)
     K.mx_quantize(rows, count, step, codes, scales, (width // MX_BLOCK + 15) // 16 * 16)
     return codes, scales
 
@@ -129,12 +147,13 @@ def mx_quantize(x):
 def mx_dequantize(codes, scales, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values ``[..., width]`` of an MXFP4 tensor: exact in float32, rounded once
     to float16 or bfloat16."""
-    stride = _matrix(codes, scales, 0)
+    two = isinstance(codes, torch.Tensor) and codes.dim() == 2
+    stride = _matrix(codes, scales, 2) if two else _check_matrix(codes, scales, 0, None)
     if dtype not in K.DTYPE_IDS:
         raise IqkRuntimeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     K.check_current(codes.device)
     *lead, half = codes.shape
-    out = torch.empty((*lead, half * 2), dtype=dtype, device=codes.device)
+    out = codes.new_empty((*lead, half * 2), dtype=dtype)
     K.mx_dequantize(codes, scales, stride, out)
     return out
 
@@ -150,12 +169,12 @@ def mx_linear(x, codes, scales, out_dtype: torch.dtype | None = None) -> torch.T
     """``q(x) W^T`` ``[..., out]`` for ``x [..., width]`` and ``W`` = ``codes [out,
     width / 2]``, ``scales [out, width / 32]``; ``q`` is :func:`mx_quantize`."""
     rows, count, step = _rows(x)
-    stride = _matrix(codes, scales, 2, x.device)
+    stride = _matrix(codes, scales, 2, x)
     out, half = codes.shape
     *lead, width = x.shape
     if half * 2 != width:
         raise IqkRuntimeError(f"x of width {width} meets a matrix of {half * 2}")
-    y = torch.empty((*lead, out), dtype=_out_dtype(x, out_dtype), device=x.device)
+    y = x.new_empty((*lead, out), dtype=_out_dtype(x, out_dtype))
     if count and out:
         K.mx_linear(rows, count, step, codes, scales, stride, y)
     return y
@@ -175,7 +194,7 @@ def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = 
     (uint8, ``kernels.mx_workspace_bytes``), read by
     ``kernels.mx_read_error``."""
     rows, count, step = _rows(x)
-    stride = _matrix(codes, scales, 3, x.device)
+    stride = _matrix(codes, scales, 3, x)
     if not isinstance(indices, torch.Tensor) or indices.device != x.device \
             or indices.dtype not in (torch.int32, torch.int64):
         raise IqkRuntimeError("indices must be an int32 or int64 tensor beside x")
@@ -188,7 +207,7 @@ def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = 
         raise IqkRuntimeError(
             f"{pairs} token-expert pairs do not tile {count} activation "
             f"row(s); the operand and the routing disagree")
-    y = torch.empty((*indices.shape, 1, out), dtype=_out_dtype(x, out_dtype), device=x.device)
+    y = x.new_empty((*indices.shape, 1, out), dtype=_out_dtype(x, out_dtype))
     if pairs and out:
         if experts == 0:
             return y.zero_()
@@ -211,10 +230,10 @@ class MxSwitchGLU(nn.Module):
             raise IqkRuntimeError(f"num_experts {num_experts} is not in 1 to 4096")
         self.num_experts, self.hidden, self.inter = num_experts, hidden, inter
         for name, (rows, width) in self._shapes().items():
-            self.register_buffer(f"{name}_codes", torch.zeros(
-                (num_experts, rows, width // 2), dtype=torch.uint8, device=device))
+            codes = torch.zeros((num_experts, rows, width // 2), dtype=torch.uint8, device=device)
+            self.register_buffer(f"{name}_codes", codes)
             self.register_buffer(f"{name}_scales", _scale_rows(
-                (num_experts, rows), width // MX_BLOCK, device).zero_())
+                (num_experts, rows), width // MX_BLOCK, codes).zero_())
 
     def _shapes(self):
         return {"gate": (self.inter, self.hidden), "up": (self.inter, self.hidden),
