@@ -219,7 +219,9 @@ class MxSwitchGLU(nn.Module):
     """One SwitchGLU layer of MXFP4 experts, ``(x, indices, scores)`` as
     ``IqkSwitchGLU``: gate and up ``[experts, inter, hidden]``, down ``[experts,
     hidden, inter]``, ``h = silu(gate) * up * score`` in float32, and each
-    token's sum over its experts."""
+    token's sum over its experts. The scores go in before the down projection's
+    quantisation of ``h``, whose scales they move with it (a power of two
+    exactly, another factor up to the rounding of a 4-bit value)."""
 
     def __init__(self, num_experts: int, hidden: int, inter: int, device=None):
         super().__init__()
@@ -255,27 +257,32 @@ class MxSwitchGLU(nn.Module):
         """Quantise and install one projection's float matrices ``[experts, rows, width]``."""
         self.load(name, *mx_quantize(weights))
 
-    def forward(self, x, indices, scores) -> torch.Tensor:
+    def forward(self, x, indices, scores=None) -> torch.Tensor:
         """``x [..., hidden]``, ``indices`` and ``scores [..., top_k]`` ->
-        ``[..., hidden]`` float32."""
+        ``[..., hidden]`` float32; with ``scores`` None each pair's own output,
+        ``[..., top_k, hidden]``. Index -1 contributes nothing."""
         lead, k = tuple(indices.shape[:-1]), indices.shape[-1]
-        if tuple(x.shape) != lead + (self.hidden,) or scores.shape != indices.shape:
+        if tuple(x.shape) != lead + (self.hidden,) or \
+                (scores is not None and scores.shape != indices.shape):
             raise IqkRuntimeError(
                 f"x {tuple(x.shape)}, indices {tuple(indices.shape)} and scores "
-                f"{tuple(scores.shape)} do not belong together")
+                f"{None if scores is None else tuple(scores.shape)} do not belong together")
         sel = indices.reshape(-1, k).to(torch.int32).contiguous()
         rows = x.reshape(-1, 1, 1, self.hidden)
-        out = torch.empty((rows.shape[0], self.hidden), dtype=torch.float32, device=x.device)
-        if not sel.numel():
-            return out.zero_().view(lead + (self.hidden,))
         f32 = torch.float32
+        if not sel.numel():
+            shape = lead + ((self.hidden,) if scores is not None else (k, self.hidden))
+            return torch.zeros(shape, dtype=f32, device=x.device)
         gate = mx_switch_linear(rows, sel, self.gate_codes, self.gate_scales, f32)
         up = mx_switch_linear(rows, sel, self.up_codes, self.up_scales, f32)
-        w = scores.reshape(-1).to(f32).contiguous()
+        w = None if scores is None else scores.detach().reshape(-1).to(f32).contiguous()
         h = torch.empty((sel.numel(), self.inter), dtype=f32, device=x.device)
         K.swiglu_rows(gate.view(-1, self.inter), up.view(-1, self.inter), w, h)
         y = mx_switch_linear(h.view(-1, k, 1, self.inter), sel, self.down_codes,
                              self.down_scales, f32)
+        if scores is None:
+            return y.view(lead + (k, self.hidden))
+        out = torch.empty((rows.shape[0], self.hidden), dtype=f32, device=x.device)
         K.pairs_combine(y, sel, k, self.num_experts, out)
         return out.view(lead + (self.hidden,))
 

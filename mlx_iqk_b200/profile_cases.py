@@ -4,11 +4,17 @@
     python -m mlx_iqk_b200.profile_cases grouped --member iq2_ks --tokens 2048
     python -m mlx_iqk_b200.profile_cases dequant --member iq2_ks [--experts 64]
     python -m mlx_iqk_b200.profile_cases layer   --tokens 2048
+    python -m mlx_iqk_b200.profile_cases mx      --tokens 2048 [--experts 256] [--width 4096]
+    python -m mlx_iqk_b200.profile_cases router  --tokens 16384
 
 ``layer`` is one config-5 MoE layer through ``ExpertParallelMoE`` on one GPU
 (gate/up IQ2_KS, down IQ2_K, top-6 of 256 experts): both preparations, the
 three grouped GEMMs, the SwiGLU and combine kernels, eager (the layer reads
 its index check on the host, so it is not captured in a graph).
+
+``mx`` is one routed MXFP4 projection (``--experts 1``: one matrix, every token
+through it); ``router`` the top-6 choice with the balance loss, forward and
+backward.
 
 Each case builds random relayout streams for 256 experts (the benchmark
 geometry: [2048, 4096] for gate-shaped, [4096, 2048] for down-shaped
@@ -119,7 +125,8 @@ def timed(fn, reps: int, graph: bool = False) -> float:
 
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=("gemv", "grouped", "dequant", "layer", "step", "dense"))
+    ap.add_argument("case", choices=("gemv", "grouped", "dequant", "layer", "step", "dense",
+                                     "mx", "router"))
     ap.add_argument("--member", default="iq2_ks")
     ap.add_argument("--batch", type=int, default=8, help="gemv: tokens (top-6 each)")
     ap.add_argument("--tokens", type=int, default=2048, help="grouped: tokens (top-6 each)")
@@ -157,6 +164,42 @@ def main() -> None:
         print(json.dumps({"case": "layer", "experts": E, "tokens": T, "pairs": P,
                           "us": round(ms * 1e3, 2), "tflops": round(flops / (ms * 1e-3) / 1e12, 1),
                           "tokens_per_s": round(T / (ms * 1e-3), 1)}))
+        return
+    if args.case == "mx":
+        from .mx import mx_linear, mx_quantize, mx_switch_linear
+        T, k = args.tokens, 1 if E == 1 else min(6, E)
+        codes = torch.randint(0, 256, (E, out, n // 2), generator=gen, device=dev,
+                              dtype=torch.uint8)
+        scales = mx_quantize(torch.randn((E, out, n), generator=gen, device=dev,
+                                         dtype=torch.bfloat16))[1]
+        x = torch.randn((T, 1, 1, n), generator=gen, device=dev).to(torch.bfloat16)
+        sel = torch.topk(torch.randn((T, E), generator=gen, device=dev), k).indices.int()
+        if E == 1:
+            ms = timed(lambda: mx_linear(x, codes[0], scales[0]), args.reps, args.graph)
+        else:
+            ms = timed(lambda: mx_switch_linear(x, sel, codes, scales), args.reps, args.graph)
+        nbytes = len(set(sel.reshape(-1).tolist())) * out * (n // 2 + n // 32)
+        flops = 2.0 * T * k * out * n
+        print(json.dumps({"case": "mx", "experts": E, "tokens": T, "out": out, "in": n,
+                          "us": round(ms * 1e3, 2), "bytes": nbytes,
+                          "GBps": round(nbytes / (ms * 1e-3) / 1e9, 1),
+                          "tflops": round(flops / (ms * 1e-3) / 1e12, 1)}))
+        return
+    if args.case == "router":
+        from .router import route_balanced
+        T = args.tokens
+        z = torch.randn((T, E), generator=gen, device=dev).to(torch.bfloat16).requires_grad_()
+        gw = torch.randn((T, 6), generator=gen, device=dev)
+        gl = torch.ones((), device=dev)
+
+        def one():
+            _, w, loss, _ = route_balanced(z, 6)
+            torch.autograd.grad([w, loss], [z], [gw, gl])
+
+        ms = timed(one, args.reps)
+        nbytes = 3 * T * E * 2 + T * 6 * 12
+        print(json.dumps({"case": "router", "experts": E, "tokens": T, "us": round(ms * 1e3, 2),
+                          "bytes": nbytes, "GBps": round(nbytes / (ms * 1e-3) / 1e9, 1)}))
         return
     if args.case == "dense":
         # the dense decode GEMV at the lm_head shape ([129280, 4096], --batch

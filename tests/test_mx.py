@@ -387,6 +387,36 @@ def test_layer_behind_the_router(cuda, t):
     assert np.linalg.norm(got - want) <= 5e-3 * np.linalg.norm(want)
 
 
+@pytest.mark.gpu
+def test_layer_without_scores(cuda):
+    g = torch.Generator().manual_seed(3)
+    layer = MxSwitchGLU(6, 64, 96, device="cuda")
+    for name, shape in (("gate", (6, 96, 64)), ("up", (6, 96, 64)), ("down", (6, 64, 96))):
+        layer.load_weights(name, torch.randn(shape, generator=g).cuda())
+    x = torch.randn((5, 2, 64), generator=g).cuda()
+    idx = torch.randint(-1, 6, (5, 2, 3), generator=g).cuda()
+    pairs = layer(x, idx)
+    assert pairs.shape == (5, 2, 3, 64)
+    assert (pairs[idx < 0] == 0).all()
+    # scores of 1 are no factor: the sum of the pairs, in the combine's order
+    whole = layer(x, idx, torch.ones(idx.shape, device="cuda"))
+    assert torch.equal(whole, pairs[:, :, 0] + pairs[:, :, 1] + pairs[:, :, 2])
+    assert layer(x[:0], idx[:0]).shape == (0, 2, 3, 64)
+    assert layer(x[:0], idx[:0], torch.ones((0, 2, 3), device="cuda")).shape == (0, 2, 64)
+
+
+@pytest.mark.gpu
+def test_example_trains_and_serves(cuda):
+    """The balance loss falls towards 1, and a decode step repeats the prefill's
+    row: the same products, whose float32 sums may be cut elsewhere, so that an
+    h near a tie can round to a neighbouring 4-bit value (as in the layer test)."""
+    from mlx_iqk_b200 import moe_example
+    seen = moe_example.run(experts=16, hidden=128, inter=64, tokens=200, top_k=2, steps=12)
+    assert float(seen["balance"][-1]) < float(seen["balance"][0])
+    got, want = seen["decode"], seen["prefill"][:4]
+    assert float((got - want).norm()) <= 5e-3 * float(want.norm())
+
+
 # ---------------------------------------------------------------- refusals
 
 
