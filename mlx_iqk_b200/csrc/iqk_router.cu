@@ -31,6 +31,8 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "iqk_common.cuh"
 #include "iqk_host.cuh"
 
@@ -67,39 +69,33 @@ __device__ __forceinline__ float ratio(float z, float c, int sigmoid) {
     return z >= 0.f ? 1.f / (1.f + expf(-z)) : expf(z - c) / (1.f + expf(z));
 }
 
+template <int V>
+__device__ __forceinline__ void ratios(const float (&z)[V], float c, int sigmoid, float (&r)[V]) {
+    if (sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = ratio(z[i], c, 1);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = expf(z[i] - c);
+    }
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
 
-// Order-preserving key of a logit: NaN above all numbers, -0 equal to +0,
-// -inf (no expert) and places past E are 0, below every number's key.
+// Order-preserving key of a logit. Adding +0 makes -0 equal to +0 and every NaN
+// the one whose key is above all numbers'; -inf (no expert, and places past E)
+// is the one value whose key is below kNone.
+constexpr uint32_t kNone = 0x00800000u;
 __device__ __forceinline__ uint32_t key_of(float z) {
-    if (z != z) return 0xffffffffu;
-    if (z == -CUDART_INF_F) return 0u;
     const uint32_t b = __float_as_uint(z + 0.f);
-    return (b >> 31) ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
-    if (key == 0xffffffffu) return CUDART_NAN_F;
     return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
-}
-
-// A 16-bit logit's ordered bits in the upper 22 of a word (the low ten are
-// free for the expert), and back.
-template <typename T> __device__ __forceinline__ uint32_t key16(float z, uint32_t key) {
-    if (sizeof(T) == 4) return key;
-    if (z != z) return 0xffff0000u;
-    const T v = from_float<T>(z + 0.f);
-    const uint32_t b = *reinterpret_cast<const uint16_t *>(&v);
-    return ((b >> 15) ? (~b & 0xffffu) : (b | 0x8000u)) << 16;
-}
-template <typename T> __device__ __forceinline__ float value16(uint32_t key) {
-    const uint32_t k = key >> 16;
-    if (sizeof(T) == 4 || k == 0xffffu) return CUDART_NAN_F;
-    const uint16_t b = (uint16_t)((k >> 15) ? k & 0x7fffu : ~k);
-    return to_float<T>(*reinterpret_cast<const T *>(&b));
 }
 
 // The segment of row t and the row after that segment's end: the largest g
@@ -146,27 +142,76 @@ __device__ __forceinline__ void load_row(const RouteArgs &a, int64_t t, int lane
     }
 }
 
+// The key of the row's largest logit; below kNone where the row has no expert.
 template <int V> __device__ __forceinline__ uint32_t row_peak(const float (&z)[V]) {
-    uint32_t best = 0;
+    float best = z[0];
 #pragma unroll
-    for (int i = 0; i < V; ++i) best = max(best, key_of(z[i]));
-    return __reduce_max_sync(kFull, best);
+    for (int i = 1; i < V; ++i)  // NaN wins, as in the keys
+        asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(best) : "f"(z[i]));
+    return __reduce_max_sync(kFull, key_of(best));
 }
 
-// The top_k largest of the row: lane j gets choice j (index -1 past the last).
-// 16-bit logits have 16-bit keys: key and 1023 - expert share a word, and one
-// warp maximum finds the largest and, among equals, the first. 32-bit keys take
-// a second one for the expert.
+// Lane j gets choice j of the top_k largest (index -1 past the last).
+//
+// A 16-bit logit fills the upper 22 bits of its f32 key at most, and 1023 -
+// expert the ten below: one warp maximum finds the largest and, among equals,
+// the first. With up to eight values a lane, each lane sorts its own first (19
+// exchanges); then a choice is the maximum of the lanes' heads, and the lane
+// that held it moves up its list: 14 instructions a choice for the 35 of a
+// search through unsorted values.
+template <typename T, int V, int N> struct Sorted {
+    uint32_t key[V];
+    __device__ __forceinline__ explicit Sorted(const float (&z)[V], int lane) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            key[i] = (key_of(z[i]) & ~1023u) | (1023u - expert_of<N>(lane, i));
+        // odd-even merge sort, falling
+#pragma unroll
+        for (int p = 1; p < V; p *= 2)
+#pragma unroll
+            for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+                for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+                    for (int i = 0; i < k; ++i)
+                        if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                            const uint32_t a = key[i + j], b = key[i + j + k];
+                            key[i + j] = max(a, b);
+                            key[i + j + k] = min(a, b);
+                        }
+    }
+    __device__ __forceinline__ uint32_t peak() const { return __reduce_max_sync(kFull, key[0]); }
+    // the low bits of a negative value's key are the ones of a zero
+    __device__ __forceinline__ static float logit(uint32_t top) {
+        return value_of((top & ~1023u) | ((top >> 31) ? 0u : 1023u));
+    }
+    __device__ __forceinline__ void choose(const RouteArgs &a, int lane, uint32_t top, int &index,
+                                           float &value) {
+        index = -1;
+        value = -CUDART_INF_F;
+        for (int j = 0; top >= kNone; top = peak()) {
+            if (lane == j) {
+                index = 1023 - (int)(top & 1023u);
+                value = logit(top);
+            }
+            if (++j == a.top_k) break;
+            if (key[0] == top) {
+#pragma unroll
+                for (int i = 0; i + 1 < V; ++i) key[i] = key[i + 1];
+                key[V - 1] = 0;
+            }
+        }
+    }
+};
+
+// Unsorted: 32-bit keys, whose expert takes a second warp maximum, and rows of
+// more than eight values a lane, where a sort costs more than it saves.
 template <typename T, int V, int N>
 __device__ __forceinline__ void choose(const RouteArgs &a, const float (&z)[V], int lane,
                                        int &index, float &value) {
-    constexpr bool kPacked = sizeof(T) == 2;
     uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        key[i] = key_of(z[i]);
-        if (kPacked && key[i]) key[i] = key16<T>(z[i], key[i]) | (1023u - expert_of<N>(lane, i));
-    }
+    for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
     index = -1;
     value = -CUDART_INF_F;
     for (int j = 0; j < a.top_k; ++j) {
@@ -174,29 +219,25 @@ __device__ __forceinline__ void choose(const RouteArgs &a, const float (&z)[V], 
 #pragma unroll
         for (int i = 0; i < V; ++i) best = max(best, key[i]);
         const uint32_t top = __reduce_max_sync(kFull, best);
-        if (top == 0) break;
-        int first;
-        if (kPacked) {
-            first = 1023 - (int)(top & 1023u);
+        if (top < kNone) break;
+        int first = kMaxExperts;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (key[i] == top) key[i] = 0;
-        } else {
-            first = kMaxExperts;
+        for (int i = V - 1; i >= 0; --i)
+            if (key[i] == top) first = expert_of<N>(lane, i);
+        first = __reduce_min_sync(kFull, first);
 #pragma unroll
-            for (int i = V - 1; i >= 0; --i)
-                if (key[i] == top) first = expert_of<N>(lane, i);
-            first = __reduce_min_sync(kFull, first);
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (first == expert_of<N>(lane, i)) key[i] = 0;
-        }
+        for (int i = 0; i < V; ++i)
+            if (first == expert_of<N>(lane, i)) key[i] = 0;
         if (lane == j) {
             index = first;
-            value = kPacked ? value16<T>(top) : value_of(top);
+            value = value_of(top);
         }
     }
 }
+
+struct Nothing {
+    template <typename Z> __device__ __forceinline__ Nothing(const Z &, int) {}
+};
 
 template <typename T, int V, int N, bool CHOOSE, bool BALANCE>
 __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lane,
@@ -211,22 +252,25 @@ __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lan
     }
     float z[V];
     load_row<T, V, N>(a, t, lane, z);
-    const uint32_t peak = row_peak<V>(z);
-    const float top = value_of(peak);
+    constexpr bool kSort = CHOOSE && sizeof(T) == 2 && V <= 8;
+    typename std::conditional<kSort, Sorted<T, V, N>, Nothing>::type sorted(z, lane);
+    uint32_t peak;
+    if constexpr (kSort) peak = sorted.peak();
+    else peak = row_peak<V>(z);
+    const float top = kSort ? Sorted<T, V, N>::logit(peak) : value_of(peak);
     const float c = a.sigmoid ? fminf(top, 0.f) : top;
     float total = 1.f;
     if (BALANCE || (CHOOSE && !a.renormalize && !a.sigmoid)) {
         float part = 0.f;
+        ratios<V>(z, c, a.sigmoid, score);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            score[i] = ratio(z[i], c, a.sigmoid);
-            part += score[i];
-        }
+        for (int i = 0; i < V; ++i) part += score[i];
         total = warp_sum(part);
     }
     if (CHOOSE) {
         float value, w;
-        choose<T, V, N>(a, z, lane, index, value);
+        if constexpr (kSort) sorted.choose(a, lane, peak, index, value);
+        else choose<T, V, N>(a, z, lane, index, value);
         if (a.renormalize) {
             const float r = index >= 0 ? ratio(value, c, a.sigmoid) : 0.f;
             w = r / warp_sum(r);
@@ -245,7 +289,7 @@ __device__ __forceinline__ bool route_row(const RouteArgs &a, int64_t t, int lan
 #pragma unroll
         for (int i = 0; i < V; ++i) score[i] *= inv;
     }
-    return peak != 0;
+    return peak >= kNone;
 }
 
 // A warp a row.
@@ -342,12 +386,17 @@ __global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(32 * kFini
 balance_finish_kernel(RouteArgs a, float *loss, int32_t *counts, float *slope) {
     __shared__ float scores[kFinishWarps][32], part_sum[kFinishWarps], total;
     __shared__ int32_t picked[kFinishWarps][32];
-    __shared__ int filled;
+    constexpr int kKept = 256;
+    __shared__ int filled, kept[kKept];  // rows of the first segments
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) filled = 0;
     __syncthreads();
     int mine = 0;
-    for (int g = warp; g < a.segments; g += kFinishWarps) mine += rows_of(a, g, lane) > 0;
+    for (int g = warp; g < a.segments; g += kFinishWarps) {
+        const int n = rows_of(a, g, lane);
+        if (lane == 0 && g < kKept) kept[g] = n;
+        mine += n > 0;
+    }
     if (lane == 0 && mine) atomicAdd(&filled, mine);
     __syncthreads();
     const float mean = 1.f / (float)max(filled, 1);
@@ -358,7 +407,8 @@ balance_finish_kernel(RouteArgs a, float *loss, int32_t *counts, float *slope) {
     for (int g0 = 0; g0 < a.segments; g0 += kFinishWarps / share) {
         const int g = g0 + warp / share;
         int first = 0, last = -1, n = 0;
-        if (g < a.segments && blocks_of(a, g, first, last)) n = rows_of(a, g, lane);
+        if (g < a.segments && blocks_of(a, g, first, last))
+            n = g < kKept ? kept[g] : rows_of(a, g, lane);
         const float inv = n > 0 ? 1.f / (float)n : 0.f;
         for (int e0 = blockIdx.x * 32; e0 < a.experts; e0 += kFinishCtas * 32) {
             const int e = e0 + lane;
@@ -450,7 +500,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, RouteG
             }
         }
         const uint32_t peak = keep ? row_peak<V>(z) : 0u;
-        if (peak == 0) {  // no expert: nothing depends on this row
+        if (peak < kNone) {  // no expert: nothing depends on this row
 #pragma unroll
             for (int i = 0; i < V; ++i) dz[i] = 0.f;
         } else {
@@ -459,11 +509,9 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, RouteG
             float inv = 1.f;
             if (there || softmax_all) {
                 float part = 0.f;
+                ratios<V>(z, c, a.sigmoid, dz);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dz[i] = ratio(z[i], c, a.sigmoid);
-                    part += dz[i];
-                }
+                for (int i = 0; i < V; ++i) part += dz[i];
                 inv = 1.f / warp_sum(part);
             }
             // the choice's part: lane j adds `own` at its expert, and every
@@ -498,13 +546,13 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, RouteG
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float v = 0.f;
-                if (there) {
-                    const float h = a.sigmoid ? logistic(-z[i]) : 1.f;
-                    v = dz[i] * inv * h * (slope[i] - dot);
-                }
-                if (softmax_all) v -= dz[i] * inv * shared;
-                dz[i] = v;
+                const float s = dz[i] * inv;
+                const float v = there ? s * (slope[i] - dot) : 0.f;
+                dz[i] = softmax_all ? v - s * shared : v;
+            }
+            if (a.sigmoid && there) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) dz[i] *= logistic(-z[i]);
             }
             if (d.weights) {
 #pragma unroll

@@ -32,6 +32,16 @@ MAX_TOP_K = 32
 _SCORING = {"softmax": 0, "sigmoid": 1}
 
 
+def _rows(logits):
+    """``logits`` as ``[tokens, experts]`` rows whose columns are adjacent."""
+    experts = logits.shape[-1]
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, experts)
+    step, inner = rows.stride()
+    if inner != 1 or (step < experts and rows.shape[0] > 1):
+        rows = rows.contiguous()
+    return rows
+
+
 def _check(logits, top_k, scoring, mask, offsets=None):
     """The call's logits as ``[tokens, experts]`` rows, its mask, offsets and scoring id."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
@@ -49,9 +59,7 @@ def _check(logits, top_k, scoring, mask, offsets=None):
         raise IqkRuntimeError(f"scoring must be one of {sorted(_SCORING)}, got {scoring!r}")
     dev = logits.device
     K.check_current(dev)
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, experts)
-    if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < experts):
-        rows = rows.contiguous()
+    rows = _rows(logits)
     if mask is not None:
         if mask.dtype != torch.bool or mask.device != dev:
             raise IqkRuntimeError("mask must be a bool tensor beside the logits")
@@ -87,8 +95,6 @@ class _Route(torch.autograd.Function):
             ctx.mark_non_differentiable(indices)
         ctx.call = call
         ctx.save_for_backward(logits, indices, mask, offsets)
-        # rows is logits itself, or the copy that made its columns adjacent
-        ctx.rows = None if rows is logits else rows
         return (indices if choose else None), weights, loss, counts
 
     @staticmethod
@@ -103,8 +109,8 @@ class _Route(torch.autograd.Function):
         slope = None if grad_loss is None else ctx.slope
         if grad_weights is None and slope is None:
             return None, None, None, None
-        grad = K.route_backward(logits if ctx.rows is None else ctx.rows, mask, offsets,
-                                *ctx.call, indices, grad_weights, slope, grad_loss)
+        grad = K.route_backward(_rows(logits), mask, offsets, *ctx.call, indices, grad_weights,
+                                slope, grad_loss)
         return grad if logits.dim() == 2 else grad.view(logits.shape), None, None, None
 
 

@@ -355,6 +355,28 @@ def test_one_gradient_alone_broadcast_gradients_and_no_second_derivative(cuda):
 
 
 @pytest.mark.gpu
+def test_gradient_of_other_layouts_and_changed_logits(cuda):
+    z = make(24, 16, torch.float32, seed=3)
+    gw = torch.randn((24, 2), generator=torch.Generator().manual_seed(1)).cuda()
+
+    def grad(x, view):
+        idx, w = route(view(x), 2, renormalize=False)
+        return torch.autograd.grad(w.reshape(24, 2), [x], gw)[0]
+
+    want = grad(z.clone().requires_grad_(), lambda x: x)
+    assert torch.equal(grad(z.clone().requires_grad_(), lambda x: x.view(2, 3, 4, 16)), want)
+    t = z.t().contiguous().requires_grad_()    # columns not adjacent
+    assert torch.equal(grad(t, lambda x: x.t()).t(), want)
+    for shape in ((24, 16), (4, 6, 16)):       # logits written over before their gradient
+        x = z.clone().view(shape)
+        y = x.requires_grad_() * 1.0
+        _, w = route(y, 2)
+        y.add_(1.0)
+        with pytest.raises(RuntimeError):
+            w.sum().backward()
+
+
+@pytest.mark.gpu
 def test_on_a_side_stream(cuda):
     z = make(3000, 256, torch.bfloat16, seed=6)
     want = route_balanced(z, 6)
