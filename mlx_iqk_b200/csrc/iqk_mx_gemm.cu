@@ -10,12 +10,14 @@
 // (up to 128 rows), so a call with one token moves the matrix once and wastes
 // only tensor-core columns that are idle anyway.
 //
-// Persistent, one CTA an SM, 12 warps:
-//   warp 0      TMA producer: per unit of 512 columns the codes of 128 outputs
-//               (two 128-byte-swizzle atoms) and of the tile's rows, and both
-//               sides' scales (16 bytes a row)
-//   warp 1      MMA issuer: eight K = 64 steps a unit
-//   warp 2      tensor memory
+// Persistent, one CTA an SM, 16 warps; a unit is 512 columns, a stage half of it:
+//   warp 0      TMA producer: per stage the codes of 128 outputs and of the
+//               tile's rows, a 128-byte-swizzle atom each
+//   warp 1      MMA issuer: four K = 64 steps a stage
+//   warp 2      tensor memory; zeros to rows of pairs without an expert
+//   warp 3      TMA of both sides' scales, 16 bytes a row and unit, on a ring of
+//               their own: they run ahead of the codes, so that a unit's scales
+//               are in tensor memory before its codes have come
 //   warps 4-7   scale movers: the MMA reads scales from tensor memory, word
 //               (row mod 32, row / 32) of each 128 columns, the same in all
 //               four lane quarters; a row's 16 scale bytes are four such
@@ -23,13 +25,17 @@
 //               columns
 //   warps 8-11  epilogue: tcgen05.ld, y stored (a warp's lanes are 32
 //               consecutive outputs of one row)
-//   warps 12-15 (few rows only) activations: the rows' 512 columns read from x,
+//   warps 12-15 the second half of the tile's rows in the epilogue. Few rows:
+//               activations instead: the rows' 512 columns read from x,
 //               rounded and written where TMA would have put them, so that
 //               such a call is one launch; each CTA also sorts its (at most
 //               64) pairs by itself. With up to 4 rows a tile each warp takes
 //               every fourth unit, so that four units' loads are under way
 //               (8 tokens' down projection 52 -> 39 us); with more, the warps
 //               share each unit (37 rows 14.2 -> 12 us)
+// Whole 512-column stages with their scales, of which three fit, made each
+// stage wait for its own load, move and products: 4096 x 4096 x 8192 95 us,
+// now 83.
 // Accumulators are double-buffered, scale buffers four deep.
 //
 // Work: item = (128 outputs, tile of rows); a call of few items takes 64 or 32
@@ -60,34 +66,35 @@ namespace {
 
 using namespace dev;
 
-constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kSortWarp = 3, kMover0 = 4, kEpi0 = 8,
+constexpr int kThreads = 512;
+constexpr int kProducer = 0, kIssuer = 1, kTmemWarp = 2, kScaleWarp = 3, kMover0 = 4, kEpi0 = 8,
               kRound0 = 12;
-__host__ __device__ constexpr int threads_of(bool few) { return few ? 512 : 384; }
 constexpr int kOuts = 128;              // outputs of an item at most (the MMA's M)
-constexpr int kUnit = 512;              // columns of a pipeline stage
-constexpr int kScales = 4;              // scale buffers in tensor memory
+constexpr int kUnit = 512;              // columns of a 16-byte row of scales
+constexpr int kStageK = 256;            // columns of a stage: one swizzle atom a side
+constexpr int kScales = 4;              // scale slots, in shared and in tensor memory
 constexpr int kBoxes = 4;               // row boxes: 16, 32, 64, 128
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 24;
 constexpr int kSmemCap = 227 * 1024;
-constexpr int kBarBytes = 384;
+constexpr int kBarBytes = 640;
 constexpr int kFewCap = 16, kFewPairs = 64;          // one launch: rows of a tile, routed pairs
 constexpr int kFewTable = kFewPairs * (16 + 2 * 4 * kFewCap);  // tiles; pairs, rows of x
 constexpr int kMaxCtas = 148;
 constexpr uint32_t kSaved = 14;
 
-// Shared memory of a stage: codes of the matrix and of the rows (two swizzle
-// atoms of 256 columns each), scales; in whole kilobytes, as the swizzle is.
-__host__ __device__ constexpr int stage_bytes(int cap, int outs) {
-    return (2 * (outs + cap) * 128 + (outs + cap) * 16 + 1023) / 1024 * 1024;
+// Shared memory: stages (codes of the outputs and of the rows), scale slots.
+__host__ __device__ constexpr int stage_bytes(int cap, int outs) { return (outs + cap) * 128; }
+__host__ __device__ constexpr int slot_bytes(int cap, int outs) { return (outs + cap) * 16; }
+// The MMA reads 128 outputs of a stage whatever an item has: what follows the
+// last stage must be shared memory too.
+__host__ __device__ constexpr int spare_bytes(int cap, int outs) {
+    return kOuts * 128 > stage_bytes(cap, outs) ? kOuts * 128 - stage_bytes(cap, outs) : 0;
 }
-// The MMA reads 128 outputs of an atom whatever an item has: what follows an
-// atom must be shared memory too.
-__host__ __device__ constexpr int spare_bytes(int outs) { return (kOuts - outs) * 128; }
-__host__ __device__ constexpr int smem_fixed(int outs) {
-    return 1024 + kBarBytes + kFewTable + spare_bytes(outs);
+__host__ __device__ constexpr int smem_fixed(int cap, int outs) {
+    return 1024 + kBarBytes + kFewTable + spare_bytes(cap, outs) + kScales * slot_bytes(cap, outs);
 }
 __host__ __device__ constexpr int stages_for(int cap, int outs) {
-    const int n = (kSmemCap - smem_fixed(outs)) / stage_bytes(cap, outs);
+    const int n = (kSmemCap - smem_fixed(cap, outs)) / stage_bytes(cap, outs);
     return n < kMaxStages ? n : kMaxStages;
 }
 
@@ -97,7 +104,7 @@ struct ProductArgs {
     int32_t *hdr;
     const int32_t *order;  // null: one matrix, row p is pair p
     const int4 *tiles;
-    int32_t *tickets;      // four per shared item, one for 32 outputs
+    int32_t *tickets;      // per shared item: 32 outputs x half of the rows
     float *slots;          // [ctas, 2, cap, 128]
     void *y;
     int y_dtype;
@@ -186,6 +193,25 @@ __device__ __forceinline__ int box_of(const ProductArgs &a, const int4 &tile) {
     const int rows = a.tiles ? tile.z : a.cap;
     return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
 }
+
+// The stages of a part: [first, last) of the item's width / 256. The last
+// unit's second half may lie past the width.
+__device__ __forceinline__ int first_stage(const Part &q) { return 2 * q.u0; }
+__device__ __forceinline__ int last_stage(const Part &q, int stages) {
+    return min(2 * q.u1, stages);
+}
+
+// A place in a ring of stages or scale slots.
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++s == stages) {
+            s = 0;
+            phase ^= 1u;
+        }
+    }
+};
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -334,7 +360,7 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, const float 
 
 // FEW: activations of type XT, rounded in the kernel; else from the workspace.
 template <bool FEW, typename XT>
-__global__ void __launch_bounds__(threads_of(FEW), 1)
+__global__ void __launch_bounds__(kThreads, 1)
 mx_product_kernel(const __grid_constant__ ProductArgs args,
                   const __grid_constant__ MapsOf<FEW> maps) {
     ProductArgs a = args;
@@ -344,10 +370,12 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     const uint32_t smem = (raw + 1023u) & ~1023u;
     const int S = a.stages, cap = a.cap;
     const uint32_t stage = (uint32_t)stage_bytes(cap, a.outs);
-    char *bars = smem_raw + (smem - raw) + S * stage;
+    const uint32_t slots = smem + S * stage, slot = (uint32_t)slot_bytes(cap, a.outs);
+    char *bars = smem_raw + (smem - raw) + S * stage + kScales * slot;
     uint64_t *full = reinterpret_cast<uint64_t *>(bars);
     uint64_t *empty = full + kMaxStages;
-    uint64_t *sready = empty + kMaxStages, *sfree = sready + kScales;
+    uint64_t *sfull = empty + kMaxStages, *sempty = sfull + kScales;
+    uint64_t *sready = sempty + kScales, *sfree = sready + kScales;
     uint64_t *dfull = sfree + kScales, *dempty = dfull + 2, *drain = dempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
@@ -363,12 +391,14 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             bar_init(&empty[i], 1);
         }
         for (int i = 0; i < kScales; ++i) {
+            bar_init(&sfull[i], !FEW ? 1 : a.spread ? 5 : 2);
+            bar_init(&sempty[i], 4);
             bar_init(&sready[i], 4);
             bar_init(&sfree[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(&dfull[i], 1);
-            bar_init(&dempty[i], 4);
+            bar_init(&dempty[i], FEW ? 4 : 8);
         }
         bar_init(drain, 1);
         *abort_flag = 0;
@@ -384,7 +414,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         tc_fence_before();
     }
     if (FEW && a.sel) {
-        if (warp == kSortWarp) {
+        if (warp == kScaleWarp) {
             bool bad;
             const int n = sort_few(a, lane, few_tiles, few_pairs, few_rows, bad);
             if (lane == 0) {
@@ -409,10 +439,42 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             atomicOr(a.hdr + 3, IQK_DEVERR_TIMEOUT);
         }
     };
-    const uint32_t atom = (uint32_t)a.outs * 128;
-    const uint32_t off_b = 2 * atom, off_sa = off_b + 2 * cap * 128, off_sb = off_sa + a.outs * 16;
+    const uint32_t off_b = (uint32_t)a.outs * 128, off_sb = (uint32_t)a.outs * 16;
+    const int width = (int)a.width, item_stages = (width + kStageK - 1) / kStageK;
 
     if (warp == kProducer) {
+        if (lane == 0) {
+            int g = 0;
+            Ring ring;
+            bool ok = true;
+            Part q;
+            for (uint32_t i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
+                int out0;
+                const int4 tl = tile_of(a, plan, q.item, out0);
+                const int box = box_of(a, tl);
+                // few rows: written by the rounding warps
+                const uint32_t bytes = (uint32_t)(128 * (a.outs + (FEW ? 0 : 16 << box)));
+                const int row0 = (int)((int64_t)tl.x * a.out_features + out0);
+                for (int t = first_stage(q); t < last_stage(q, item_stages); ++t, ++g, ring.next(S)) {
+                    if (!bar_wait_poll(&empty[ring.s], ring.phase ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    bar_expect_tx(&full[ring.s], bytes);
+                    const uint32_t st = smem + ring.s * stage;
+                    tma_2d(st, &maps.w, t * 128, row0, &full[ring.s]);
+                    if constexpr (!FEW)
+                        tma_2d(st + off_b, &maps.x[box], t * 128, tl.y, &full[ring.s]);
+                }
+            }
+            if (!ok) give_up();
+            for (int d = 0; d < S && d < g; ++d) {  // every copy lands before the CTA exits
+                const int gg = g - 1 - d;
+                if (!bar_wait_poll(&full[gg % S], (uint32_t)(gg / S) & 1u, nullptr)) give_up();
+            }
+        }
+        __syncwarp();
+    } else if (warp == kScaleWarp) {
         if (lane == 0) {
             int g = 0;
             bool ok = true;
@@ -420,79 +482,97 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             for (uint32_t i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
                 int out0;
                 const int4 tl = tile_of(a, plan, q.item, out0);
-                const int box = box_of(a, tl), rows = 16 << box;
+                const int box = box_of(a, tl);
+                const uint32_t bytes = (uint32_t)(16 * (a.outs + (FEW ? 0 : 16 << box)));
                 const int row0 = (int)((int64_t)tl.x * a.out_features + out0);
                 for (int u = q.u0; u < q.u1; ++u, ++g) {
-                    const int s = g % S;
-                    if (!bar_wait(&empty[s], ((uint32_t)(g / S) & 1u) ^ 1u, abort_flag)) {
+                    const int b = g % kScales;
+                    if (!bar_wait_poll(&sempty[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag)) {
                         ok = false;
                         break;
                     }
-                    // the second half of the last unit may lie past the width
-                    const int atoms = (int)min((int64_t)2, (a.width - (int64_t)u * kUnit + 255) / 256);
-                    const int xrows = FEW ? 0 : rows;  // few rows: written by the rounding warps
-                    bar_expect_tx(&full[s], (uint32_t)((atoms * 128 + 16) * (a.outs + xrows)));
-                    const uint32_t st = smem + s * stage;
-                    for (int t = 0; t < atoms; ++t) {
-                        tma_2d(st + t * atom, &maps.w, u * 256 + t * 128, row0, &full[s]);
-                        if constexpr (!FEW)
-                            tma_2d(st + off_b + t * rows * 128, &maps.x[box], u * 256 + t * 128,
-                                   tl.y, &full[s]);
-                    }
-                    tma_2d(st + off_sa, &maps.ws, u * 16, row0, &full[s]);
-                    if constexpr (!FEW) tma_2d(st + off_sb, &maps.xs[box], u * 16, tl.y, &full[s]);
+                    bar_expect_tx(&sfull[b], bytes);
+                    tma_2d(slots + b * slot, &maps.ws, u * 16, row0, &sfull[b]);
+                    if constexpr (!FEW)
+                        tma_2d(slots + b * slot + off_sb, &maps.xs[box], u * 16, tl.y, &sfull[b]);
                 }
             }
             if (!ok) give_up();
-            for (int d = 0; d < S && d < g; ++d) {  // every copy lands before the CTA exits
+            for (int d = 0; d < kScales && d < g; ++d) {
                 const int gg = g - 1 - d;
-                if (!bar_wait(&full[gg % S], (uint32_t)(gg / S) & 1u, nullptr)) give_up();
+                if (!bar_wait_poll(&sfull[gg % kScales], (uint32_t)(gg / kScales) & 1u, nullptr)) give_up();
             }
         }
         __syncwarp();
     } else if (warp == kIssuer) {
-        int g = 0, n = 0;
+        // One warp's dependent instructions bound this loop, so it is bare: the
+        // issuing lane is elected once, a unit's two stages are taken together,
+        // and a product's operands are adds to theirs.
+        const bool leader = elect_one();
+        const int last_steps = (width - (item_stages - 1) * kStageK + 63) / 64;
+        const uint64_t desc0 = sw128_desc(smem);
+        const uint32_t desc_stage = stage >> 4, desc_b = off_b >> 4;
+        int n = 0;
+        Ring ring, slot_ring;
         bool ok = true;
         Part q;
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i, ++n) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
-            const int rows = 16 << box_of(a, tl);
             const int npad = (tl.z + 15) & ~15;
+            const uint32_t even = idesc_mxf4(kOuts, npad, 0), odd = idesc_mxf4(kOuts, npad, 2);
             const int acc = n & 1;
-            ok = n < 2 || bar_wait_spin(&dempty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            for (int u = q.u0; u < q.u1; ++u, ++g) {
-                const int s = g % S, b = g % kScales;
-                ok = bar_wait_spin(&full[s], (uint32_t)(g / S) & 1u, abort_flag) &&
-                     bar_wait_spin(&sready[b], (uint32_t)(g / kScales) & 1u, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);  // elect.sync needs the warp converged
+            const uint32_t d = tmem + acc * cap;
+            if (n >= 2)
+                ok = bar_wait_poll(&dempty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag);
+            for (int u = q.u0; u < q.u1; ++u, slot_ring.next(kScales)) {
+                const int b = slot_ring.s, left = item_stages - 2 * u;  // stages from here
+                const Ring lo = ring;
+                ring.next(S);
+                const Ring hi = left > 1 ? ring : lo;
+                if (left > 1) ring.next(S);
+                ok = ok && bar_wait_poll(&sready[b], slot_ring.phase, abort_flag) &&
+                     bar_wait_poll(&full[lo.s], lo.phase, abort_flag) &&
+                     bar_wait_poll(&full[hi.s], hi.phase, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const int steps = (int)min((int64_t)8, (a.width - (int64_t)u * kUnit + 63) / 64);
-                if (elect_one()) {
-                    const uint32_t st = smem + s * stage;
+                if (leader) {
+                    // a step is 32 bytes of each operand: 2 in a descriptor's 16-byte units
+                    const uint64_t da = desc0 + lo.s * desc_stage, db = da + desc_b;
+                    const uint64_t ea = desc0 + hi.s * desc_stage, eb = ea + desc_b;
                     const uint32_t sa = scale_col + b * 32, sb = sa + 16;
-                    for (int k = 0; k < steps; ++k) {
-                        const uint32_t in = (uint32_t)(k & 3) * 32;
-                        tc_mma_mxf4(tmem + acc * cap, sw128_desc(st + (k >> 2) * atom + in),
-                                    sw128_desc(st + off_b + (k >> 2) * rows * 128 + in),
-                                    idesc_mxf4(kOuts, npad, (k & 1) * 2), sa + (k >> 1) * 4,
-                                    sb + (k >> 1) * 4, (u > q.u0 || k > 0) ? 1u : 0u);
+                    const uint32_t more = u > q.u0 ? 1u : 0u;
+                    if (left > 2 || (left == 2 && last_steps == 4)) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_mxf4(d, da + 2 * k, db + 2 * k, k & 1 ? odd : even,
+                                        sa + (k >> 1) * 4, sb + (k >> 1) * 4, k ? 1u : more);
+                        tc_commit(&empty[lo.s]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_mxf4(d, ea + 2 * k, eb + 2 * k, k & 1 ? odd : even,
+                                        sa + 8 + (k >> 1) * 4, sb + 8 + (k >> 1) * 4, 1u);
+                        tc_commit(&empty[hi.s]);
+                    } else {
+                        const int steps = (left - 1) * 4 + last_steps;
+                        for (int k = 0; k < steps; ++k) {
+                            const uint64_t ka = k < 4 ? da + 2 * k : ea + 2 * (k - 4);
+                            tc_mma_mxf4(d, ka, ka + desc_b, k & 1 ? odd : even,
+                                        sa + (k >> 1) * 4, sb + (k >> 1) * 4, k ? 1u : more);
+                        }
+                        tc_commit(&empty[lo.s]);
+                        if (left > 1) tc_commit(&empty[hi.s]);
                     }
-                    tc_commit(&empty[s]);
                     tc_commit(&sfree[b]);
+                    if (u + 1 == q.u1) tc_commit(&dfull[acc]);
                 }
-                __syncwarp();
             }
-            if (!ok) break;
-            if (elect_one()) tc_commit(&dfull[acc]);
-            __syncwarp();
+            ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok && lane == 0) give_up();
         __syncwarp();
-        if (elect_one()) tc_commit(drain);  // every MMA ends before tensor memory is freed
+        if (leader) tc_commit(drain);  // every MMA ends before tensor memory is freed
         __syncwarp();
     } else if (warp >= kMover0 && warp < kMover0 + 4) {
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
@@ -504,21 +584,21 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int rows = 16 << box_of(a, tl);
             for (int u = q.u0; u < q.u1; ++u, ++g) {
-                const int s = g % S, b = g % kScales;
-                ok = bar_wait(&full[s], (uint32_t)(g / S) & 1u, abort_flag) &&
-                     (g < kScales ||
-                      bar_wait(&sfree[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag));
+                const int b = g % kScales;
+                const uint32_t phase = (uint32_t)(g / kScales) & 1u;
+                ok = bar_wait_poll(&sfull[b], phase, abort_flag) &&
+                     (g < kScales || bar_wait_poll(&sfree[b], phase ^ 1u, abort_flag));
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t st = smem + s * stage;
+                const uint32_t sl = slots + b * slot;
                 const uint32_t dst = scale_col + quarter + b * 32;
                 uint4 w[4], x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = 32 * j + lane;
-                    w[j] = r < a.outs ? lds128(st + off_sa + r * 16) : make_uint4(0u, 0u, 0u, 0u);
-                    x[j] = r < rows ? lds128(st + off_sb + r * 16) : make_uint4(0u, 0u, 0u, 0u);
+                    w[j] = r < a.outs ? lds128(sl + r * 16) : make_uint4(0u, 0u, 0u, 0u);
+                    x[j] = r < rows ? lds128(sl + off_sb + r * 16) : make_uint4(0u, 0u, 0u, 0u);
                 }
                 tmem_st4(dst + 0, w[0].x, w[1].x, w[2].x, w[3].x);
                 tmem_st4(dst + 4, w[0].y, w[1].y, w[2].y, w[3].y);
@@ -531,7 +611,10 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sready[b]);
+                if (lane == 0) {
+                    bar_arrive(&sready[b]);
+                    bar_arrive(&sempty[b]);
+                }
             }
         }
         if (!ok) give_up();
@@ -540,18 +623,27 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         const int block = lane & 15, turn = warp - kRound0;
         const int first = (lane >> 4) + (a.spread ? 2 * turn : 0), step = a.spread ? 8 : 2;
         int g = 0;
+        Ring ring;
         bool ok = true;
         Part q;
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             for (int u = q.u0; u < q.u1; ++u, ++g) {
+                const int halves = min(2, item_stages - 2 * u);
+                const Ring lo = ring;
+                ring.next(S);
+                const Ring hi = halves == 2 ? ring : lo;
+                if (halves == 2) ring.next(S);
                 if (!a.spread && (g & 3) != turn) continue;
-                const int s = g % S;
-                ok = bar_wait(&empty[s], ((uint32_t)(g / S) & 1u) ^ 1u, abort_flag);
+                const int b = g % kScales;
+                ok = bar_wait_poll(&empty[lo.s], lo.phase ^ 1u, abort_flag) &&
+                     bar_wait_poll(&empty[hi.s], hi.phase ^ 1u, abort_flag) &&
+                     bar_wait_poll(&sempty[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const uint32_t st = smem + s * stage;
+                const uint32_t st = smem + (block < 8 ? lo.s : hi.s) * stage + off_b;
+                const uint32_t sl = slots + b * slot + off_sb;
                 const int64_t col = (int64_t)u * kUnit + block * kMxBlock;
 #pragma unroll 2
                 for (int r = first; r < tl.z; r += step) {
@@ -574,27 +666,33 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
 #pragma unroll
                         for (int j = 0; j < 4; ++j) w[j] = codes8(v[j], inv);
                     }
-                    // row r of the swizzle atom of 256 columns, its 16-byte chunk block % 8
-                    const uint32_t at = st + off_b + (block >> 3) * kFewCap * 128 + r * 128 +
-                                        ((uint32_t)((block & 7) ^ (r & 7)) << 4);
+                    // row r of the swizzle atom of 256 columns, its 16-byte chunk block % 8;
+                    // the scale byte in any case, codes where the unit has the half
+                    const uint32_t at = st + r * 128 + ((uint32_t)((block & 7) ^ (r & 7)) << 4);
+                    if (block < 8 || halves == 2)
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[0]),
                                  "r"(w[1]), "r"(w[2]), "r"(w[3])
                                  : "memory");
-                    asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(st + off_sb + r * 16 + block),
+                    asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(sl + r * 16 + block),
                                  "r"(byte)
                                  : "memory");
                 }
                 // the MMA reads shared memory through the asynchronous proxy
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
-                if (lane == 0) bar_arrive(&full[s]);
+                if (lane == 0) {
+                    bar_arrive(&full[lo.s]);
+                    if (halves == 2) bar_arrive(&full[hi.s]);
+                    bar_arrive(&sfull[b]);
+                }
             }
         }
         if (!ok) give_up();
-    } else if (warp >= kEpi0 && warp < kEpi0 + 4) {
+    } else if (warp >= kEpi0) {
         const int quarter = warp & 3;
         const int r = 32 * quarter + lane;  // this thread's output of the item
         const bool active = 32 * quarter < a.outs;
+        const int half = (warp - kEpi0) / 4;
         const bool pairs = a.out_features % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % 4 == 0;
         int n = 0;
         Part q;
@@ -602,7 +700,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int acc = n & 1;
-            const bool ok = bar_wait(&dfull[acc], (uint32_t)(n >> 1) & 1u, abort_flag);
+            const bool ok = bar_wait_poll(&dfull[acc], (uint32_t)(n >> 1) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) {
                 give_up();
                 break;
@@ -614,9 +712,12 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             const bool first = plan.s0 / plan.units == shared_item;
             float *slot = a.slots + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * cap * kOuts;
             const uint32_t src = tmem + ((uint32_t)(32 * quarter) << 16) + acc * cap;
-            for (int c = 0; active && c < tl.z; c += 16) {
+            // this warp's rows of the tile
+            const int cut = FEW ? tl.z : min(tl.z, ((tl.z + 1) / 2 + 15) & ~15);
+            const int c0 = half ? cut : 0, c1 = half ? tl.z : cut;
+            for (int c = c0; active && c < c1; c += 16) {
                 uint32_t d[2][8];
-                const int here = min(16, tl.z - c);
+                const int here = min(16, c1 - c);
                 const int64_t base = whole ? row_base(a, tl, c, lane) : 0;
                 tmem_ld8(src + c, d[0]);  // accumulators have a multiple of 16 columns
                 tmem_ld8(src + c + 8, d[1]);
@@ -649,17 +750,17 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             __threadfence();
             __syncwarp();
             uint32_t done = 0;
-            if (lane == 0) done = (uint32_t)atomicAdd(&a.tickets[shared_item * 4 + quarter], 1);
+            if (lane == 0) done = (uint32_t)atomicAdd(&a.tickets[shared_item * 8 + half * 4 + quarter], 1);
             if (__shfl_sync(0xffffffffu, done, 0) != o1 - o0) continue;
             __threadfence();
             // no part is left to count: the ticket is 0 again for the next call
-            if (lane == 0) a.tickets[shared_item * 4 + quarter] = 0;
+            if (lane == 0) a.tickets[shared_item * 8 + half * 4 + quarter] = 0;
             // the first owner's run may have begun in an earlier item
             const bool early = plan.start(o0) / plan.units != shared_item;
-            constexpr int kBatch = FEW ? 16 : 32;  // loads under way
-            for (int c = 0; c < tl.z; c += kBatch) {
+            constexpr int kBatch = 16;  // loads under way
+            for (int c = c0; c < c1; c += kBatch) {
                 float v[kBatch] = {};
-                const int here = min(kBatch, tl.z - c);
+                const int here = min(kBatch, c1 - c);
                 for (uint32_t o = o0; o <= o1; ++o) {
                     const float *part = a.slots +
                         ((int64_t)o * 2 + (o == o0 && early ? 1 : 0)) * cap * kOuts + c * kOuts + r;
@@ -671,8 +772,8 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             }
         }
     }
-    if (warp == kTmemWarp || warp == kSortWarp) {  // rows of pairs without an expert
-        const int64_t at = blockIdx.x * 2 + (warp == kSortWarp), step = gridDim.x * 2;
+    if (warp == kTmemWarp) {  // rows of pairs without an expert
+        const int64_t at = blockIdx.x, step = gridDim.x;
         if (FEW && a.sel) {
             for (int64_t p = at; p < a.pairs; p += step)
                 if (a.sel[p] < 0 || a.sel[p] >= a.experts) zero_row(a, p, lane);
@@ -682,7 +783,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     }
     __syncthreads();
     if (warp == kTmemWarp) {
-        if (lane == 0 && !bar_wait(drain, 0, nullptr)) give_up();
+        if (lane == 0 && !bar_wait_poll(drain, 0, nullptr)) give_up();
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -777,7 +878,7 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
     L.pitch = (width / kMxBlock + 15) / 16 * 16;
     L.max_tiles = (num_experts < pairs ? num_experts : pairs) + pairs / L.cap + 1;
     L.hdr = take(64);
-    L.tickets = take(sizeof(int32_t) * 4 * 2 * kMaxCtas);
+    L.tickets = take(sizeof(int32_t) * 8 * kMaxCtas);
     L.order = take(sizeof(int32_t) * (size_t)pairs);
     L.place = take(sizeof(int32_t) * (size_t)((pairs + 3) / 4 * 4));
     L.tiles = take(16 * (size_t)L.max_tiles);
@@ -802,9 +903,9 @@ cudaError_t launch_kernel(const ProductArgs &a, const MapsOf<FEW> &maps, int sms
         if (err != cudaSuccess) return err;
         if (dev >= 0) attr_done[dev].store(true);
     }
-    const int smem = smem_fixed(a.outs) + a.stages * stage_bytes(a.cap, a.outs);
+    const int smem = smem_fixed(a.cap, a.outs) + a.stages * stage_bytes(a.cap, a.outs);
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    mx_product_kernel<FEW, XT><<<(unsigned)grid, threads_of(FEW), smem, stream>>>(a, maps);
+    mx_product_kernel<FEW, XT><<<(unsigned)grid, kThreads, smem, stream>>>(a, maps);
     return cudaGetLastError();
 }
 
@@ -855,7 +956,7 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
 
 // State of the one-launch product: hdr, tickets, slots.
 constexpr size_t kStateTickets = 256;
-constexpr size_t kStateSlots = kStateTickets + (sizeof(int32_t) * 4 * 2 * kMaxCtas + 255) / 256 * 256;
+constexpr size_t kStateSlots = kStateTickets + (sizeof(int32_t) * 8 * kMaxCtas + 255) / 256 * 256;
 
 static_assert(kStateSlots <= 8192, "the caller clears 8192 bytes");
 

@@ -87,6 +87,23 @@ __device__ __forceinline__ bool bar_wait_spin(uint64_t *b, uint32_t parity, vola
     return true;
 }
 
+// bar_wait for waits that follow one another closely: try_wait itself sleeps
+// until the phase completes or a short limit passes, and the clock, whose
+// reading takes longer than many of these waits, is looked at once in 256 tries.
+__device__ __forceinline__ bool bar_wait_poll(uint64_t *b, uint32_t parity, volatile int *abort) {
+    if (bar_test(b, parity)) return true;
+    unsigned long long t0 = 0;
+    for (uint32_t tries = 1;; ++tries) {
+        if (bar_test(b, parity)) return true;
+        if (tries % 256 == 0) {
+            if (abort && *abort) return false;
+            const unsigned long long t = now_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > kWaitNs) return false;
+        }
+    }
+}
+
 // ---- TMA (no multicast anywhere)
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
                                        uint64_t *b) {
