@@ -33,9 +33,11 @@
 //               every fourth unit, so that four units' loads are under way
 //               (8 tokens' down projection 52 -> 39 us); with more, the warps
 //               share each unit (37 rows 14.2 -> 12 us)
-// Whole 512-column stages with their scales, of which three fit, made each
-// stage wait for its own load, move and products: 4096 x 4096 x 8192 95 us,
-// now 83.
+// One warp's chain of dependent instructions issues every product, so what it
+// waits for and computes paces the kernel: with whole units as stages, of which
+// three fit, and three barriers a unit 4096 x 4096 x 8192 took 95 us; half-unit
+// stages, scales that run ahead and one barrier a unit take 74 (its copies
+// alone 59).
 // Accumulators are double-buffered, scale buffers four deep.
 //
 // Work: item = (128 outputs, tile of rows); a call of few items takes 64 or 32
@@ -74,7 +76,7 @@ constexpr int kUnit = 512;              // columns of a 16-byte row of scales
 constexpr int kStageK = 256;            // columns of a stage: one swizzle atom a side
 constexpr int kScales = 4;              // scale slots, in shared and in tensor memory
 constexpr int kBoxes = 4;               // row boxes: 16, 32, 64, 128
-constexpr int kMaxStages = 24;
+constexpr int kMaxUnits = 12;           // units in flight: two stages each
 constexpr int kSmemCap = 227 * 1024;
 constexpr int kBarBytes = 640;
 constexpr int kFewCap = 16, kFewPairs = 64;          // one launch: rows of a tile, routed pairs
@@ -93,14 +95,14 @@ __host__ __device__ constexpr int spare_bytes(int cap, int outs) {
 __host__ __device__ constexpr int smem_fixed(int cap, int outs) {
     return 1024 + kBarBytes + kFewTable + spare_bytes(cap, outs) + kScales * slot_bytes(cap, outs);
 }
-__host__ __device__ constexpr int stages_for(int cap, int outs) {
-    const int n = (kSmemCap - smem_fixed(cap, outs)) / stage_bytes(cap, outs);
-    return n < kMaxStages ? n : kMaxStages;
+__host__ __device__ constexpr int units_for(int cap, int outs) {
+    const int n = (kSmemCap - smem_fixed(cap, outs)) / (2 * stage_bytes(cap, outs));
+    return n < kMaxUnits ? n : kMaxUnits;
 }
 
 struct ProductArgs {
     int64_t out_features, width, pairs;
-    int cap, outs, stages;
+    int cap, outs, units;  // units: in flight
     int32_t *hdr;
     const int32_t *order;  // null: one matrix, row p is pair p
     const int4 *tiles;
@@ -194,19 +196,12 @@ __device__ __forceinline__ int box_of(const ProductArgs &a, const int4 &tile) {
     return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
 }
 
-// The stages of a part: [first, last) of the item's width / 256. The last
-// unit's second half may lie past the width.
-__device__ __forceinline__ int first_stage(const Part &q) { return 2 * q.u0; }
-__device__ __forceinline__ int last_stage(const Part &q, int stages) {
-    return min(2 * q.u1, stages);
-}
-
-// A place in a ring of stages or scale slots.
+// A place in a ring of units or scale slots.
 struct Ring {
     int s = 0;
     uint32_t phase = 0;
-    __device__ __forceinline__ void next(int stages) {
-        if (++s == stages) {
+    __device__ __forceinline__ void next(int size) {
+        if (++s == size) {
             s = 0;
             phase ^= 1u;
         }
@@ -368,14 +363,19 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     // swizzle atoms repeat every 1024 bytes of shared memory
     const uint32_t raw = saddr(smem_raw);
     const uint32_t smem = (raw + 1023u) & ~1023u;
-    const int S = a.stages, cap = a.cap;
+    const int U = a.units, cap = a.cap;
+    // Scale buffers in use. No more than units in flight: a mover that waits for
+    // the buffer of unit g - B knows that unit's products are done, and so that
+    // `ready` of unit g - U counts no more when it arrives there for unit g.
+    const int B = min(kScales, U);
     const uint32_t stage = (uint32_t)stage_bytes(cap, a.outs);
-    const uint32_t slots = smem + S * stage, slot = (uint32_t)slot_bytes(cap, a.outs);
-    char *bars = smem_raw + (smem - raw) + S * stage + kScales * slot;
-    uint64_t *full = reinterpret_cast<uint64_t *>(bars);
-    uint64_t *empty = full + kMaxStages;
-    uint64_t *sfull = empty + kMaxStages, *sempty = sfull + kScales;
-    uint64_t *sready = sempty + kScales, *sfree = sready + kScales;
+    const uint32_t slots = smem + 2 * U * stage, slot = (uint32_t)slot_bytes(cap, a.outs);
+    char *bars = smem_raw + (smem - raw) + 2 * U * stage + kScales * slot;
+    // ready: a unit's codes are in shared memory and its scales in tensor memory
+    uint64_t *ready = reinterpret_cast<uint64_t *>(bars);
+    uint64_t *empty = ready + kMaxUnits;  // per stage
+    uint64_t *sfull = empty + 2 * kMaxUnits, *sempty = sfull + kScales;
+    uint64_t *sfree = sempty + kScales;   // per scale buffer in tensor memory
     uint64_t *dfull = sfree + kScales, *dempty = dfull + 2, *drain = dempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
@@ -386,14 +386,14 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S; ++i) {
-            bar_init(&full[i], !FEW ? 1 : a.spread ? 5 : 2);
-            bar_init(&empty[i], 1);
+        for (int i = 0; i < U; ++i) {
+            bar_init(&ready[i], !FEW ? 5 : a.spread ? 9 : 6);
+            bar_init(&empty[2 * i], 1);
+            bar_init(&empty[2 * i + 1], 1);
         }
         for (int i = 0; i < kScales; ++i) {
             bar_init(&sfull[i], !FEW ? 1 : a.spread ? 5 : 2);
             bar_init(&sempty[i], 4);
-            bar_init(&sready[i], 4);
             bar_init(&sfree[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -455,28 +455,34 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 // few rows: written by the rounding warps
                 const uint32_t bytes = (uint32_t)(128 * (a.outs + (FEW ? 0 : 16 << box)));
                 const int row0 = (int)((int64_t)tl.x * a.out_features + out0);
-                for (int t = first_stage(q); t < last_stage(q, item_stages); ++t, ++g, ring.next(S)) {
-                    if (!bar_wait_poll(&empty[ring.s], ring.phase ^ 1u, abort_flag)) {
-                        ok = false;
-                        break;
+                for (int u = q.u0; ok && u < q.u1; ++u, ++g, ring.next(U)) {
+                    // the last unit's second half may lie past the width
+                    const int halves = min(2, item_stages - 2 * u);
+                    for (int h = 0; h < halves; ++h) {
+                        const int s = 2 * ring.s + h;
+                        if (!bar_wait_poll(&empty[s], ring.phase ^ 1u, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        if (h == 0) bar_expect_tx(&ready[ring.s], halves * bytes);
+                        const uint32_t st = smem + s * stage;
+                        tma_2d(st, &maps.w, u * 256 + h * 128, row0, &ready[ring.s]);
+                        if constexpr (!FEW)
+                            tma_2d(st + off_b, &maps.x[box], u * 256 + h * 128, tl.y, &ready[ring.s]);
                     }
-                    bar_expect_tx(&full[ring.s], bytes);
-                    const uint32_t st = smem + ring.s * stage;
-                    tma_2d(st, &maps.w, t * 128, row0, &full[ring.s]);
-                    if constexpr (!FEW)
-                        tma_2d(st + off_b, &maps.x[box], t * 128, tl.y, &full[ring.s]);
                 }
             }
             if (!ok) give_up();
-            for (int d = 0; d < S && d < g; ++d) {  // every copy lands before the CTA exits
+            for (int d = 0; d < U && d < g; ++d) {  // every copy lands before the CTA exits
                 const int gg = g - 1 - d;
-                if (!bar_wait_poll(&full[gg % S], (uint32_t)(gg / S) & 1u, nullptr)) give_up();
+                if (!bar_wait_poll(&ready[gg % U], (uint32_t)(gg / U) & 1u, nullptr)) give_up();
             }
         }
         __syncwarp();
     } else if (warp == kScaleWarp) {
         if (lane == 0) {
             int g = 0;
+            Ring ring;
             bool ok = true;
             Part q;
             for (uint32_t i = 0; ok && !*abort_flag && part_of(plan, i, q); ++i) {
@@ -485,9 +491,9 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 const int box = box_of(a, tl);
                 const uint32_t bytes = (uint32_t)(16 * (a.outs + (FEW ? 0 : 16 << box)));
                 const int row0 = (int)((int64_t)tl.x * a.out_features + out0);
-                for (int u = q.u0; u < q.u1; ++u, ++g) {
-                    const int b = g % kScales;
-                    if (!bar_wait_poll(&sempty[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag)) {
+                for (int u = q.u0; u < q.u1; ++u, ++g, ring.next(B)) {
+                    const int b = ring.s;
+                    if (!bar_wait_poll(&sempty[b], ring.phase ^ 1u, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -498,22 +504,22 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 }
             }
             if (!ok) give_up();
-            for (int d = 0; d < kScales && d < g; ++d) {
+            for (int d = 0; d < B && d < g; ++d) {
                 const int gg = g - 1 - d;
-                if (!bar_wait_poll(&sfull[gg % kScales], (uint32_t)(gg / kScales) & 1u, nullptr)) give_up();
+                if (!bar_wait_poll(&sfull[gg % B], (uint32_t)(gg / B) & 1u, nullptr)) give_up();
             }
         }
         __syncwarp();
     } else if (warp == kIssuer) {
         // One warp's dependent instructions bound this loop, so it is bare: the
-        // issuing lane is elected once, a unit's two stages are taken together,
-        // and a product's operands are adds to theirs.
+        // issuing lane is elected once, one barrier says that a unit's codes and
+        // scales are there, and a product's operands are adds to the unit's.
         const bool leader = elect_one();
         const int last_steps = (width - (item_stages - 1) * kStageK + 63) / 64;
         const uint64_t desc0 = sw128_desc(smem);
         const uint32_t desc_stage = stage >> 4, desc_b = off_b >> 4;
-        int n = 0;
-        Ring ring, slot_ring;
+        int n = 0, b = 0;  // b: the unit's scale buffer
+        Ring ring;
         bool ok = true;
         Part q;
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i, ++n) {
@@ -525,22 +531,16 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             const uint32_t d = tmem + acc * cap;
             if (n >= 2)
                 ok = bar_wait_poll(&dempty[acc], ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag);
-            for (int u = q.u0; u < q.u1; ++u, slot_ring.next(kScales)) {
-                const int b = slot_ring.s, left = item_stages - 2 * u;  // stages from here
-                const Ring lo = ring;
-                ring.next(S);
-                const Ring hi = left > 1 ? ring : lo;
-                if (left > 1) ring.next(S);
-                ok = ok && bar_wait_poll(&sready[b], slot_ring.phase, abort_flag) &&
-                     bar_wait_poll(&full[lo.s], lo.phase, abort_flag) &&
-                     bar_wait_poll(&full[hi.s], hi.phase, abort_flag);
+            for (int u = q.u0; u < q.u1; ++u, ring.next(U), b = b + 1 == B ? 0 : b + 1) {
+                const int left = item_stages - 2 * u;  // stages from here
+                ok = ok && bar_wait_poll(&ready[ring.s], ring.phase, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
                     // a step is 32 bytes of each operand: 2 in a descriptor's 16-byte units
-                    const uint64_t da = desc0 + lo.s * desc_stage, db = da + desc_b;
-                    const uint64_t ea = desc0 + hi.s * desc_stage, eb = ea + desc_b;
+                    const uint64_t da = desc0 + 2 * ring.s * desc_stage, db = da + desc_b;
+                    const uint64_t ea = da + desc_stage, eb = ea + desc_b;
                     const uint32_t sa = scale_col + b * 32, sb = sa + 16;
                     const uint32_t more = u > q.u0 ? 1u : 0u;
                     if (left > 2 || (left == 2 && last_steps == 4)) {
@@ -548,12 +548,11 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                         for (int k = 0; k < 4; ++k)
                             tc_mma_mxf4(d, da + 2 * k, db + 2 * k, k & 1 ? odd : even,
                                         sa + (k >> 1) * 4, sb + (k >> 1) * 4, k ? 1u : more);
-                        tc_commit(&empty[lo.s]);
+                        tc_commit(&empty[2 * ring.s]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             tc_mma_mxf4(d, ea + 2 * k, eb + 2 * k, k & 1 ? odd : even,
                                         sa + 8 + (k >> 1) * 4, sb + 8 + (k >> 1) * 4, 1u);
-                        tc_commit(&empty[hi.s]);
                     } else {
                         const int steps = (left - 1) * 4 + last_steps;
                         for (int k = 0; k < steps; ++k) {
@@ -561,9 +560,9 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                             tc_mma_mxf4(d, ka, ka + desc_b, k & 1 ? odd : even,
                                         sa + (k >> 1) * 4, sb + (k >> 1) * 4, k ? 1u : more);
                         }
-                        tc_commit(&empty[lo.s]);
-                        if (left > 1) tc_commit(&empty[hi.s]);
+                        tc_commit(&empty[2 * ring.s]);
                     }
+                    tc_commit(&empty[2 * ring.s + 1]);  // in any case: its phase counts units
                     tc_commit(&sfree[b]);
                     if (u + 1 == q.u1) tc_commit(&dfull[acc]);
                 }
@@ -576,18 +575,17 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         __syncwarp();
     } else if (warp >= kMover0 && warp < kMover0 + 4) {
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
-        int g = 0;
+        Ring ring, buffer;
         bool ok = true;
         Part q;
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
             int out0;
             const int4 tl = tile_of(a, plan, q.item, out0);
             const int rows = 16 << box_of(a, tl);
-            for (int u = q.u0; u < q.u1; ++u, ++g) {
-                const int b = g % kScales;
-                const uint32_t phase = (uint32_t)(g / kScales) & 1u;
-                ok = bar_wait_poll(&sfull[b], phase, abort_flag) &&
-                     (g < kScales || bar_wait_poll(&sfree[b], phase ^ 1u, abort_flag));
+            for (int u = q.u0; u < q.u1; ++u, ring.next(U), buffer.next(B)) {
+                const int b = buffer.s;
+                ok = bar_wait_poll(&sfull[b], buffer.phase, abort_flag) &&
+                     bar_wait_poll(&sfree[b], buffer.phase ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
@@ -612,7 +610,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    bar_arrive(&sready[b]);
+                    bar_arrive(&ready[ring.s]);
                     bar_arrive(&sempty[b]);
                 }
             }
@@ -623,7 +621,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         const int block = lane & 15, turn = warp - kRound0;
         const int first = (lane >> 4) + (a.spread ? 2 * turn : 0), step = a.spread ? 8 : 2;
         int g = 0;
-        Ring ring;
+        Ring ring, scales;
         bool ok = true;
         Part q;
         for (uint32_t i = 0; ok && part_of(plan, i, q); ++i) {
@@ -631,18 +629,18 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
             const int4 tl = tile_of(a, plan, q.item, out0);
             for (int u = q.u0; u < q.u1; ++u, ++g) {
                 const int halves = min(2, item_stages - 2 * u);
-                const Ring lo = ring;
-                ring.next(S);
-                const Ring hi = halves == 2 ? ring : lo;
-                if (halves == 2) ring.next(S);
+                const Ring at = ring, buffer = scales;
+                ring.next(U);
+                scales.next(B);
                 if (!a.spread && (g & 3) != turn) continue;
-                const int b = g % kScales;
-                ok = bar_wait_poll(&empty[lo.s], lo.phase ^ 1u, abort_flag) &&
-                     bar_wait_poll(&empty[hi.s], hi.phase ^ 1u, abort_flag) &&
-                     bar_wait_poll(&sempty[b], ((uint32_t)(g / kScales) & 1u) ^ 1u, abort_flag);
+                const int b = buffer.s;
+                ok = bar_wait_poll(&empty[2 * at.s], at.phase ^ 1u, abort_flag) &&
+                     (halves == 1 ||
+                      bar_wait_poll(&empty[2 * at.s + 1], at.phase ^ 1u, abort_flag)) &&
+                     bar_wait_poll(&sempty[b], buffer.phase ^ 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const uint32_t st = smem + (block < 8 ? lo.s : hi.s) * stage + off_b;
+                const uint32_t st = smem + (2 * at.s + (block >> 3)) * stage + off_b;
                 const uint32_t sl = slots + b * slot + off_sb;
                 const int64_t col = (int64_t)u * kUnit + block * kMxBlock;
 #pragma unroll 2
@@ -668,9 +666,9 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                     }
                     // row r of the swizzle atom of 256 columns, its 16-byte chunk block % 8;
                     // the scale byte in any case, codes where the unit has the half
-                    const uint32_t at = st + r * 128 + ((uint32_t)((block & 7) ^ (r & 7)) << 4);
+                    const uint32_t to = st + r * 128 + ((uint32_t)((block & 7) ^ (r & 7)) << 4);
                     if (block < 8 || halves == 2)
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[0]),
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to), "r"(w[0]),
                                  "r"(w[1]), "r"(w[2]), "r"(w[3])
                                  : "memory");
                     asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(sl + r * 16 + block),
@@ -681,8 +679,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    bar_arrive(&full[lo.s]);
-                    if (halves == 2) bar_arrive(&full[hi.s]);
+                    bar_arrive(&ready[at.s]);
                     bar_arrive(&sfull[b]);
                 }
             }
@@ -903,7 +900,7 @@ cudaError_t launch_kernel(const ProductArgs &a, const MapsOf<FEW> &maps, int sms
         if (err != cudaSuccess) return err;
         if (dev >= 0) attr_done[dev].store(true);
     }
-    const int smem = smem_fixed(a.cap, a.outs) + a.stages * stage_bytes(a.cap, a.outs);
+    const int smem = smem_fixed(a.cap, a.outs) + 2 * a.units * stage_bytes(a.cap, a.outs);
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
     mx_product_kernel<FEW, XT><<<(unsigned)grid, kThreads, smem, stream>>>(a, maps);
     return cudaGetLastError();
@@ -928,7 +925,7 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     a.pairs = p.pairs;
     a.cap = p.L.cap;
     a.outs = p.L.outs;
-    a.stages = stages_for(a.cap, a.outs);
+    a.units = units_for(a.cap, a.outs);
     a.hdr = reinterpret_cast<int32_t *>(p.ws + p.L.hdr);
     if (p.routed) {
         a.order = reinterpret_cast<const int32_t *>(p.ws + p.L.order);
@@ -983,7 +980,7 @@ cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms) {
     a.pairs = p.pairs;
     a.cap = kFewCap;
     a.outs = shape_of(p.pairs, p.num_experts, p.out_features, kFewCap).outs;
-    a.stages = stages_for(a.cap, a.outs);
+    a.units = units_for(a.cap, a.outs);
     a.hdr = reinterpret_cast<int32_t *>(p.state);
     a.tickets = reinterpret_cast<int32_t *>(p.state + kStateTickets);
     a.slots = reinterpret_cast<float *>(p.state + kStateSlots);
