@@ -30,23 +30,27 @@
 //               rounded and written where TMA would have put them, so that
 //               such a call is one launch; each CTA also sorts its (at most
 //               64) pairs by itself. With up to 4 rows a tile each warp takes
-//               every fourth unit, so that four units' loads are under way
-//               (8 tokens' down projection 52 -> 39 us); with more, the warps
-//               share each unit (37 rows 14.2 -> 12 us)
-// One warp's chain of dependent instructions issues every product, so what it
-// waits for and computes paces the kernel: with whole units as stages, of which
-// three fit, and three barriers a unit 4096 x 4096 x 8192 took 95 us; half-unit
-// stages, scales that run ahead and one barrier a unit take 74 (its copies
-// alone 59).
-// Accumulators are double-buffered, scale buffers four deep.
+//               every fourth unit, so that four units' loads are under way (a
+//               quarter off 8 tokens' down projection); with more, the warps
+//               share each unit (a sixth off a call of 37 rows)
+// Accumulators are double-buffered, scale buffers up to four deep.
+//
+// What bounds it. A call whose matrix comes from HBM runs at the copy rate: the
+// head product, 129280 x 4096 for one token, takes 49 us (281.6 MB, 43 at the
+// copy rate, after 4.5 us of start), a routed prefill 192 us (1.21 GB). One
+// whose matrix stays in L2 is bound by what an SM can load, 64 bytes a clock:
+// 4096 x 4096 x 8192 takes 74 us (3.7 PFLOP/s), its copies alone 59. One warp's
+// chain of dependent instructions issues every product, so what it waits for
+// paces the kernel: with whole units as stages, of which three fit, and three
+// barriers a unit that case took 95 us.
 //
 // Work: item = (128 outputs, tile of rows); a call of few items takes 64 or 32
 // outputs to an item and leaves the MMA's other rows unused, which spreads the
-// matrix over more SMs. One matrix: rows innermost, so that
-// it is read from memory once. Routed: outputs innermost, so that CTAs that run
-// together read one matrix's rows next to each other (the other order strides
-// by whole matrices and reads slower); an expert's next tile finds its matrix
-// in L2. The CTAs take items in turn. Where the last round would leave many of
+// matrix over more SMs. One matrix: rows innermost, so that it is read from
+// memory once. Routed: outputs innermost, so that CTAs that run together read
+// one matrix's rows next to each other (the other order strides by whole
+// matrices: a tenth slower in a prefill); an expert's next tile finds its
+// matrix in L2. The CTAs take items in turn. Where the last round would leave many of
 // them idle over a wide matrix, its items are cut into equal runs of units, and
 // the parts of an item meet in f32 slots of the workspace: the last CTA to
 // finish adds them in order, so results repeat bit for bit.
@@ -144,8 +148,8 @@ __device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles
     p.items = p.tiles * p.nblocks;
     // The last round's items are shared when that saves kSaved units or more:
     // joining parts costs 4 to 8 us (a fence, a counter and the sums), a unit
-    // 0.4 us for a CTA that has the memory to itself. Cutting every call of
-    // under one round cost a 4096-wide decode (8 units) 13 us for 9.
+    // 0.4 us for a CTA that has the memory to itself. A decode step's 96 items
+    // of 8 units were done after 13 us when cut to fill all SMs, after 10 whole.
     const uint32_t rest = p.items % ctas, run = (rest * p.units + ctas - 1) / ctas;
     p.whole = p.units - run < kSaved ? p.items : p.items - rest;
     // fewer items than CTAs, at most 2^11 units each: 32 bits hold all * runs
