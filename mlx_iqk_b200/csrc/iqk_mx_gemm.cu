@@ -672,9 +672,9 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
                     // the scale byte in any case, codes where the unit has the half
                     const uint32_t to = st + r * 128 + ((uint32_t)((block & 7) ^ (r & 7)) << 4);
                     if (block < 8 || halves == 2)
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to), "r"(w[0]),
-                                 "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                 : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to),
+                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
                     asm volatile("st.shared.u8 [%0], %1;\n" ::"r"(sl + r * 16 + block),
                                  "r"(byte)
                                  : "memory");

@@ -193,6 +193,30 @@ def test_linear(cuda, dtype, rows, width, out):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,out", [
+    (1, 8192, 64), (3, 16384, 200), (16, 10016, 97), (20, 8224, 33), (40, 16384, 130),
+    (64, 9984, 260), (70, 16384, 300), (129, 12320, 520), (300, 20480, 128), (1, 40000, 1)])
+def test_linear_of_wide_rows(cuda, rows, width, out):
+    """Wide enough that CTAs share an item and join its parts; twice, since the
+    counters of the first call serve the second."""
+    codes, scales, w = make_matrix((out, width), seed=rows + out)
+    x = make_x((rows, width), torch.float32, seed=rows)
+    y = mx_linear(x, codes, scales)
+    check(y, rounded(x), w, torch.float32)
+    assert torch.equal(y, mx_linear(x, codes, scales))
+    check(mx_linear(x.half() / 64, codes, scales), rounded(x.half() / 64), w, torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,experts", [(1, 3, 5), (20, 3, 6), (90, 2, 3)])
+def test_switch_linear_of_wide_rows(cuda, t, k, experts):
+    codes, scales, w, x, idx = routed_case(t, k, experts, False, torch.float32, 8224, 70, t)
+    idx[t // 2, 0] = -1
+    for _ in range(2):
+        check_routed(mx_switch_linear(x, idx.cuda(), codes, scales), x, idx, w, torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 5, 150])
 def test_linear_out_types_strides_axes_and_repeats(cuda, rows):
     codes, scales, w = make_matrix((200, 1024), seed=3)
