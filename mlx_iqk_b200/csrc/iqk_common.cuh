@@ -10,6 +10,19 @@
 
 namespace iqk {
 
+// Programmatic dependent launch (PTX griddepcontrol). A kernel
+// launched with programmatic stream serialization may start while the previous
+// kernel of the stream is still draining: it does its shared-memory set-up,
+// then waits for that kernel's completion (and its memory) before it reads or
+// writes any global memory that the previous kernel may touch, and at once lets
+// the next kernel start.
+__device__ __forceinline__ void grid_dep_wait() {
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+__device__ __forceinline__ void grid_dep_launch() {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
 // iq2nl_values (base alphabet 0..3, shifted alphabet 4..7) as int8 bytes:
 // T0 = {-31, -13, 1, 17}, T1 = {-26, -8, 6, 22}, little-endian in one word so
 // a byte permute indexes them directly.

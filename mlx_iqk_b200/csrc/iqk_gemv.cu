@@ -47,6 +47,7 @@
 
 #include "iqk_common.cuh"
 #include "iqk_gemv.cuh"
+#include "iqk_host.cuh"
 #include "iqk_tables.cuh"
 
 namespace iqk {
@@ -69,18 +70,6 @@ __device__ __forceinline__ void mma_s8(int32_t d[4], const uint32_t a[4], uint32
         "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-}
-
-// Programmatic dependent launch (PTX griddepcontrol). Both decode kernels are
-// launched with programmatic stream serialization: a kernel may start while
-// the previous kernel of the stream is still draining, does its shared-memory
-// set-up, then waits for that kernel's completion (and its memory) before it
-// reads or writes any global memory, and at once lets the next kernel start.
-__device__ __forceinline__ void grid_dep_wait() {
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-}
-__device__ __forceinline__ void grid_dep_launch() {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 }
 
 // ------------------------------------------------------------- prep kernel
@@ -1307,23 +1296,6 @@ static int gemv_smem_for(int member, int n, bool narrow, bool glu) {
 #undef IQK_SM
 }
 int gemv_smem_for(int member, int n, bool narrow) { return gemv_smem_for(member, n, narrow, false); }
-
-// Launch configuration with programmatic stream serialization (the kernel
-// waits with griddepcontrol.wait before its first global-memory access).
-struct PdlLaunch {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    PdlLaunch(unsigned grid, unsigned block, size_t smem, cudaStream_t stream) {
-        cfg.gridDim = dim3(grid);
-        cfg.blockDim = dim3(block);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = stream;
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-};
 
 cudaError_t launch_gemv_prepare(const void *x, int x_dtype, int64_t x_rows, int n,
                                 int64_t num_experts, const int32_t *sel, const int32_t *tok,

@@ -31,4 +31,21 @@ inline int num_sms_current() {
     return sms;
 }
 
+// Launch configuration with programmatic stream serialization (the kernel
+// waits with griddepcontrol.wait, see grid_dep_wait).
+struct PdlLaunch {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    PdlLaunch(unsigned grid, unsigned block, size_t smem, cudaStream_t stream) {
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(block);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+};
+
 }  // namespace iqk

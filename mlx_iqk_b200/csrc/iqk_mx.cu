@@ -30,15 +30,18 @@ namespace {
 
 // Row r of the output is row r of x; with `place`, row r of x goes to the rows
 // place[r * copies ..] of its `copies` pairs (-1: none), so that a token's row
-// is read and rounded once. Block 0 clears the words that the product kernel
-// counts in.
+// is read and rounded once. That launch overlaps the sort that writes `place`:
+// it waits for the sort after its first rows are read and rounded (`place` is
+// volatile so that no load of it is moved above the wait). Block 0 clears the
+// words that the product kernel counts in.
 // I: an index type that holds rows * width / 16.
 template <typename T, bool WIDE, typename I>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const T *__restrict__ x, I rows, I width, int64_t row_stride,
                    uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
-                   int64_t scale_stride, const int32_t *__restrict__ place, int copies,
+                   int64_t scale_stride, const volatile int32_t *place, int copies,
                    int32_t *__restrict__ zero, int zero_words) {
+    grid_dep_launch();
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < zero_words; i += blockDim.x) zero[i] = 0;
     constexpr int kShare = (int)sizeof(T) / 2;      // threads of a block
@@ -68,6 +71,7 @@ mx_quantize_kernel(const T *__restrict__ x, I rows, I width, int64_t row_stride,
             raw[j].get(v);
             word[j] = codes8(v, inv);
         }
+        if (place) grid_dep_wait();
         for (int j = 0; j < copies; ++j) {
             const int64_t to = place ? (int64_t)place[(int64_t)at.row * copies + j] : (int64_t)at.row;
             if (to < 0) continue;
@@ -77,6 +81,7 @@ mx_quantize_kernel(const T *__restrict__ x, I rows, I width, int64_t row_stride,
                 scales[to * scale_stride + (int64_t)(at.col / kShare)] = (uint8_t)byte;
         }
     }
+    if (place) grid_dep_wait();  // a thread without items, too
 }
 
 // 2^(byte - 127); 255 is NaN.
@@ -132,6 +137,7 @@ constexpr int kSortCtas = 8;
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(1024)
 mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLayout L,
                char *ws) {
+    grid_dep_launch();
     extern __shared__ int32_t cnt[];  // [num_experts + 1]: the last has no expert
     __shared__ int32_t warp_rows[32], warp_tiles[32], none_base;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, wid = tid >> 5;
@@ -291,10 +297,13 @@ cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t w
     const unsigned blocks = stream_blocks(rows * width * (int64_t)element(dtype) / 64, sms);
     const bool wide = aligned(x, 16) && row_stride * (int64_t)element(dtype) % 16 == 0;
     const bool small = rows * (width / 16) < (int64_t)1 << 31;
+    PdlLaunch pl(blocks, 256, 0, stream);
+    if (!place) pl.cfg.numAttrs = 0;  // what precedes it may have written x
+    cudaError_t err;
 #define IQK_QI(T, W, I)                                                                         \
-    mx_quantize_kernel<T, W, I><<<blocks, 256, 0, stream>>>(                                    \
-        static_cast<const T *>(x), (I)rows, (I)width, row_stride, codes, scales, scale_stride,  \
-        place, copies, zero, zero_words)
+    err = cudaLaunchKernelEx(&pl.cfg, mx_quantize_kernel<T, W, I>, static_cast<const T *>(x),   \
+                             (I)rows, (I)width, row_stride, codes, scales, scale_stride, place, \
+                             copies, zero, zero_words)
 #define IQK_Q(T)                                        \
     do {                                                \
         if (wide && small) IQK_QI(T, true, uint32_t);   \
@@ -307,7 +316,7 @@ cudaError_t launch_mx_quantize(const void *x, int dtype, int64_t rows, int64_t w
     else IQK_Q(__nv_bfloat16);
 #undef IQK_QI
 #undef IQK_Q
-    return cudaGetLastError();
+    return err;
 }
 
 }  // namespace iqk

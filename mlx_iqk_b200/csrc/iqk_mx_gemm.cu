@@ -417,6 +417,8 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         tmem_relinquish();
         tc_fence_before();
     }
+    grid_dep_wait();
+    grid_dep_launch();
     if (FEW && a.sel) {
         if (warp == kScaleWarp) {
             bool bad;
@@ -906,8 +908,8 @@ cudaError_t launch_kernel(const ProductArgs &a, const MapsOf<FEW> &maps, int sms
     }
     const int smem = smem_fixed(a.cap, a.outs) + 2 * a.units * stage_bytes(a.cap, a.outs);
     const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-    mx_product_kernel<FEW, XT><<<(unsigned)grid, kThreads, smem, stream>>>(a, maps);
-    return cudaGetLastError();
+    PdlLaunch pl((unsigned)grid, kThreads, (size_t)smem, stream);
+    return cudaLaunchKernelEx(&pl.cfg, mx_product_kernel<FEW, XT>, a, maps);
 }
 
 cudaError_t encode_matrix(MatrixMaps &maps, const uint8_t *codes, const uint8_t *scales,
