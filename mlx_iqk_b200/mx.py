@@ -262,6 +262,9 @@ class MxSwitchGLU(nn.Module):
         ``[..., hidden]`` float32; with ``scores`` None each pair's own output,
         ``[..., top_k, hidden]``. Index -1 contributes nothing."""
         lead, k = tuple(indices.shape[:-1]), indices.shape[-1]
+        if scores is not None and (not isinstance(scores, torch.Tensor)
+                                   or scores.device != x.device):
+            raise IqkRuntimeError("scores must be a tensor beside x")
         if tuple(x.shape) != lead + (self.hidden,) or \
                 (scores is not None and scores.shape != indices.shape):
             raise IqkRuntimeError(
