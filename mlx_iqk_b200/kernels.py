@@ -705,10 +705,21 @@ def mx_linear(x: torch.Tensor, rows: int, row_stride: int, codes: torch.Tensor,
         raise_for_status(status, "iqk_mx_linear")
 
 
+def check_mx_workspace(workspace: torch.Tensor, device: torch.device | None = None) -> None:
+    """A caller's workspace reaches the kernels as an address: refuse what is not
+    contiguous bytes on the GPU (on ``device``, where given)."""
+    if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 \
+            or not workspace.is_cuda or not workspace.is_contiguous() \
+            or (device is not None and workspace.device != device):
+        raise IqkRuntimeError("workspace must be a contiguous uint8 tensor beside the activations")
+
+
 def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
               codes: torch.Tensor, scales: torch.Tensor, scale_stride: int, y: torch.Tensor,
               workspace: torch.Tensor | None = None) -> None:
     """``iqk_mx_routed``: ``y [pairs, out]`` through the stacked matrices."""
+    if workspace is not None:
+        check_mx_workspace(workspace, y.device)
     pairs, width = sel.numel(), x.shape[-1]
     experts, out_features = codes.shape[0], codes.shape[1]
     if workspace is None:
@@ -729,6 +740,9 @@ def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
 
 def mx_read_error(workspace: torch.Tensor) -> int:
     """``iqk_mx_read_error``: the device error bits of a routed product's workspace."""
+    check_mx_workspace(workspace)
+    if workspace.numel() < 16:
+        raise IqkRuntimeError("workspace is no routed product's: it has no error word")
     flags = ctypes.c_int32(0)
     raise_for_status(library().iqk_mx_read_error(workspace.data_ptr(), ctypes.byref(flags),
                                                  stream_handle(workspace.device)),

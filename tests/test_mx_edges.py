@@ -6,8 +6,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mlx_iqk_b200 import MxSwitchGLU
+from mlx_iqk_b200 import MxSwitchGLU, mx_switch_linear
 from mlx_iqk_b200 import kernels as K
+from test_mx import make_matrix, make_x
 
 
 # ------------------------------------------------------ the layer's arguments
@@ -33,3 +34,38 @@ def test_layer_refuses_host_scores(cuda):
     with pytest.raises(K.IqkRuntimeError, match="scores"):
         layer(x, idx, torch.ones((3, 2)))
     assert layer(x, idx, torch.ones((3, 2), device="cuda")).shape == (3, 64)
+
+
+# ---------------------------------------------------------- caller's workspace
+
+
+def test_host_workspaces_are_refused():
+    x, y = torch.zeros((2, 64)), torch.zeros((2, 32))
+    sel = torch.zeros(2, dtype=torch.int32)
+    codes, scales = (torch.zeros((4, 32, n), dtype=torch.uint8) for n in (32, 16))
+    with pytest.raises(K.IqkRuntimeError, match="workspace"):
+        K.mx_routed(x, 2, 64, sel, codes, scales, 16, y,
+                    torch.zeros(1 << 20, dtype=torch.uint8))
+    with pytest.raises(K.IqkRuntimeError, match="workspace"):
+        K.mx_read_error(torch.zeros(1 << 20, dtype=torch.uint8))
+
+
+@pytest.mark.gpu
+def test_workspaces_of_another_kind_are_refused(cuda):
+    codes, scales, _ = make_matrix((4, 32, 64), seed=1)
+    x = make_x((3, 1, 1, 64), torch.float32, seed=2)
+    idx = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    need = K.mx_workspace_bytes(6, 4, 64, 32)
+    want = mx_switch_linear(x, idx, codes, scales)
+    good = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert torch.equal(mx_switch_linear(x, idx, codes, scales, workspace=good), want)
+    for bad in (torch.empty(need, dtype=torch.uint8),
+                torch.empty(need, dtype=torch.uint8).pin_memory(),
+                torch.empty(need, dtype=torch.int32, device="cuda"),
+                torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2],
+                good[:need - 256]):
+        with pytest.raises(K.IqkRuntimeError):
+            mx_switch_linear(x, idx, codes, scales, workspace=bad)
+    with pytest.raises(K.IqkRuntimeError, match="workspace"):
+        K.mx_read_error(good[:8])
+    assert K.mx_read_error(good) == 0
