@@ -36,6 +36,11 @@ from .kernels import IqkKernelError, IqkRuntimeError
 MX_BLOCK = 32
 
 
+def _check_no_gradient(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise IqkRuntimeError(f"the MXFP4 operators carry no gradient: detach {what}")
+
+
 def _rows(x, what="x"):
     """``(x, rows, row_stride)`` of float rows whose columns are adjacent: ``x``
     itself, or a copy where its layout is not one of evenly spaced rows."""
@@ -43,8 +48,7 @@ def _rows(x, what="x"):
         raise IqkRuntimeError(f"{what} must be a tensor on the GPU")
     if x.dtype not in K.DTYPE_IDS:
         raise IqkRuntimeError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise IqkRuntimeError(f"the MXFP4 operators carry no gradient: detach {what}")
+    _check_no_gradient(x, what)
     width = x.shape[-1] if x.dim() else 0
     if width <= 0 or width % MX_BLOCK:
         raise IqkKernelError(
@@ -260,11 +264,14 @@ class MxSwitchGLU(nn.Module):
     def forward(self, x, indices, scores=None) -> torch.Tensor:
         """``x [..., hidden]``, ``indices`` and ``scores [..., top_k]`` ->
         ``[..., hidden]`` float32; with ``scores`` None each pair's own output,
-        ``[..., top_k, hidden]``. Index -1 contributes nothing."""
+        ``[..., top_k, hidden]``. Index -1 contributes nothing. Scores that ask
+        for a gradient are refused: to train a router, leave them out and weight
+        the pairs' outputs."""
         lead, k = tuple(indices.shape[:-1]), indices.shape[-1]
-        if scores is not None and (not isinstance(scores, torch.Tensor)
-                                   or scores.device != x.device):
-            raise IqkRuntimeError("scores must be a tensor beside x")
+        if scores is not None:
+            if not isinstance(scores, torch.Tensor) or scores.device != x.device:
+                raise IqkRuntimeError("scores must be a tensor beside x")
+            _check_no_gradient(scores, "scores")
         if tuple(x.shape) != lead + (self.hidden,) or \
                 (scores is not None and scores.shape != indices.shape):
             raise IqkRuntimeError(
@@ -278,7 +285,7 @@ class MxSwitchGLU(nn.Module):
             return torch.zeros(shape, dtype=f32, device=x.device)
         gate = mx_switch_linear(rows, sel, self.gate_codes, self.gate_scales, f32)
         up = mx_switch_linear(rows, sel, self.up_codes, self.up_scales, f32)
-        w = None if scores is None else scores.detach().reshape(-1).to(f32).contiguous()
+        w = None if scores is None else scores.reshape(-1).to(f32).contiguous()
         h = torch.empty((sel.numel(), self.inter), dtype=f32, device=x.device)
         K.swiglu_rows(gate.view(-1, self.inter), up.view(-1, self.inter), w, h)
         y = mx_switch_linear(h.view(-1, k, 1, self.inter), sel, self.down_codes,

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mlx_iqk_b200 import MxSwitchGLU, mx_switch_linear
+from mlx_iqk_b200 import MxSwitchGLU, mx_switch_linear, route
 from mlx_iqk_b200 import kernels as K
 from test_mx import make_matrix, make_x
 
@@ -69,3 +69,25 @@ def test_workspaces_of_another_kind_are_refused(cuda):
     with pytest.raises(K.IqkRuntimeError, match="workspace"):
         K.mx_read_error(good[:8])
     assert K.mx_read_error(good) == 0
+
+
+def test_layer_refuses_scores_that_ask_for_a_gradient():
+    layer, x, idx = small_layer("cpu")
+    scores = torch.ones((3, 2), requires_grad=True)
+    with pytest.raises(K.IqkRuntimeError, match="no gradient.*scores"):
+        layer(x, idx, scores)
+    with torch.no_grad(), pytest.raises(K.IqkRuntimeError, match="on the GPU"):
+        layer(x, idx, scores)  # without a graph they are plain numbers
+
+
+@pytest.mark.gpu
+def test_layer_behind_a_router_under_training(cuda):
+    """The router's weights as scores: refused while a graph is built, served without one."""
+    layer, x, idx = small_layer("cuda")
+    logits = torch.zeros((3, 4), device="cuda", requires_grad=True)
+    indices, weights = route(logits, 2)
+    with pytest.raises(K.IqkRuntimeError, match="no gradient.*scores"):
+        layer(x, indices, weights)
+    want = layer(x, indices, weights.detach())
+    with torch.no_grad():
+        assert torch.equal(layer(x, indices, weights), want)
