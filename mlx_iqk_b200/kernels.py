@@ -15,6 +15,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from .format import (DENSE_MEMBER_IDS, MEMBER_IDS, IqkFormatError, check_dense_member,
                      check_member, check_row_width)
@@ -243,6 +244,13 @@ def check_current(device: torch.device) -> None:
         raise IqkRuntimeError(
             f"tensors on {device}, but the current device is {torch.cuda.current_device()}")
     check_device(device)
+
+
+def refuse_tangent(t: torch.Tensor, what: str) -> None:
+    """The kernels have no forward-mode derivative: a dual tensor's tangent would
+    be lost without a word, since a call by address does not see it."""
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise IqkRuntimeError(f"{what} carries a tangent: there is no forward-mode derivative")
 
 
 def stream_handle(device: torch.device) -> int:

@@ -14,8 +14,9 @@ Scores are ``softmax`` over the experts or ``sigmoid`` of each logit. A logit
 of ``-inf`` is no expert, and ``mask`` (bool, one per token) leaves whole rows
 out: the places of a row without an expert hold index ``-1`` and weight 0,
 which the experts' products turn into zero rows. Everything is differentiable
-in ``logits`` (float32, float16 or bfloat16); sums are float32 and joined in a
-fixed order, so results repeat bit for bit.
+in ``logits`` (float32, float16 or bfloat16), once and in reverse mode: forward
+mode and second derivatives are refused. Sums are float32 and joined in a fixed
+order, so results repeat bit for bit.
 """
 
 from __future__ import annotations
@@ -48,6 +49,7 @@ def _check(logits, top_k, scoring, mask, offsets=None):
         raise IqkRuntimeError("logits must be a tensor on the GPU")
     if logits.dtype not in K.DTYPE_IDS:
         raise IqkRuntimeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    K.refuse_tangent(logits, "logits")
     if logits.dim() < 1:
         raise IqkRuntimeError("logits must have an expert axis")
     experts = logits.shape[-1]

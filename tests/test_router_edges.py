@@ -1,0 +1,40 @@
+"""The router at its edges: derivatives it does not have, indices and offsets out
+of the common range, more tokens than the kernels take at once. Definitions and
+tolerances are those of ``test_router``."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from mlx_iqk_b200 import balance_loss, route, route_balanced
+from mlx_iqk_b200 import kernels as K
+from test_router import make
+
+
+def test_a_tangent_is_seen():
+    x = torch.ones(3)
+    K.refuse_tangent(x, "x")
+    with forward_ad.dual_level():
+        K.refuse_tangent(x, "x")
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        for t in (dual, dual.view(3, 1)):
+            with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
+                K.refuse_tangent(t, "x")
+            with torch.no_grad(), pytest.raises(K.IqkRuntimeError, match="forward-mode"):
+                K.refuse_tangent(t, "x")
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(cuda):
+    z = make(5, 12, torch.float32, seed=1)
+    idx, _ = route(z, 3)
+    with forward_ad.dual_level():
+        for primal in (z, z.clone().requires_grad_()):
+            dual = forward_ad.make_dual(primal, torch.ones_like(z))
+            for call in (lambda: route(dual, 3), lambda: route_balanced(dual, 3),
+                         lambda: balance_loss(dual, idx)):
+                with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
+                    call()
+        assert torch.equal(route(z, 3)[0], idx)  # others are served as ever
