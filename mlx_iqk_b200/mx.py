@@ -39,6 +39,7 @@ MX_BLOCK = 32
 def _check_no_gradient(t, what):
     if t.requires_grad and torch.is_grad_enabled():
         raise IqkRuntimeError(f"the MXFP4 operators carry no gradient: detach {what}")
+    K.refuse_tangent(t, what)
 
 
 def _rows(x, what="x"):

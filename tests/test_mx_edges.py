@@ -5,8 +5,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
-from mlx_iqk_b200 import MxSwitchGLU, mx_switch_linear, route
+from mlx_iqk_b200 import MxSwitchGLU, mx_linear, mx_quantize, mx_switch_linear, route
 from mlx_iqk_b200 import kernels as K
 from test_mx import make_matrix, make_x
 
@@ -91,3 +92,25 @@ def test_layer_behind_a_router_under_training(cuda):
     want = layer(x, indices, weights.detach())
     with torch.no_grad():
         assert torch.equal(layer(x, indices, weights), want)
+
+
+def test_layer_refuses_scores_with_a_tangent():
+    layer, x, idx = small_layer("cpu")
+    with forward_ad.dual_level():
+        scores = forward_ad.make_dual(torch.ones((3, 2)), torch.ones((3, 2)))
+        with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
+            layer(x, idx, scores)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(cuda):
+    codes, scales, _ = make_matrix((32, 64), seed=1)
+    idx = torch.zeros((2, 1), dtype=torch.int32, device="cuda")
+    x = torch.ones((2, 64), device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        for call in (lambda: mx_quantize(dual), lambda: mx_linear(dual, codes, scales),
+                     lambda: mx_switch_linear(dual.view(2, 1, 1, 64), idx, codes[None],
+                                              scales[None])):
+            with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
+                call()
