@@ -458,6 +458,10 @@ int iqk_dense_gemv(int member, const void *x, int64_t tokens, const void *const 
  * with the call's indices) and of the loss (the forward's slope, and one f32
  * at grad_loss); either may be NULL.
  */
+/* The operators take int32 expert indices. out [count] holds 64-bit ones, those
+ * beyond 32 bits at the type's ends (no expert, as any index outside the range). */
+int iqk_narrow_indices(const int64_t *indices, int64_t count, int32_t *out, iqk_stream_t stream);
+
 int iqk_route(const void *logits, int dtype, int64_t tokens, int64_t num_experts,
               int64_t row_stride, const uint8_t *mask, int top_k, int scoring, int renormalize,
               float scale, int32_t *indices, float *weights, iqk_stream_t stream);

@@ -582,6 +582,15 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, RouteG
     }
 }
 
+// 64-bit expert indices to 32 bits: what lies beyond them is held at the type's
+// ends, which are no experts. Dropping the upper half would make 2^32 + 3 expert 3.
+__global__ void __launch_bounds__(256)
+narrow_indices_kernel(const int64_t *__restrict__ in, int64_t count, int32_t *__restrict__ out) {
+    const int64_t step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += step)
+        out[i] = (int32_t)max((int64_t)INT32_MIN, min((int64_t)INT32_MAX, in[i]));
+}
+
 struct RouteLayout {
     size_t score, count, rows, total;
     int64_t blocks, per_block;
@@ -691,6 +700,17 @@ RouteArgs route_args(const void *logits, int64_t tokens, int64_t experts, int64_
 using namespace iqk;
 
 extern "C" {
+
+int iqk_narrow_indices(const int64_t *indices, int64_t count, int32_t *out, iqk_stream_t stream) {
+    if (count < 0) return IQK_ERR_GEOMETRY;
+    if (count == 0) return IQK_OK;
+    if (!indices || !out) return IQK_ERR_ARGUMENT;
+    if (!aligned(indices, 8) || !aligned(out, 4)) return IQK_ERR_ALIGNMENT;
+    const int64_t want = (count + 255) / 256, most = (int64_t)num_sms_current() * 8;
+    narrow_indices_kernel<<<(unsigned)(want < most ? want : most), 256, 0,
+                            reinterpret_cast<cudaStream_t>(stream)>>>(indices, count, out);
+    return cuda_status(cudaGetLastError());
+}
 
 int iqk_route(const void *logits, int dtype, int64_t tokens, int64_t num_experts,
               int64_t row_stride, const uint8_t *mask, int top_k, int scoring, int renormalize,

@@ -154,6 +154,8 @@ def library() -> ctypes.CDLL:
     lib.iqk_pairs_combine.argtypes = [vp, vp, i64, i32, i64, i64, vp, i32, vp]
     lib.iqk_pairs_combine.restype = i32
     f32 = ctypes.c_float
+    lib.iqk_narrow_indices.argtypes = [vp, i64, vp, vp]
+    lib.iqk_narrow_indices.restype = i32
     lib.iqk_route.argtypes = [vp, i32, i64, i64, i64, vp, i32, i32, i32, f32, vp, vp, vp]
     lib.iqk_route.restype = i32
     lib.iqk_balance_workspace_bytes.argtypes = [i64, i64, i64]
@@ -200,7 +202,7 @@ def exported_symbols() -> list[str]:
             "iqk_dequant_floor", "iqk_grouped_run_range", "iqk_pack",
             "iqk_gemv_glu_run", "iqk_swiglu_rows", "iqk_check_bounded_wait",
             "iqk_dense_dequant", "iqk_dense_gemv",
-            "iqk_route", "iqk_balance_workspace_bytes", "iqk_route_balanced",
+            "iqk_narrow_indices", "iqk_route", "iqk_balance_workspace_bytes", "iqk_route_balanced",
             "iqk_route_backward", "iqk_mx_quantize", "iqk_mx_dequantize",
             "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error",
             "iqk_mx_few_state_bytes", "iqk_mx_few_fits", "iqk_mx_few"]
@@ -561,6 +563,23 @@ def grouped_read_error(workspace: torch.Tensor) -> int:
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def expert_indices(indices: torch.Tensor) -> torch.Tensor:
+    """``indices`` as the contiguous int32 that the kernels read. What 32 bits do not
+    hold stays outside the experts (``iqk_narrow_indices``) and does not wrap into them."""
+    if indices.dtype == torch.int32:
+        return indices.contiguous()
+    if indices.dtype.itemsize < 4 or not indices.is_cuda:
+        return indices.to(torch.int32).contiguous()
+    wide = indices.to(torch.int64).contiguous()
+    check_current(wide.device)
+    out = wide.new_empty(wide.shape, dtype=torch.int32)
+    status = library().iqk_narrow_indices(wide.data_ptr(), wide.numel(), out.data_ptr(),
+                                          stream_handle(wide.device))
+    if status:
+        raise_for_status(status, "iqk_narrow_indices")
+    return out
 
 
 @functools.lru_cache(maxsize=1024)

@@ -206,7 +206,7 @@ def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = 
     experts, out, half = codes.shape
     if half * 2 != x.shape[-1]:
         raise IqkRuntimeError(f"x of width {x.shape[-1]} meets matrices of {half * 2}")
-    sel = indices.to(torch.int32).contiguous()
+    sel = K.expert_indices(indices)
     pairs = sel.numel()
     if pairs and (count == 0 or pairs % count):
         raise IqkRuntimeError(
@@ -278,7 +278,7 @@ class MxSwitchGLU(nn.Module):
             raise IqkRuntimeError(
                 f"x {tuple(x.shape)}, indices {tuple(indices.shape)} and scores "
                 f"{None if scores is None else tuple(scores.shape)} do not belong together")
-        sel = indices.reshape(-1, k).to(torch.int32).contiguous()
+        sel = K.expert_indices(indices.reshape(-1, k))
         rows = x.reshape(-1, 1, 1, self.hidden)
         f32 = torch.float32
         if not sel.numel():

@@ -174,7 +174,7 @@ def balance_loss(logits, indices, *, scoring: str = "softmax", mask=None, offset
         raise IqkRuntimeError("indices must be on the logits' device")
     top_k = indices.shape[-1]
     rows, mask, offsets, scoring = _check(logits, top_k, scoring, mask, offsets)
-    sel = indices.to(torch.int32).contiguous()
+    sel = K.expert_indices(indices)
     call = (top_k, scoring, True, 1.0)
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, (rows, sel, mask, offsets), call, True)[2:]

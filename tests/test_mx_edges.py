@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from mlx_iqk_b200 import MxSwitchGLU, mx_linear, mx_quantize, mx_switch_linear, route
 from mlx_iqk_b200 import kernels as K
-from test_mx import make_matrix, make_x
+from test_mx import check_routed, make_matrix, make_x
 
 
 # ------------------------------------------------------ the layer's arguments
@@ -114,3 +114,63 @@ def test_forward_mode_is_refused(cuda):
                                               scales[None])):
             with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
                 call()
+
+
+# ------------------------------------------------------------- expert indices
+
+# int64 values whose lower 32 bits name an expert, or -1
+BEYOND = [2 ** 32 + 3, 2 ** 32 - 1, -2 ** 32, 2 ** 40 + 1, -2 ** 63, 2 ** 63 - 1, 2 ** 31]
+
+
+def test_narrowing_refuses_before_any_device_call():
+    lib = K.library()
+    x = 0x10000
+    assert lib.iqk_narrow_indices(x, -1, x, None) == 3
+    assert lib.iqk_narrow_indices(None, 0, None, None) == 0
+    assert lib.iqk_narrow_indices(None, 4, x, None) == 4
+    assert lib.iqk_narrow_indices(x, 4, None, None) == 4
+    assert lib.iqk_narrow_indices(x + 4, 4, x, None) == 5
+    assert lib.iqk_narrow_indices(x, 4, x + 2, None) == 5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [7, 300])
+def test_indices_beyond_32_bits_are_no_expert(cuda, t):
+    codes, scales, w = make_matrix((5, 40, 96), seed=t)
+    x = make_x((t, 1, 1, 96), torch.float32, seed=t)
+    idx = torch.arange(2 * t).view(t, 2) % 5
+    idx[:7, 1] = torch.tensor(BEYOND)
+    ws = torch.empty(K.mx_workspace_bytes(2 * t, 5, 96, 40), dtype=torch.uint8, device="cuda")
+    y = mx_switch_linear(x, idx.cuda(), codes, scales, workspace=ws)
+    assert K.mx_read_error(ws) == K.DEVERR_EXPERT
+    for got in (y, mx_switch_linear(x, idx.cuda(), codes, scales),
+                mx_switch_linear(x, idx.t().contiguous().cuda().t(), codes, scales)):
+        assert (got[:7, 1] == 0).all()
+        check_routed(got, x, idx, w, torch.float32)
+
+
+@pytest.mark.gpu
+def test_layer_takes_indices_beyond_32_bits_for_no_expert(cuda):
+    layer = MxSwitchGLU(4, 64, 32, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    for name, shape in (("gate", (4, 32, 64)), ("up", (4, 32, 64)), ("down", (4, 64, 32))):
+        layer.load_weights(name, torch.randn(shape, generator=g).cuda())
+    x = torch.randn((7, 64), generator=g).cuda()
+    idx = torch.zeros((7, 2), dtype=torch.int64)
+    idx[:, 1] = torch.tensor(BEYOND)
+    none = torch.where(idx > 0, -1, idx).clamp(min=-1)
+    pairs = layer(x, idx.cuda())
+    assert (pairs[:, 1] == 0).all() and torch.equal(pairs, layer(x, none.cuda()))
+    ones = torch.ones((7, 2), device="cuda")
+    assert torch.equal(layer(x, idx.cuda(), ones), layer(x, none.cuda(), ones))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [0, 1, 255, 1000, 148 * 8 * 256 * 2 + 5])
+def test_narrowed_indices(cuda, count):
+    g = torch.Generator().manual_seed(count)
+    wide = torch.randint(-2 ** 62, 2 ** 62, (count,), generator=g) >> \
+        torch.randint(0, 62, (count,), generator=g)
+    got = K.expert_indices(wide.cuda())
+    assert got.dtype == torch.int32
+    assert torch.equal(got.cpu().long(), wide.clamp(-2 ** 31, 2 ** 31 - 1))

@@ -10,7 +10,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from mlx_iqk_b200 import balance_loss, route, route_balanced
 from mlx_iqk_b200 import kernels as K
-from test_router import make
+from test_router import LOSS_TOL, close, make, ref_balance
 
 
 def test_a_tangent_is_seen():
@@ -38,3 +38,16 @@ def test_forward_mode_is_refused(cuda):
                 with pytest.raises(K.IqkRuntimeError, match="forward-mode"):
                     call()
         assert torch.equal(route(z, 3)[0], idx)  # others are served as ever
+
+
+@pytest.mark.gpu
+def test_balance_of_indices_beyond_32_bits(cuda):
+    """Entries outside the experts count for none, whatever their lower 32 bits are."""
+    z = make(9, 10, torch.float32, seed=5)
+    idx = torch.arange(27).view(9, 3) % 10
+    idx[:7, 1] = torch.tensor([2 ** 32 + 3, 2 ** 32 - 1, -2 ** 32, 2 ** 40 + 1, -2 ** 63,
+                               2 ** 63 - 1, 2 ** 31])
+    loss, counts = balance_loss(z, idx.cuda())
+    want, want_counts = ref_balance(z.double().cpu(), idx, "softmax")
+    assert torch.equal(counts.cpu(), want_counts)
+    close(loss, want, LOSS_TOL)
