@@ -878,7 +878,8 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
         off += (bytes + 255) & ~size_t(255);
         return at;
     };
-    const Shape shape = shape_of(pairs, num_experts, out_features, 128);
+    // a call of no pairs has the shape of a call of one
+    const Shape shape = shape_of(pairs > 0 ? pairs : 1, num_experts, out_features, 128);
     L.cap = shape.cap;
     L.outs = shape.outs;
     L.pitch = (width / kMxBlock + 15) / 16 * 16;

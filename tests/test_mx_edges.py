@@ -174,3 +174,15 @@ def test_narrowed_indices(cuda, count):
     got = K.expert_indices(wide.cuda())
     assert got.dtype == torch.int32
     assert torch.equal(got.cpu().long(), wide.clamp(-2 ** 31, 2 ** 31 - 1))
+
+
+# ------------------------------------------------------------- workspace sizes
+
+
+def test_workspace_of_an_empty_call():
+    """A call of no pairs has a workspace size, and it serves one."""
+    lib = K.library()
+    assert 0 < lib.iqk_mx_workspace_bytes(0, 4, 64, 64) <= lib.iqk_mx_workspace_bytes(1, 4, 64, 64)
+    assert lib.iqk_mx_workspace_bytes(0, 1, 64, 64) > 0
+    x = 0x10000
+    assert lib.iqk_mx_routed(x, 0, 4, 64, x, 0, x, x, 16, 4, 64, 64, x, 0, x, 0, None) == 0
