@@ -246,6 +246,25 @@ class MxSwitchGLU(nn.Module):
         return {"gate": (self.inter, self.hidden), "up": (self.inter, self.hidden),
                 "down": (self.hidden, self.inter)}
 
+    def _lay_out_scales(self) -> None:
+        """Scale rows back on 16-byte boundaries: a copy of a buffer that is a view of
+        wider rows is packed."""
+        for name in self._shapes():
+            scales = self._buffers[f"{name}_scales"]
+            experts, rows, _ = scales.shape
+            outer, step, inner = scales.stride()
+            if inner != 1 or step % 16 or outer != rows * step or scales.data_ptr() % 16:
+                self._buffers[f"{name}_scales"] = mx_aligned_scales(scales)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._lay_out_scales()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out_scales()
+
     def load(self, name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
         """Install one projection's matrices (``gate``, ``up`` or ``down``)."""
         if name not in self._shapes():

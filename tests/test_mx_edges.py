@@ -3,6 +3,9 @@ what happens after an error. Definitions and bounds are those of ``test_mx``."""
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -186,3 +189,59 @@ def test_workspace_of_an_empty_call():
     assert lib.iqk_mx_workspace_bytes(0, 1, 64, 64) > 0
     x = 0x10000
     assert lib.iqk_mx_routed(x, 0, 4, 64, x, 0, x, x, 16, 4, 64, 64, x, 0, x, 0, None) == 0
+
+
+# --------------------------------------------------------- a layer that moves
+
+
+def scale_buffers(layer):
+    return [layer.gate_scales, layer.up_scales, layer.down_scales]
+
+
+def aligned_rows(layer):
+    return all(s.stride(-1) == 1 and s.stride(1) % 16 == 0 and s.stride(1) >= s.shape[2] and
+               s.stride(0) == s.shape[1] * s.stride(1) for s in scale_buffers(layer))
+
+
+def test_scale_rows_keep_their_boundaries_when_a_layer_moves(tmp_path):
+    layer = MxSwitchGLU(2, 2880, 768)  # 90 and 24 scales a row, 96 and 32 bytes apart
+    assert aligned_rows(layer) and layer.gate_scales.stride(1) == 96
+    for scales in scale_buffers(layer):
+        scales.copy_(torch.randint(100, 130, scales.shape, dtype=torch.uint8))
+    want = [s.clone() for s in scale_buffers(layer)]
+
+    def same(other):
+        assert aligned_rows(other)
+        for s, w in zip(scale_buffers(other), want):
+            assert s.shape == w.shape and torch.equal(s, w)
+
+    assert aligned_rows(copy.deepcopy(layer).to("meta"))
+    moved = copy.deepcopy(layer).to("meta").to_empty(device="cpu")
+    assert aligned_rows(moved)
+    moved.load_state_dict(layer.state_dict())
+    same(moved)
+    packed = {k: v.contiguous().clone() for k, v in layer.state_dict().items()}
+    for assign in (False, True):
+        other = MxSwitchGLU(2, 2880, 768)
+        other.load_state_dict(packed, assign=assign)
+        same(other)
+    parent = torch.nn.Sequential(copy.deepcopy(layer)).half().to(torch.bfloat16)
+    same(parent[0])
+    same(pickle.loads(pickle.dumps(layer)))
+    torch.save(layer.state_dict(), tmp_path / "layer.pt")
+    other = MxSwitchGLU(2, 2880, 768)
+    other.load_state_dict(torch.load(tmp_path / "layer.pt"), assign=True)
+    same(other)
+
+
+@pytest.mark.gpu
+def test_a_layer_made_on_the_host_serves_after_cuda(cuda):
+    g = torch.Generator().manual_seed(4)
+    there, here = MxSwitchGLU(3, 96, 160, device="cuda"), MxSwitchGLU(3, 96, 160)
+    for name, shape in (("gate", (3, 160, 96)), ("up", (3, 160, 96)), ("down", (3, 96, 160))):
+        there.load_weights(name, torch.randn(shape, generator=g).cuda())
+        here.load(name, getattr(there, f"{name}_codes").cpu(), getattr(there, f"{name}_scales").cpu())
+    x = torch.randn((5, 96), generator=g).cuda()
+    idx = torch.tensor([[0, 2], [1, 0], [-1, 1], [2, 2], [1, 2]], device="cuda")
+    scores = torch.rand((5, 2), generator=g).cuda()
+    assert torch.equal(here.cuda()(x, idx, scores), there(x, idx, scores))
