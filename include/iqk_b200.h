@@ -547,7 +547,9 @@ int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream
  * one matrix, 64 of a small one). The first 8192 bytes of `state`
  * (iqk_mx_few_state_bytes) must be zero before its first call; each call leaves it ready for the next one on
  * the same stream. Calls that may overlap in time need a state each.
- * iqk_mx_read_error reads its error bits.
+ * iqk_mx_read_error reads its error bits. After IQK_DEVERR_TIMEOUT the state's
+ * counters are lost: later calls are right without them (wide rows slower)
+ * until the 8192 bytes are zero again.
  */
 size_t iqk_mx_few_state_bytes(void);
 

@@ -142,7 +142,8 @@ struct Plan {
     __device__ uint32_t start(uint32_t cta) const { return all * min(cta, runs) / runs; }
 };
 
-__device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles) {
+// join: items may be shared.
+__device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles, bool join) {
     Plan p;
     const uint32_t ctas = gridDim.x;
     p.nblocks = (uint32_t)((a.out_features + a.outs - 1) / a.outs);
@@ -154,7 +155,7 @@ __device__ __forceinline__ Plan make_plan(const ProductArgs &a, int routed_tiles
     // 0.4 us for a CTA that has the memory to itself. A decode step's 96 items
     // of 8 units were done after 13 us when cut to fill all SMs, after 10 whole.
     const uint32_t rest = p.items % ctas, run = (rest * p.units + ctas - 1) / ctas;
-    p.whole = p.units - run < kSaved ? p.items : p.items - rest;
+    p.whole = !join || p.units - run < kSaved ? p.items : p.items - rest;
     // fewer items than CTAs, at most 2^11 units each: 32 bits hold all * runs
     p.all = (p.items - p.whole) * p.units;
     p.runs = max(1u, min(ctas, p.all));
@@ -387,6 +388,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
     int *tile_count = reinterpret_cast<int *>(tmem_slot + 2);
+    int *no_join = reinterpret_cast<int *>(tmem_slot + 3);
     int4 *few_tiles = reinterpret_cast<int4 *>(bars + kBarBytes);
     int32_t *few_pairs = reinterpret_cast<int32_t *>(few_tiles + kFewPairs);
     int32_t *few_rows = few_pairs + kFewPairs * kFewCap;
@@ -422,6 +424,11 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     }
     grid_dep_wait();
     grid_dep_launch();
+    // The state of few rows outlives the call. One whose wait ran out leaves its
+    // error word set and counts parts that never came: until the caller has
+    // cleared both, its calls share no item.
+    if (FEW && threadIdx.x == 0)
+        *no_join = a.width > kSaved * kUnit ? *(volatile int32_t *)(a.hdr + 3) : 0;
     if (FEW && a.sel) {
         if (warp == kScaleWarp) {
             bool bad;
@@ -440,7 +447,8 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
     // columns: two accumulators of `cap`, then the scale buffers, 16 columns
     // a side and buffer (four words a row group, 128 rows)
     const uint32_t scale_col = tmem + 2 * cap;
-    const Plan plan = make_plan(a, !a.tiles ? 0 : FEW ? *tile_count : a.hdr[1]);
+    const Plan plan = make_plan(a, !a.tiles ? 0 : FEW ? *tile_count : a.hdr[1],
+                                !FEW || *no_join == 0);
 
     auto give_up = [&]() {
         if (!*abort_flag) {

@@ -12,7 +12,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from mlx_iqk_b200 import MxSwitchGLU, mx_linear, mx_quantize, mx_switch_linear, route
 from mlx_iqk_b200 import kernels as K
-from test_mx import check_routed, make_matrix, make_x
+from test_mx import check, check_routed, make_matrix, make_x, rounded
 
 
 # ------------------------------------------------------ the layer's arguments
@@ -245,3 +245,39 @@ def test_a_layer_made_on_the_host_serves_after_cuda(cuda):
     idx = torch.tensor([[0, 2], [1, 0], [-1, 1], [2, 2], [1, 2]], device="cuda")
     scores = torch.rand((5, 2), generator=g).cuda()
     assert torch.equal(here.cuda()(x, idx, scores), there(x, idx, scores))
+
+
+# ------------------------------------------------------- after an expired wait
+
+
+def poison(tickets):
+    """The state of the current stream's one-launch calls as a call leaves it whose
+    wait ran out: the error word set, parts of shared items counted that never came."""
+    stream = K.stream_handle(torch.device("cuda", torch.cuda.current_device()))
+    state = K._FEW_STATES[torch.cuda.current_device(), stream]
+    words = state[:8192].view(torch.int32)
+    words[3] = K.DEVERR_TIMEOUT
+    words[64:64 + 8 * 148] = tickets
+    return words
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tickets", [1, 20, -1])
+def test_one_launch_calls_recover_from_an_expired_wait(cuda, tickets):
+    """Rows wide enough that CTAs join parts of an item behind the counters."""
+    codes, scales, w = make_matrix((200, 16384), seed=1)
+    x = make_x((3, 16384), torch.float32, seed=2)
+    mats = make_matrix((5, 70, 8224), seed=3)
+    rows = make_x((4, 1, 1, 8224), torch.float32, seed=4)
+    idx = torch.tensor([[0, 4], [1, 0], [3, -1], [4, 4]])
+    check(mx_linear(x, codes, scales), rounded(x), w, torch.float32)
+    words = poison(tickets)
+    for seed in range(5, 8):  # other inputs: the parts of the call before do not serve
+        x = make_x((3, 16384), torch.float32, seed)
+        rows = make_x((4, 1, 1, 8224), torch.float32, seed)
+        check(mx_linear(x, codes, scales), rounded(x), w, torch.float32)
+        check_routed(mx_switch_linear(rows, idx.cuda(), *mats[:2]), rows, idx, mats[2],
+                     torch.float32)
+    assert int(words[3]) == K.DEVERR_TIMEOUT  # until it is read
+    words.zero_()
+    check(mx_linear(x, codes, scales), rounded(x), w, torch.float32)
