@@ -540,6 +540,16 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
 int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream);
 
 /*
+ * A product whose bounded wait expires (its y is then not complete) also ORs
+ * IQK_DEVERR_TIMEOUT into one word of the device, which outlasts workspaces
+ * and states. iqk_mx_take_errors reads it into *flags, clears it and
+ * synchronises the stream; iqk_mx_error_word gives its device address.
+ */
+int iqk_mx_take_errors(int32_t *flags, iqk_stream_t stream);
+
+int iqk_mx_error_word(int32_t **word);
+
+/*
  * iqk_mx_few: iqk_mx_routed, or with sel NULL iqk_mx_linear (num_experts 1,
  * pairs = x_rows), of few rows in one launch; the same products and f32 sums
  * (a long row's sum may be cut at other columns).

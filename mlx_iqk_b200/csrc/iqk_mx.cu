@@ -449,6 +449,25 @@ int iqk_mx_read_error(const void *workspace, int32_t *flags, iqk_stream_t stream
     return cuda_status(err);
 }
 
+int iqk_mx_error_word(int32_t **word) {
+    if (!word) return IQK_ERR_ARGUMENT;
+    return cuda_status(mx_error_word(word));
+}
+
+int iqk_mx_take_errors(int32_t *flags, iqk_stream_t stream) {
+    if (!flags) return IQK_ERR_ARGUMENT;
+    *flags = 0;
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    int32_t *word = nullptr, value = 0;
+    cudaError_t err = mx_error_word(&word);
+    if (err == cudaSuccess)
+        err = cudaMemcpyAsync(&value, word, sizeof(value), cudaMemcpyDeviceToHost, s);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(s);
+    if (err == cudaSuccess && value) err = cudaMemsetAsync(word, 0, sizeof(value), s);
+    if (err == cudaSuccess) *flags = value;
+    return cuda_status(err);
+}
+
 size_t iqk_mx_few_state_bytes(void) { return mx_few_state_bytes(); }
 
 int iqk_mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,

@@ -54,6 +54,7 @@ struct MxFew {
     char *state;
 };
 
+cudaError_t mx_error_word(int32_t **word);  // on the current device
 size_t mx_few_state_bytes();
 bool mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
                  bool routed);

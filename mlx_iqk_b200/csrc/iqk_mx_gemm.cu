@@ -361,6 +361,10 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, const float 
     else store_columns<__nv_bfloat16, C>(a, v, n, base, lane, out, pairs);
 }
 
+// Error bits of every product on this device, beside those of a call's own
+// workspace or state, which may be gone before anyone reads them.
+__device__ int32_t device_errors;
+
 // FEW: activations of type XT, rounded in the kernel; else from the workspace.
 template <bool FEW, typename XT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -454,6 +458,7 @@ mx_product_kernel(const __grid_constant__ ProductArgs args,
         if (!*abort_flag) {
             *abort_flag = 1;
             atomicOr(a.hdr + 3, IQK_DEVERR_TIMEOUT);
+            atomicOr(&device_errors, IQK_DEVERR_TIMEOUT);
         }
     };
     const uint32_t off_b = (uint32_t)a.outs * 128, off_sb = (uint32_t)a.outs * 16;
@@ -967,6 +972,10 @@ cudaError_t launch_mx_product(const MxProduct &p, cudaStream_t stream, int sms) 
     }
     if (err != cudaSuccess) return err;
     return launch_kernel<false, float>(a, maps, sms, stream);
+}
+
+cudaError_t mx_error_word(int32_t **word) {
+    return cudaGetSymbolAddress(reinterpret_cast<void **>(word), device_errors);
 }
 
 // State of the one-launch product: hdr, tickets, slots.

@@ -185,6 +185,10 @@ def library() -> ctypes.CDLL:
     lib.iqk_mx_few.restype = i32
     lib.iqk_mx_read_error.argtypes = [vp, ctypes.POINTER(ctypes.c_int32), vp]
     lib.iqk_mx_read_error.restype = i32
+    lib.iqk_mx_take_errors.argtypes = [ctypes.POINTER(ctypes.c_int32), vp]
+    lib.iqk_mx_take_errors.restype = i32
+    lib.iqk_mx_error_word.argtypes = [ctypes.POINTER(vp)]
+    lib.iqk_mx_error_word.restype = i32
     _LIB = lib
     return lib
 
@@ -205,6 +209,7 @@ def exported_symbols() -> list[str]:
             "iqk_narrow_indices", "iqk_route", "iqk_balance_workspace_bytes", "iqk_route_balanced",
             "iqk_route_backward", "iqk_mx_quantize", "iqk_mx_dequantize",
             "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error",
+            "iqk_mx_take_errors", "iqk_mx_error_word",
             "iqk_mx_few_state_bytes", "iqk_mx_few_fits", "iqk_mx_few"]
 
 
@@ -774,6 +779,22 @@ def mx_read_error(workspace: torch.Tensor) -> int:
     raise_for_status(library().iqk_mx_read_error(workspace.data_ptr(), ctypes.byref(flags),
                                                  stream_handle(workspace.device)),
                      "iqk_mx_read_error")
+    return int(flags.value)
+
+
+def mx_take_errors(device: torch.device) -> int:
+    """``iqk_mx_take_errors``: the error bits that MXFP4 products left on ``device`` since
+    this was last asked (synchronises the current stream). After an error the states of
+    the one-launch products start anew."""
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    check_current(device)
+    flags = ctypes.c_int32(0)
+    raise_for_status(library().iqk_mx_take_errors(ctypes.byref(flags), stream_handle(device)),
+                     "iqk_mx_take_errors")
+    if flags.value:
+        for key in [k for k in _FEW_STATES if k[0] == device.index]:
+            del _FEW_STATES[key]
     return int(flags.value)
 
 

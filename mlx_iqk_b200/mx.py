@@ -23,6 +23,9 @@ Activations are quantised inside the product, so that both operands are 4-bit
 on the tensor cores; products and sums are float32, rounded once to
 ``out_dtype`` (the activations' type unless given). These are serving
 operators: they carry no gradient and refuse an input that asks for one.
+
+Every wait inside the products is bounded. One that expires leaves the call's
+output incomplete and ``DEVERR_TIMEOUT`` for ``kernels.mx_take_errors(device)``.
 """
 
 from __future__ import annotations

@@ -4,6 +4,7 @@ what happens after an error. Definitions and bounds are those of ``test_mx``."""
 from __future__ import annotations
 
 import copy
+import ctypes
 import pickle
 
 import pytest
@@ -281,3 +282,32 @@ def test_one_launch_calls_recover_from_an_expired_wait(cuda, tickets):
     assert int(words[3]) == K.DEVERR_TIMEOUT  # until it is read
     words.zero_()
     check(mx_linear(x, codes, scales), rounded(x), w, torch.float32)
+
+
+def test_error_entries_refuse_before_any_device_call():
+    lib = K.library()
+    assert lib.iqk_mx_take_errors(None, None) == 4
+    assert lib.iqk_mx_error_word(None) == 4
+
+
+@pytest.mark.gpu
+def test_an_expired_wait_can_be_read_without_a_workspace(cuda):
+    """A wait that nothing satisfies leaves its bit in the device's word, as one inside
+    a product does; reading clears it and drops the states that it may have spoiled."""
+    device = torch.device("cuda", torch.cuda.current_device())
+    codes, scales, w = make_matrix((200, 16384), seed=1)
+    x = make_x((3, 16384), torch.float32, seed=2)
+    want = mx_linear(x, codes, scales)
+    assert K.mx_take_errors(device) == 0
+    assert torch.equal(mx_linear(x, codes, scales), want)  # the state was kept
+    words, stream = poison(20), K.stream_handle(device)
+    word = ctypes.c_void_p()
+    assert K.library().iqk_mx_error_word(ctypes.byref(word)) == 0
+    assert K.library().iqk_check_bounded_wait(1_000_000, word, stream) == 0
+    assert K.mx_take_errors(device) == K.DEVERR_TIMEOUT
+    assert K.mx_take_errors(torch.device("cuda")) == 0
+    assert torch.equal(mx_linear(x, codes, scales), want)
+    fresh = K._FEW_STATES[device.index, stream]
+    assert fresh.data_ptr() != words.data_ptr() and int(fresh[:8192].view(torch.int32)[3]) == 0
+    with pytest.raises(K.IqkRuntimeError):
+        K.mx_take_errors(torch.device("cpu"))
