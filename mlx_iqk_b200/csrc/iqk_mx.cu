@@ -128,12 +128,19 @@ mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restric
 // it counts its pairs by expert (counting hands out the ranks, so that the
 // second pass needs no atomics), reads the other CTAs' counts, and gives each
 // of its pairs its place behind those of the CTAs before it. Pairs without an
-// expert go to the tail of `order` and have place -1. The order of an expert's
-// pairs changes no result: each is a row of its own. CTA 0 cuts each expert's
+// expert go to the tail of `order` and have place -1. CTA 0 cuts each expert's
 // run into tiles of at most L.cap rows. Latency bounds it: one CTA took 14 us
 // for 12288 pairs, most of it in shared-memory atomics.
+//
+// Each pair is a row of its own, so its tile changes no result as long as every
+// item is summed whole; the atomics' order may then decide it. Where items can
+// be shared (mx_may_join), tiles are cut at different columns and the row's f32
+// sum depends on its tile: there ranks are handed out in the pairs' order
+// (STABLE), so that a result repeats bit for bit; 12288 pairs take 4 us longer
+// (of 167 us: 8192 columns, 2048 outputs, 64 experts).
 constexpr int kSortCtas = 8;
 
+template <bool STABLE>
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(1024)
 mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLayout L,
                char *ws) {
@@ -166,7 +173,44 @@ mx_sort_kernel(const int32_t *__restrict__ sel, int pairs, int num_experts, MxLa
     auto is_expert = [&](int e) { return e >= 0 && e < num_experts; };
     int stray = 0;
     __syncthreads();
-    for (int p = p0 + 4 * tid; p < p1; p += 4 * nt) {
+    if constexpr (STABLE) {
+        // A thread a pair: the warps find each pair's mates among their 32, and
+        // warp 0 hands out the ranks, warp after warp.
+        constexpr uint32_t kAll = 0xffffffffu;
+        __shared__ int32_t bucket[1024];  // a pair's, then the rank of its first mate
+        __shared__ uint32_t mates[1024];
+        for (int p = p0; p < p1; p += 1024) {
+            const int q = p + tid;
+            const bool there = q < p1;
+            const int v = there ? sel[q] : -1;
+            const int b = is_expert(v) ? v : num_experts;
+            stray |= b == num_experts && v != -1;
+            const uint32_t same = __match_any_sync(kAll, b) & __ballot_sync(kAll, there);
+            bucket[tid] = b;
+            mates[tid] = there ? same : 0u;
+            __syncthreads();
+            for (int w = 0; wid == 0 && w < min(32, (p1 - p + 31) / 32); w += 8) {
+                int e[8];
+                uint32_t m[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    e[j] = bucket[32 * (w + j) + lane];
+                    m[j] = mates[32 * (w + j) + lane];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int first = cnt[e[j]];
+                    __syncwarp();
+                    if (lane == __ffs(m[j]) - 1) cnt[e[j]] = first + __popc(m[j]);
+                    bucket[32 * (w + j) + lane] = first;
+                    __syncwarp();
+                }
+            }
+            __syncthreads();
+            if (there) place[q] = bucket[tid] + __popc(same & ((1u << lane) - 1u));
+        }
+    }
+    for (int p = p0 + 4 * tid; !STABLE && p < p1; p += 4 * nt) {
         int e[4];
         buckets(p, e);
         int4 ranks = make_int4(0, 0, 0, 0);
@@ -425,8 +469,13 @@ int iqk_mx_routed(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride
     if (!mx_items_ok(p)) return IQK_ERR_GEOMETRY;
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int sms = num_sms_current();
-    mx_sort_kernel<<<kSortCtas, 1024, sizeof(int32_t) * (size_t)(num_experts + 1), s>>>(
-        sel, (int)pairs, (int)num_experts, p.L, p.ws);
+    const size_t counts = sizeof(int32_t) * (size_t)(num_experts + 1);
+    if (mx_may_join(width))
+        mx_sort_kernel<true><<<kSortCtas, 1024, counts, s>>>(sel, (int)pairs, (int)num_experts,
+                                                             p.L, p.ws);
+    else
+        mx_sort_kernel<false><<<kSortCtas, 1024, counts, s>>>(sel, (int)pairs, (int)num_experts,
+                                                              p.L, p.ws);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return cuda_status(err);
     err = launch_mx_quantize(x, x_dtype, x_rows, width, row_stride,

@@ -25,6 +25,9 @@ struct MxLayout {
     __host__ __device__ int zeroed() const { return (int)((order - hdr) / 4); }  // words that start at 0
 };
 
+// Rows of this width are wide enough that CTAs may share an item and join its parts.
+bool mx_may_join(int64_t width);
+
 MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t out_features);
 
 // One call of the product: pairs sorted by expert (order and tiles), or, for a

@@ -53,7 +53,8 @@
 // matrix in L2. The CTAs take items in turn. Where the last round would leave many of
 // them idle over a wide matrix, its items are cut into equal runs of units, and
 // the parts of an item meet in f32 slots of the workspace: the last CTA to
-// finish adds them in order, so results repeat bit for bit.
+// finish adds them in order. Routed pairs of such widths are sorted in their own
+// order, so that a pair is in the same tile each time: results repeat bit for bit.
 //
 // The kernel is a programmatic dependent launch: barriers and tensor memory are
 // set up while the kernel before it drains (1.5 us off each call in a row).
@@ -882,6 +883,10 @@ Shape shape_of(int64_t pairs, int64_t experts, int64_t out_features, int most) {
 }
 
 }  // namespace
+
+// A round's share of an item is a unit at least, so what sharing saves is below
+// the item's units (make_plan).
+bool mx_may_join(int64_t width) { return width > (int64_t)kSaved * kUnit; }
 
 MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t out_features) {
     MxLayout L{};

@@ -11,7 +11,8 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from mlx_iqk_b200 import MxSwitchGLU, mx_linear, mx_quantize, mx_switch_linear, route
+from mlx_iqk_b200 import (MxSwitchGLU, mx_dequantize, mx_linear, mx_quantize, mx_switch_linear,
+                          route)
 from mlx_iqk_b200 import kernels as K
 from test_mx import check, check_routed, make_matrix, make_x, rounded
 
@@ -311,3 +312,62 @@ def test_an_expired_wait_can_be_read_without_a_workspace(cuda):
     assert fresh.data_ptr() != words.data_ptr() and int(fresh[:8192].view(torch.int32)[3]) == 0
     with pytest.raises(K.IqkRuntimeError):
         K.mx_take_errors(torch.device("cpu"))
+
+
+# ---------------------------------------------------------- results that repeat
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,experts,width,out", [(1280, 4, 4, 16384, 64), (600, 2, 3, 16384, 300),
+                                                   (700, 3, 5, 12320, 130), (45, 2, 2, 8224, 33)])
+def test_wide_routed_calls_repeat_bit_for_bit(cuda, t, k, experts, width, out):
+    """An expert has several tiles whose sums are cut at different columns. Blocks of
+    sizes from 2^-20 to 2^20 make every f32 sum depend on where it is cut."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    codes, scales = mx_quantize(torch.randn((experts, out, width), generator=g, device="cuda"))
+    size = torch.randint(-20, 21, (t, 1, 1, width // 32), generator=g, device="cuda")
+    x = torch.randn((t, 1, 1, width), generator=g, device="cuda") * \
+        torch.exp2(size.float()).repeat_interleave(32, -1)
+    idx = torch.stack([torch.randperm(experts, generator=g, device="cuda")[:k]
+                       for _ in range(t)]).int()
+    idx[::7, 0] = -1
+    idx[5, 0] = experts + 3
+    y = mx_switch_linear(x, idx, codes, scales)
+    for _ in range(12):
+        assert torch.equal(mx_switch_linear(x, idx, codes, scales), y)
+    # each pair against its own row through its own matrix, in 64 bits
+    xq, w = mx_dequantize(*mx_quantize(x)).double().view(t, width), mx_dequantize(codes, scales)
+    for e in range(experts):
+        tt, jj = (idx == e).nonzero(as_tuple=True)
+        want = xq[tt] @ w[e].double().t()
+        room = xq[tt].abs() @ w[e].double().abs().t()
+        err = (y[tt, jj, 0].double() - want).abs()
+        assert (err <= (width / 64 + 8) * 2.0 ** -23 * room * (1 + 2.0 ** -24) +
+                2.0 ** -24 * want.abs()).all()
+    assert (y[(idx < 0) | (idx >= experts)] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,experts", [(33, 4096), (1030, 4096), (5000, 3), (257, 1)])
+def test_wide_routed_sort(cuda, t, experts):
+    """Counting in the pairs' order: many experts, few, stray indices, odd counts; the
+    indices begin off 16-byte boundaries."""
+    width = 8192
+    codes = torch.randint(0, 256, (experts, 1, width // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.full((experts, 1, width // 32), 122, dtype=torch.uint8, device="cuda")
+    g = torch.Generator().manual_seed(t)
+    flat = torch.randint(-2, experts + 2, (3 * t + 1,), generator=g).int().cuda()
+    idx = flat[1:].view(t, 3)
+    x = make_x((1, 1, 1, width), torch.bfloat16, seed=t)
+    ws = torch.empty(K.mx_workspace_bytes(3 * t, experts, width, 1), dtype=torch.uint8,
+                     device="cuda")
+    y = mx_switch_linear(x, idx, codes, scales, torch.float32, workspace=ws)
+    assert K.mx_read_error(ws) == (K.DEVERR_EXPERT if ((idx < -1) | (idx >= experts)).any() else 0)
+    xq = mx_dequantize(*mx_quantize(x)).double().view(width)
+    w = mx_dequantize(codes, scales).double().view(experts, width)
+    want, room = w @ xq, w.abs() @ xq.abs()
+    here = (idx >= 0) & (idx < experts)
+    assert (y.view(t, 3)[~here] == 0).all()
+    pick = idx[here].long()
+    err = (y.view(t, 3)[here].double() - want[pick]).abs()
+    assert (err <= (width / 64 + 8) * 2.0 ** -23 * room[pick] * 1.001).all()
