@@ -17,7 +17,7 @@ constexpr int kMxBlock = 32;  // values under one scale
 //   tiles  [max_tiles] int4: {expert, first position, rows (<= cap), 0}
 //   codes  [pairs, width / 2], scales [pairs, pitch]: the activations in
 //          sorted order
-//   slots  f32: shared items' parts
+//   slots  f32: shared items' parts (wide rows only)
 struct MxLayout {
     size_t hdr, tickets, order, place, tiles, codes, scales, slots, total;
     int64_t max_tiles, pitch;

@@ -909,7 +909,7 @@ MxLayout mx_layout(int64_t pairs, int64_t num_experts, int64_t width, int64_t ou
     L.tiles = take(16 * (size_t)L.max_tiles);
     L.codes = take((size_t)pairs * (size_t)(width / 2));
     L.scales = take((size_t)pairs * (size_t)L.pitch);
-    L.slots = take(sizeof(float) * 2 * kMaxCtas * kOuts * (size_t)L.cap);
+    L.slots = take(mx_may_join(width) ? sizeof(float) * 2 * kMaxCtas * kOuts * (size_t)L.cap : 0);
     L.total = off;
     return L;
 }

@@ -371,3 +371,19 @@ def test_wide_routed_sort(cuda, t, experts):
     pick = idx[here].long()
     err = (y.view(t, 3)[here].double() - want[pick]).abs()
     assert (err <= (width / 64 + 8) * 2.0 ** -23 * room[pick] * 1.001).all()
+
+
+# ------------------------------------------------------------------ memory held
+
+
+@pytest.mark.parametrize("pairs,experts,width,out", [(128, 1, 4096, 512), (4096, 1, 4096, 8192),
+                                                     (12288, 256, 4096, 2048), (70, 4, 7168, 64)])
+def test_workspace_holds_what_the_call_uses(pairs, experts, width, out):
+    """Codes and scales of the rows, four words a pair, tiles and counters: no parts of
+    shared items for rows that are never shared (up to 7168 columns)."""
+    need = K.mx_workspace_bytes(pairs, experts, width, out)
+    rows = pairs * (width // 2 + (width // 32 + 15) // 16 * 16)
+    tiles = 16 * (min(experts, pairs) + pairs // 16 + 1)
+    assert need <= rows + 16 * pairs + tiles + (16 << 10)
+    wide = K.mx_workspace_bytes(pairs, experts, 7200, out)
+    assert wide > pairs * (3600 + 240) + 4 * 2 * 148 * 128 * 16
