@@ -563,6 +563,11 @@ int iqk_mx_error_word(int32_t **word);
  */
 size_t iqk_mx_few_state_bytes(void);
 
+/* What a call of this width needs of it: 256 bytes where it shares no item (up
+ * to 7168 columns), and those need not be zero (iqk_mx_read_error then reads
+ * what was there). */
+size_t iqk_mx_few_state_bytes_for(int64_t width);
+
 int iqk_mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
                     int routed);
 

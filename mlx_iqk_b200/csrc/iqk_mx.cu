@@ -517,7 +517,9 @@ int iqk_mx_take_errors(int32_t *flags, iqk_stream_t stream) {
     return cuda_status(err);
 }
 
-size_t iqk_mx_few_state_bytes(void) { return mx_few_state_bytes(); }
+size_t iqk_mx_few_state_bytes(void) { return mx_few_state_bytes(1 << 20); }
+
+size_t iqk_mx_few_state_bytes_for(int64_t width) { return mx_few_state_bytes(width); }
 
 int iqk_mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
                     int routed) {
@@ -543,7 +545,7 @@ int iqk_mx_few(const void *x, int x_dtype, int64_t x_rows, int64_t row_stride, c
     if (!y || !state) return IQK_ERR_ARGUMENT;
     if (!aligned(y, element(y_dtype)) || !aligned(state, 256) || !aligned(sel, 4))
         return IQK_ERR_ALIGNMENT;
-    if (state_bytes < mx_few_state_bytes()) return IQK_ERR_WORKSPACE;
+    if (state_bytes < mx_few_state_bytes(width)) return IQK_ERR_WORKSPACE;
     const MxFew p{x, x_dtype, x_rows, row_stride, sel, pairs, codes, scales, scale_stride,
                   num_experts, out_features, width, y, y_dtype, static_cast<char *>(state)};
     return cuda_status(launch_mx_few(p, reinterpret_cast<cudaStream_t>(stream),

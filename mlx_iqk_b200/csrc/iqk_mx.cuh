@@ -58,7 +58,7 @@ struct MxFew {
 };
 
 cudaError_t mx_error_word(int32_t **word);  // on the current device
-size_t mx_few_state_bytes();
+size_t mx_few_state_bytes(int64_t width);
 bool mx_few_fits(int64_t pairs, int64_t num_experts, int64_t out_features, int64_t width,
                  bool routed);
 cudaError_t launch_mx_few(const MxFew &p, cudaStream_t stream, int sms);

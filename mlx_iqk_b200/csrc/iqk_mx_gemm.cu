@@ -989,7 +989,8 @@ constexpr size_t kStateSlots = kStateTickets + (sizeof(int32_t) * 8 * kMaxCtas +
 
 static_assert(kStateSlots <= 8192, "the caller clears 8192 bytes");
 
-size_t mx_few_state_bytes() {
+size_t mx_few_state_bytes(int64_t width) {
+    if (!mx_may_join(width)) return kStateTickets;  // no item is shared
     return kStateSlots + sizeof(float) * 2 * kMaxCtas * kOuts * kFewCap;
 }
 

@@ -179,6 +179,8 @@ def library() -> ctypes.CDLL:
     lib.iqk_mx_routed.restype = i32
     lib.iqk_mx_few_state_bytes.argtypes = []
     lib.iqk_mx_few_state_bytes.restype = sz
+    lib.iqk_mx_few_state_bytes_for.argtypes = [i64]
+    lib.iqk_mx_few_state_bytes_for.restype = sz
     lib.iqk_mx_few_fits.argtypes = [i64, i64, i64, i64, i32]
     lib.iqk_mx_few_fits.restype = i32
     lib.iqk_mx_few.argtypes = lib.iqk_mx_routed.argtypes
@@ -210,7 +212,7 @@ def exported_symbols() -> list[str]:
             "iqk_route_backward", "iqk_mx_quantize", "iqk_mx_dequantize",
             "iqk_mx_workspace_bytes", "iqk_mx_linear", "iqk_mx_routed", "iqk_mx_read_error",
             "iqk_mx_take_errors", "iqk_mx_error_word",
-            "iqk_mx_few_state_bytes", "iqk_mx_few_fits", "iqk_mx_few"]
+            "iqk_mx_few_state_bytes", "iqk_mx_few_state_bytes_for", "iqk_mx_few_fits", "iqk_mx_few"]
 
 
 def check_bounded_wait(limit_ns: int, device: torch.device) -> int:
@@ -689,20 +691,24 @@ def mx_few_fits(pairs: int, num_experts: int, out_features: int, width: int, rou
 _FEW_STATES: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def mx_few_state(device: torch.device, stream: int) -> torch.Tensor:
+def mx_few_state(device: torch.device, stream: int, width: int) -> torch.Tensor:
     """Zeroed state of the one-launch product, kept per device and stream (stream
-    order keeps a call after the one before); fresh under graph capture, where
-    its clearing is part of the graph."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    state = None if capturing else _FEW_STATES.get((device.index, stream))
+    order keeps a call after the one before). Under graph capture a fresh one of
+    what the call uses; where it counts parts, its clearing is part of the graph."""
+    if torch.cuda.is_current_stream_capturing():
+        need = int(library().iqk_mx_few_state_bytes_for(width))
+        state = torch.empty(need, dtype=torch.uint8, device=device)
+        if need > 8192:
+            state[:8192].zero_()
+        return state
+    state = _FEW_STATES.get((device.index, stream))
     if state is None:
         state = torch.empty(int(library().iqk_mx_few_state_bytes()), dtype=torch.uint8,
                             device=device)
         state[:8192].zero_()
-        if not capturing:
-            if len(_FEW_STATES) >= 64:
-                _FEW_STATES.clear()
-            _FEW_STATES[device.index, stream] = state
+        if len(_FEW_STATES) >= 64:
+            _FEW_STATES.clear()
+        _FEW_STATES[device.index, stream] = state
     return state
 
 
@@ -711,7 +717,7 @@ def mx_few(x: torch.Tensor, rows: int, row_stride: int, sel, pairs: int, codes: 
            y: torch.Tensor) -> None:
     """``iqk_mx_few``: the product of few rows; ``sel`` None for one matrix."""
     stream = stream_handle(y.device)
-    state = mx_few_state(y.device, stream)
+    state = mx_few_state(y.device, stream, x.shape[-1])
     status = library().iqk_mx_few(
         x.data_ptr(), DTYPE_IDS[x.dtype], rows, row_stride, _ptr(sel), pairs, codes.data_ptr(),
         scales.data_ptr(), scale_stride, experts, out_features, x.shape[-1], y.data_ptr(),

@@ -10,6 +10,7 @@ import pickle
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from mlx_iqk_b200 import (MxSwitchGLU, mx_dequantize, mx_linear, mx_quantize, mx_switch_linear,
                           route)
@@ -387,3 +388,51 @@ def test_workspace_holds_what_the_call_uses(pairs, experts, width, out):
     assert need <= rows + 16 * pairs + tiles + (16 << 10)
     wide = K.mx_workspace_bytes(pairs, experts, 7200, out)
     assert wide > pairs * (3600 + 240) + 4 * 2 * 148 * 128 * 16
+
+
+def test_state_of_one_launch_calls():
+    lib = K.library()
+    full = lib.iqk_mx_few_state_bytes()
+    assert lib.iqk_mx_few_state_bytes_for(7168) == 256
+    assert lib.iqk_mx_few_state_bytes_for(7200) == full > 8192
+    x = 0x10000
+
+    def few(width, state_bytes):
+        return lib.iqk_mx_few(x, 0, 2, width, None, 2, x, x, 1024, 1, 64, width, x, 0, x,
+                              state_bytes, None)
+
+    assert few(7168, 255) == 6 and few(7200, full - 1) == 6 and few(7200, 256) == 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width,cleared", [(1024, 0), (8224, 1)])
+def test_captured_one_launch_calls_allocate_and_clear_no_more_than_they_use(cuda, width, cleared):
+    codes, scales, w = make_matrix((3, 64, width), seed=1)
+    x = make_x((2, 1, 1, width), torch.bfloat16, seed=2)
+    idx = torch.tensor([[0, 2], [1, 0]], dtype=torch.int32, device="cuda")
+
+    def step():
+        return mx_switch_linear(x, idx, codes, scales), mx_linear(x, codes[1], scales[1])
+
+    step()
+    seen = []
+
+    class Ops(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            seen.append((func.overloadpacket.__name__,
+                         out.numel() if isinstance(out, torch.Tensor) else 0))
+            return out
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), Ops():
+        y, z = step()
+    names = [n for n, _ in seen]
+    assert names.count("zero_") + names.count("fill_") == 2 * cleared
+    if not cleared:
+        assert all(n <= 1024 for name, n in seen if "empty" in name)
+    x.copy_(make_x(x.shape, torch.bfloat16, seed=3))
+    for _ in range(2):
+        graph.replay()
+        check_routed(y, x, idx.cpu(), w, torch.bfloat16)
+        check(z.view(2, 64), rounded(x).reshape(2, width), w[1], torch.bfloat16)
