@@ -610,11 +610,11 @@ def route(rows: torch.Tensor, mask, top_k: int, scoring: int, renormalize: bool,
 
 
 def route_balanced(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
-                   renormalize: bool, scale: float, indices=None):
+                   renormalize: bool, scale: float, indices=None, keep_slope: bool = False):
     """``iqk_route_balanced``: ``(indices, weights, loss, counts, slope)``. With
-    ``indices`` given (a choice already made) weights are None. ``slope``, which
-    the backward call reads, is a (pointer, owner) pair: it lies in the call's
-    workspace, one allocation for both."""
+    ``indices`` given (a choice already made) weights are None. ``slope``
+    [segments, experts], which the backward call reads, is a tensor of its own when it
+    is to be kept, so that the workspace is not; else None, and lies in the workspace."""
     dev = rows.device
     tokens, experts = rows.shape
     segments = 1 if offsets is None else offsets.numel() - 1
@@ -623,18 +623,21 @@ def route_balanced(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
         indices = rows.new_empty((tokens, top_k), dtype=torch.int32)
         weights = rows.new_empty((tokens, top_k), dtype=torch.float32)
     need = balance_workspace_bytes(tokens, experts, segments)
-    ws = rows.new_empty(need + 4 * segments * experts, dtype=torch.uint8)
+    slope, extra = None, 4 * segments * experts
+    if keep_slope:
+        slope, extra = rows.new_empty((segments, experts), dtype=torch.float32), 0
+    ws = rows.new_empty(need + extra, dtype=torch.uint8)
     loss = rows.new_empty((), dtype=torch.float32)
     counts = rows.new_empty((segments, experts), dtype=torch.int32)
     base = ws.data_ptr()
     status = library().iqk_route_balanced(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         _ptr(offsets), segments, top_k, scoring, renormalize, scale, indices.data_ptr(),
-        _ptr(weights), loss.data_ptr(), counts.data_ptr(), base + need, base, need,
-        stream_handle(dev))
+        _ptr(weights), loss.data_ptr(), counts.data_ptr(),
+        slope.data_ptr() if keep_slope else base + need, base, need, stream_handle(dev))
     if status:
         raise_for_status(status, "iqk_route_balanced")
-    return indices, weights, loss, counts, (base + need, ws)
+    return indices, weights, loss, counts, slope
 
 
 def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
@@ -650,8 +653,8 @@ def route_backward(rows: torch.Tensor, mask, offsets, top_k: int, scoring: int,
     status = library().iqk_route_backward(
         rows.data_ptr(), DTYPE_IDS[rows.dtype], tokens, experts, rows.stride(0), _ptr(mask),
         _ptr(offsets), 1 if offsets is None else offsets.numel() - 1, top_k, scoring, renormalize,
-        scale, indices.data_ptr(), _ptr(grad_weights), slope[0] if slope else None,
-        _ptr(grad_loss), grad.data_ptr(), stream_handle(rows.device))
+        scale, indices.data_ptr(), _ptr(grad_weights), _ptr(slope), _ptr(grad_loss),
+        grad.data_ptr(), stream_handle(rows.device))
     if status:
         raise_for_status(status, "iqk_route_backward")
     return grad

@@ -89,7 +89,7 @@ class _Route(torch.autograd.Function):
         choose = indices is None
         if balance:
             indices, weights, loss, counts, ctx.slope = K.route_balanced(
-                rows, mask, offsets, *call, indices)
+                rows, mask, offsets, *call, indices, True)
             ctx.mark_non_differentiable(*((indices, counts) if choose else (counts,)))
         else:
             indices, weights = K.route(rows, mask, *call)
