@@ -436,3 +436,71 @@ def test_captured_one_launch_calls_allocate_and_clear_no_more_than_they_use(cuda
         graph.replay()
         check_routed(y, x, idx.cpu(), w, torch.bfloat16)
         check(z.view(2, 64), rounded(x).reshape(2, width), w[1], torch.bfloat16)
+
+
+# ------------------------------------- layouts, and more items than run at once
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [9, 40, 700])
+def test_indices_off_16_byte_boundaries(cuda, t):
+    codes, scales, w = make_matrix((6, 70, 96), seed=t)
+    x = make_x((t, 1, 1, 96), torch.float32, seed=t)
+    flat = torch.randint(-1, 6, (3 * t + 3,), generator=torch.Generator().manual_seed(t)).int()
+    for start in (1, 2, 3):
+        idx = flat.cuda()[start:start + 3 * t].view(t, 3)
+        assert idx.is_contiguous() and idx.data_ptr() % 16
+        check_routed(mx_switch_linear(x, idx, codes, scales), x, idx.cpu(), w, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [5, 40, 300])
+def test_products_of_one_row_seen_many_times(cuda, dtype, rows):
+    codes, scales, w = make_matrix((3, 130, 544), seed=rows)
+    one = make_x((1, 544), dtype, seed=rows)
+    x = one.expand(rows, 544)
+    assert x.stride(0) == 0
+    y = mx_linear(x, codes[1], scales[1])
+    check(y, rounded(x), w[1], dtype)
+    idx = torch.arange(2 * rows).view(rows, 2) % 3
+    many = x.view(rows, 1, 1, 544)
+    check_routed(mx_switch_linear(many, idx.cuda(), codes, scales), many, idx, w, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width", [(torch.bfloat16, 1013, 10016), (torch.float16, 997, 12000),
+                                              (torch.float32, 1501, 4128)])
+def test_streams_of_many_items(cuda, dtype, rows, width):
+    """Each thread takes several items, at rows and columns that its step does not
+    divide: the same codes, scales and values as in calls of a few rows."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, width), generator=g, device="cuda") * \
+        torch.exp(torch.randn((rows, 1), generator=g, device="cuda"))
+    x = x.to(dtype)
+    codes, scales = mx_quantize(x)
+    back = {out: mx_dequantize(codes, scales, out) for out in (torch.float32, torch.bfloat16)}
+    for at in range(0, rows, 100):
+        c, s = mx_quantize(x[at:at + 100])
+        assert torch.equal(codes[at:at + 100], c) and torch.equal(scales[at:at + 100], s)
+        for out, values in back.items():
+            assert torch.equal(values[at:at + 100], mx_dequantize(c, s, out))
+
+
+@pytest.mark.gpu
+def test_streams_past_32_bit_items(cuda):
+    """2^31 items and more: one row seen 8.4 million times, each the same codes."""
+    width, rows = 4096, (1 << 31) // 256 + 3
+    if torch.cuda.mem_get_info()[1] < 120 << 30:
+        pytest.skip("90 GB of device memory")
+    one = make_x((1, width), torch.bfloat16, seed=1)
+    want_codes, want_scales = mx_quantize(one)
+    codes, scales = mx_quantize(one.expand(rows, width))
+    back = mx_dequantize(codes, scales, torch.bfloat16)
+    want = mx_dequantize(want_codes, want_scales, torch.bfloat16)
+    for at in range(0, rows, 1 << 20):
+        cut = slice(at, at + (1 << 20))
+        assert (codes[cut] == want_codes).all() and (scales[cut] == want_scales).all()
+        assert (back[cut].view(torch.int16) == want.view(torch.int16)).all()
+    del codes, scales, back
+    torch.cuda.empty_cache()
