@@ -446,8 +446,10 @@ int iqk_dense_gemv(int member, const void *x, int64_t tokens, const void *const 
  *   loss = mean over segments with rows of sum_e f_ge P_ge,
  *   f_ge = num_experts count_ge / (top_k N_g),  P_ge = mean over rows of s_te,
  * s_te the score normalised over the experts and N_g the segment's rows that
- * the mask keeps. offsets [segments + 1] int32 on the device (not falling,
- * from 0 to tokens) cuts the rows into segments; NULL is one segment. With
+ * the mask keeps and that have a logit above -inf (or NaN). offsets
+ * [segments + 1] int32 on the device (not falling) cuts the rows into
+ * segments; rows before the first and from the last one on are routed and
+ * counted nowhere. NULL is one segment of all rows. With
  * weights NULL the choice is the caller's: indices is read, entries outside
  * [0, num_experts) count for no expert. slope [segments, num_experts] is kept
  * for the backward call. workspace: iqk_balance_workspace_bytes. Sums are

@@ -16,7 +16,7 @@
 //   loss = mean over segments g with N_g > 0 of sum_e f_ge P_ge
 //
 // A segment is a run of rows (packed sequences); N_g counts its rows that the
-// mask keeps and that have a finite logit. Gradients, with h_e = 1 (softmax)
+// mask keeps and that have a logit above -inf (or NaN). A row may be in none. Gradients, with h_e = 1 (softmax)
 // or 1 - sigmoid(z_e), a_e = dloss f_ge / (N_g G'), q = w / scale and g the
 // weights' gradient:
 //

@@ -157,13 +157,14 @@ def route_balanced(logits, top_k: int, *, scoring: str = "softmax", renormalize:
 def balance_loss(logits, indices, *, scoring: str = "softmax", mask=None, offsets=None):
     """``(loss, counts)`` of a choice ``indices [..., top_k]``.
 
-    Per segment ``g`` with ``N`` tokens, ``f_e = experts * counts_e / (top_k * N)``
+    Per segment ``g`` with ``N`` tokens (those that the mask leaves out, or that have
+    no logit above ``-inf``, do not count), ``f_e = experts * counts_e / (top_k * N)``
     and ``P_e`` the mean over its tokens of the score normalised over the
     experts; the loss is the mean over the segments that hold a token of
     ``sum_e f_e P_e`` (1 when the experts are used evenly). ``offsets`` (int32
-    ``[segments + 1]`` on the GPU, not falling, from 0 to the token count) cuts
-    the tokens, flattened, into segments, as packed sequences do; None is one
-    segment. ``counts`` is int32 ``[segments, experts]``; entries of
+    ``[segments + 1]`` on the GPU, not falling) cuts the tokens, flattened, into
+    segments, as packed sequences do; tokens before the first offset and from the last
+    on are in none. None is one segment of all. ``counts`` is int32 ``[segments, experts]``; entries of
     ``indices`` outside the experts count for none. Differentiable in
     ``logits`` through the mean scores (a count has no gradient).
     """
