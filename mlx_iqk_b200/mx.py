@@ -256,7 +256,8 @@ class MxSwitchGLU(nn.Module):
             scales = self._buffers[f"{name}_scales"]
             experts, rows, _ = scales.shape
             outer, step, inner = scales.stride()
-            if inner != 1 or step % 16 or outer != rows * step or scales.data_ptr() % 16:
+            if inner != 1 or step % 16 or outer != rows * step \
+                    or scales.storage_offset() % 16:
                 self._buffers[f"{name}_scales"] = mx_aligned_scales(scales)
 
     def _apply(self, fn, recurse=True):

@@ -504,3 +504,21 @@ def test_streams_past_32_bit_items(cuda):
         assert (back[cut].view(torch.int16) == want.view(torch.int16)).all()
     del codes, scales, back
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k,experts,width,out", [(1280, 4, 4, 4096, 64), (600, 2, 3, 7168, 300),
+                                                   (3000, 3, 5, 2080, 130)])
+def test_routed_calls_repeat_bit_for_bit(cuda, t, k, experts, width, out):
+    """Which of an expert's tiles a pair is in may differ from call to call, and changes
+    no result: every item of such widths is summed whole."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    codes, scales = mx_quantize(torch.randn((experts, out, width), generator=g, device="cuda"))
+    size = torch.randint(-20, 21, (t, 1, 1, width // 32), generator=g, device="cuda")
+    x = torch.randn((t, 1, 1, width), generator=g, device="cuda") * \
+        torch.exp2(size.float()).repeat_interleave(32, -1)
+    idx = torch.stack([torch.randperm(experts, generator=g, device="cuda")[:k]
+                       for _ in range(t)]).int()
+    y = mx_switch_linear(x, idx, codes, scales)
+    for _ in range(12):
+        assert torch.equal(mx_switch_linear(x, idx, codes, scales), y)
