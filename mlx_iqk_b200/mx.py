@@ -108,8 +108,8 @@ def _check_matrix(codes, scales, dims, device):
         raise IqkRuntimeError("codes must be contiguous and 16-byte aligned")
     steps = scales.stride()
     stride, step, packed = (blocks + 15) // 16 * 16, None, blocks == 1 or steps[-1] == 1
-    for axis in range(len(lead) - 2, -1, -1):  # one row, or no axis longer than 1: any stride
-        if lead[axis] == 1:
+    for axis in range(len(lead) - 2, -1, -1):  # one row or none: any stride
+        if lead[axis] == 1 or scales.numel() == 0:
             continue
         if step is None:
             stride = step = steps[axis]

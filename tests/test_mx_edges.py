@@ -522,3 +522,15 @@ def test_routed_calls_repeat_bit_for_bit(cuda, t, k, experts, width, out):
     y = mx_switch_linear(x, idx, codes, scales)
     for _ in range(12):
         assert torch.equal(mx_switch_linear(x, idx, codes, scales), y)
+
+
+@pytest.mark.gpu
+def test_matrices_without_outputs(cuda):
+    """No rows have no layout to refuse, whatever strides the empty tensor has."""
+    codes, scales, _ = make_matrix((3, 32, 64), seed=2)
+    x = make_x((2, 1, 1, 64), torch.float32, seed=1)
+    idx = torch.tensor([[0, 2], [2, -1]], device="cuda")
+    for c, s in ((codes[:, :0], scales[:, :0]),
+                 (codes[:, :0].contiguous(), scales[:, :0].contiguous())):
+        assert mx_switch_linear(x, idx, c, s).shape == (2, 2, 1, 0)
+        assert mx_dequantize(c, s).shape == (3, 0, 64)
