@@ -516,7 +516,8 @@ int iqk_route_backward(const void *logits, int dtype, int64_t tokens, int64_t nu
  * top_k pairs of a token, or one row per pair). sel -1 is no expert: its row
  * of y is zeros. Another index outside [0, num_experts) also gives zeros, and
  * sets IQK_DEVERR_EXPERT in the workspace (iqk_mx_read_error, which
- * synchronises the stream). At most 4096 experts and 2^24 pairs.
+ * synchronises the stream; a call without pairs leaves the workspace as it
+ * was). At most 4096 experts and 2^24 pairs.
  */
 int iqk_mx_quantize(const void *x, int dtype, int64_t rows, int64_t width, int64_t row_stride,
                     uint8_t *codes, uint8_t *scales, int64_t scale_stride, iqk_stream_t stream);

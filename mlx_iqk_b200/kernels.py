@@ -780,6 +780,17 @@ def mx_routed(x: torch.Tensor, rows: int, row_stride: int, sel: torch.Tensor,
         raise_for_status(status, "iqk_mx_routed")
 
 
+def mx_set_error(workspace: torch.Tensor, device: torch.device, stray: torch.Tensor) -> None:
+    """The error word of a routed call that launched no product: whether an index was
+    ``stray``, as ``iqk_mx_routed`` leaves it."""
+    check_mx_workspace(workspace, device)
+    if workspace.numel() < 16 or workspace.data_ptr() % 16:
+        raise IqkRuntimeError("workspace must hold an error word on a 16-byte boundary")
+    words = workspace[:16].view(torch.int32)
+    words.zero_()
+    words[0] = stray * DEVERR_EXPERT
+
+
 def mx_read_error(workspace: torch.Tensor) -> int:
     """``iqk_mx_read_error``: the device error bits of a routed product's workspace."""
     check_mx_workspace(workspace)

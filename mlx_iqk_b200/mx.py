@@ -216,11 +216,12 @@ def mx_switch_linear(x, indices, codes, scales, out_dtype: torch.dtype | None = 
             f"{pairs} token-expert pairs do not tile {count} activation "
             f"row(s); the operand and the routing disagree")
     y = x.new_empty((*indices.shape, 1, out), dtype=_out_dtype(x, out_dtype))
-    if pairs and out:
-        if experts == 0:
-            return y.zero_()
+    if pairs and out and experts:
         K.mx_routed(rows, count, step, sel, codes, scales, stride, y, workspace)
-    return y
+        return y
+    if workspace is not None:  # no product to leave the error word
+        K.mx_set_error(workspace, y.device, ((sel < -1) | (sel >= experts)).any())
+    return y.zero_()
 
 
 class MxSwitchGLU(nn.Module):

@@ -534,3 +534,25 @@ def test_matrices_without_outputs(cuda):
                  (codes[:, :0].contiguous(), scales[:, :0].contiguous())):
         assert mx_switch_linear(x, idx, c, s).shape == (2, 2, 1, 0)
         assert mx_dequantize(c, s).shape == (3, 0, 64)
+
+
+@pytest.mark.gpu
+def test_error_word_of_calls_without_a_product(cuda):
+    """Calls that launch no product leave an error word all the same, of their own
+    indices and not of what the workspace held."""
+    x = make_x((2, 1, 1, 64), torch.float32, seed=1)
+    codes, scales, _ = make_matrix((3, 32, 64), seed=2)
+    stray = torch.tensor([[0, 7], [2, -1]], dtype=torch.int32, device="cuda")
+    none = torch.full((2, 2), -1, dtype=torch.int32, device="cuda")
+    cases = [(x[:0], stray[:0], codes, scales, 0), (x, stray, codes[:, :0], scales[:, :0], 1),
+             (x, stray.clamp(max=2), codes[:, :0], scales[:, :0], 0),
+             (x, stray, codes[:0], scales[:0], 1), (x, none, codes[:0], scales[:0], 0)]
+    for rows, idx, c, s, want in cases:
+        ws = torch.full((K.mx_workspace_bytes(4, 3, 64, 32),), 255, dtype=torch.uint8,
+                        device="cuda")
+        y = mx_switch_linear(rows, idx, c, s, workspace=ws)
+        assert y.shape == (*idx.shape, 1, c.shape[1]) and (y == 0).all()
+        assert K.mx_read_error(ws) == want * K.DEVERR_EXPERT
+    with pytest.raises(K.IqkRuntimeError, match="workspace"):
+        mx_switch_linear(x[:0], none[:0], codes, scales,
+                         workspace=torch.empty(1 << 20, dtype=torch.uint8))
